@@ -597,6 +597,54 @@ int myelin_linear_lif_fwd_narrow_bits(const int32_t *words, const float *w,
                                       int rule, int precision,
                                       myelin_stream_t stream);
 
+/*
+ * Log probabilities of given tokens, with the entropy of each row's
+ * distribution and its top alternatives.  logits [R, V], rows of unit stride
+ * and row stride ld elements, dtype 0 (fp32) or 2 (bf16); targets [R] int64 or
+ * NULL (no given tokens, log_probs unused).  Outputs fp32: log_probs [R],
+ * entropy [R], stats [2, R] (each row's maximum and the logarithm of its sum of
+ * exponentials below it, kept for the backward pass) and, for top > 0 (at most
+ * min(64, V)), top_log_probs [R, top] with top_tokens [R, top] int64, largest
+ * first, equal logits by the lower index.
+ *   - a row whose target is ignore_index is not read: 0, 0, -inf, -1;
+ *   - any other target outside [0, V) gives log_probs NaN;
+ *   - a row of nothing but -inf: log_probs -inf, entropy 0.
+ * workspace: myelin_token_log_probs_workspace_bytes (host only; 0 where a row
+ * is not split over workgroups), 16-byte aligned.
+ * The backward pass takes the gradients of log_probs and of entropy (either
+ * may be NULL) and writes grad_logits [R, V], contiguous, in the logits' type.
+ * No counterpart in myelin.
+ */
+int64_t myelin_token_log_probs_workspace_bytes(int64_t R, int64_t V, int top);
+int myelin_token_log_probs(const void *logits, int dtype, int64_t ld,
+                           const int64_t *targets, int64_t ignore_index,
+                           float *log_probs, float *entropy, float *stats,
+                           float *top_log_probs, int64_t *top_tokens, int64_t R,
+                           int64_t V, int top, void *workspace,
+                           int64_t workspace_bytes, myelin_stream_t stream);
+int myelin_token_log_probs_bwd(const void *logits, int dtype, int64_t ld,
+                               const int64_t *targets, int64_t ignore_index,
+                               const float *stats, const float *entropy,
+                               const float *grad_log_probs,
+                               const float *grad_entropy, void *grad_logits,
+                               int64_t R, int64_t V, myelin_stream_t stream);
+
+/*
+ * Dropout from a counter-based generator; the mask is never stored.  x, y and
+ * residual (or NULL) are [steps, n] contiguous, dtype 0 (fp32) or 2 (bf16).
+ * Mask element i (of n, the same for every step) is kept where word i % 4 of
+ * Philox 4x32-10 at the counter (i / 4, offset) and key seed is >= threshold:
+ *   y = x * scale (+ residual) where kept, 0 (+ residual) elsewhere.
+ * offset is the sum of the argument and of *offset_at (device memory, or
+ * NULL), so that a captured graph can advance it.  The backward pass is the
+ * same call on the gradient, without residual.
+ * No counterpart in myelin (modules.py uses torch's dropout).
+ */
+int myelin_counter_dropout(const void *x, int dtype, const void *residual,
+                           void *y, int64_t steps, int64_t n, int64_t threshold,
+                           float scale, int64_t seed, int64_t offset,
+                           const int64_t *offset_at, myelin_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

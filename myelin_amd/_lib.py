@@ -84,6 +84,9 @@ SIGNATURES: dict[str, list] = {
     "myelin_col_sum_f32": [_P, _P, _I64, _I64, _INT, _P],
     "myelin_lif_currents_fwd": [_P] * 9 + [_I64] * 8 + [_F] * 4 + [_INT, _P],
     "myelin_linear_lif_fwd_narrow_bits": [_P] * 8 + [_I64] * 6 + [_F] * 4 + [_INT, _INT, _P],
+    "myelin_token_log_probs": [_P, _INT, _I64, _P, _I64] + [_P] * 5 + [_I64, _I64, _INT, _P, _I64, _P],
+    "myelin_token_log_probs_bwd": [_P, _INT, _I64, _P, _I64] + [_P] * 5 + [_I64, _I64, _P],
+    "myelin_counter_dropout": [_P, _INT, _P, _P, _I64, _I64, _I64, _F, _I64, _I64, _P, _P],
 }
 
 _lock = threading.Lock()
@@ -114,6 +117,8 @@ def load() -> ctypes.CDLL:
             lib.myelin_gemm_workspace_elems.restype = ctypes.c_int64
             lib.myelin_narrow_bits_fits.argtypes = [_I64, _I64, _INT]
             lib.myelin_narrow_bits_fits.restype = ctypes.c_int
+            lib.myelin_token_log_probs_workspace_bytes.argtypes = [_I64, _I64, _INT]
+            lib.myelin_token_log_probs_workspace_bytes.restype = ctypes.c_int64
             for name, argtypes in SIGNATURES.items():
                 fn = getattr(lib, name)
                 fn.argtypes = argtypes

@@ -1,0 +1,134 @@
+"""Dropout from a counter-based generator (``csrc/dropout.hip``).
+
+The mask is a function of ``(seed, offset, element)``: the backward pass
+computes it again, so a training step stores none, and the same call gives the
+same mask on any layout, device or stream.  Spiking layers usually keep one
+mask for all time steps of a sample (``time_shared=True``).
+"""
+
+from __future__ import annotations
+
+from typing import Any
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from myelin_amd import _lib
+from myelin_amd.packing import _device_of
+
+_TYPES = (torch.float32, torch.bfloat16)
+
+
+def _launch(x, residual, steps, threshold, scale, seed, offset):
+    y = torch.empty_like(x)
+    at = offset if isinstance(offset, torch.Tensor) else None
+    with _device_of(x):
+        _lib.call("myelin_counter_dropout", x.data_ptr(), _lib.DT[x.dtype], _lib.ptr(residual), y.data_ptr(), steps,
+                  x.numel() // steps if steps else 0, threshold, scale, seed, 0 if at is not None else offset,
+                  _lib.ptr(at), _lib.stream(x.device))
+    return y
+
+
+class HipCounterDropoutFunction(torch.autograd.Function):
+    """``dx`` is the dropout of the gradient with the same mask, which is
+    computed again; the residual's gradient is the gradient itself."""
+
+    @staticmethod
+    def forward(ctx: Any, x, residual, steps, threshold, scale, seed, offset):
+        ctx.set_materialize_grads(False)
+        ctx.meta = (steps, threshold, scale, seed)
+        if isinstance(offset, torch.Tensor):
+            ctx.save_for_backward(offset)
+            ctx.offset = None
+        else:
+            ctx.offset = offset
+        return _launch(x, residual, steps, threshold, scale, seed, offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, g):
+        gx = None
+        if g is not None and ctx.needs_input_grad[0]:
+            offset = ctx.saved_tensors[0] if ctx.offset is None else ctx.offset
+            gx = _launch(g.contiguous(), None, *ctx.meta, offset)
+        return gx, g if ctx.needs_input_grad[1] else None, None, None, None, None, None
+
+
+def counter_dropout(
+    x: torch.Tensor,
+    p: float,
+    seed: int,
+    offset: int | torch.Tensor = 0,
+    *,
+    residual: torch.Tensor | None = None,
+    time_shared: bool = False,
+) -> torch.Tensor:
+    """``x / (1 - p)`` with probability ``1 - p``, else 0; plus ``residual``.
+
+    ``x`` (and ``residual``, of its shape and type) is float32 or bfloat16; the
+    sum is formed in float32 and rounded once.  Calls that must not share a
+    mask differ in ``seed`` or ``offset``; ``offset`` may be an int64 device
+    tensor of one element, so that a captured graph can advance it (it must
+    then stay unchanged until the backward pass has run).  ``time_shared``
+    takes dimension 0 as time and uses one mask for all of it.
+
+    Mask element ``i`` (row-major) is word ``i % 4`` of Philox 4x32-10 at the
+    counter ``(i // 4, offset)`` and key ``seed``; it keeps where the word is at
+    least ``floor(p * 2**32)``.  Dropped NaNs and infinities are dropped.
+    """
+
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must be in [0, 1]; got {p}")
+    if not 0 <= seed < 2**63:
+        raise ValueError("seed must be in [0, 2**63)")
+    _lib.require_device(x, "x")
+    if x.dtype not in _TYPES:
+        raise ValueError(f"x must be float32 or bfloat16; got {x.dtype}")
+    if time_shared and x.ndim == 0:
+        raise ValueError("time_shared needs a time dimension")
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must match x; got {tuple(residual.shape)} and {tuple(x.shape)}")
+        if residual.device != x.device or residual.dtype != x.dtype:
+            raise ValueError("residual must have the device and dtype of x")
+        residual = residual.contiguous()
+    if isinstance(offset, torch.Tensor):
+        if offset.numel() != 1 or offset.dtype != torch.int64 or offset.device != x.device:
+            raise ValueError("an offset tensor must hold one int64 on the device of x")
+    elif not 0 <= offset < 2**63:
+        raise ValueError("offset must be in [0, 2**63)")
+    x = x.contiguous()
+    steps = x.shape[0] if time_shared else 1
+    threshold = int(p * 2**32)
+    scale = 0.0 if p == 1.0 else 1.0 / (1.0 - p)
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return HipCounterDropoutFunction.apply(x, residual, steps, threshold, scale, seed, offset)
+    return _launch(x, residual, steps, threshold, scale, seed, offset)
+
+
+class CounterDropout(nn.Module):
+    """``counter_dropout`` with a new mask for each training call.
+
+    The count of calls is a buffer (``offset``), saved with the module and
+    advanced on the device, so that a captured training step draws a new mask at
+    each replay.  In evaluation mode the input passes, plus ``residual``.
+    """
+
+    def __init__(self, p: float, seed: int = 0, time_shared: bool = False) -> None:
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must be in [0, 1]; got {p}")
+        self.p = p
+        self.seed = seed
+        self.time_shared = time_shared
+        self.register_buffer("offset", torch.zeros(1, dtype=torch.int64))
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        if not self.training:
+            return x if residual is None else x + residual
+        # a tensor of this call's own: the backward pass reads it again
+        offset = self.offset + 1
+        self.offset.copy_(offset)
+        return counter_dropout(x, self.p, self.seed, offset, residual=residual, time_shared=self.time_shared)

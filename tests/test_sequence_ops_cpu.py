@@ -1,0 +1,65 @@
+"""Host-side behaviour of the sequence-model operators: no CPU fallback, entry
+points that check their arguments without launching."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import myelin_amd as myelin
+from myelin_amd import _lib
+
+
+def test_cpu_tensors_are_rejected():
+    x = torch.zeros(3, 4)
+    with pytest.raises(ValueError, match="ROCm device"):
+        myelin.counter_dropout(x, 0.5, 0)
+    with pytest.raises(ValueError, match="ROCm device"):
+        myelin.token_log_probs(x, torch.zeros(3, dtype=torch.int64))
+
+
+def test_log_probs_entry_points_validate():
+    f = "myelin_token_log_probs"
+    # logits, dtype, ld, targets, ignore, lp, entropy, lse, top_lp, top_tok, R, V, top, ws, bytes, stream
+    ok = [16, 0, 10, None, -100, None, 16, 16, None, None, 4, 10, 0, None, 0, None]
+
+    def bad(**kw):
+        at = dict(logits=0, dtype=1, ld=2, targets=3, lp=5, entropy=6, top_lp=8, R=10, V=11, top=12, ws=13)
+        args = list(ok)
+        for k, v in kw.items():
+            args[at[k]] = v
+        return args
+
+    for kw, message in ((dict(dtype=1), "unsupported dtype"), (dict(R=-1), "non-negative"), (dict(V=0), "V positive"),
+                        (dict(V=2**31, ld=2**31), "below 2"), (dict(ld=9), "row stride"),
+                        (dict(logits=None), "null pointer"), (dict(entropy=None), "null pointer"),
+                        (dict(targets=16), "null pointer"), (dict(top=11), "top must be"),
+                        (dict(top=3), "null pointer"), (dict(V=100000, ld=100000), "workspace of")):
+        with pytest.raises(ValueError, match=message):
+            _lib.call(f, *bad(**kw))
+    assert _lib.load().myelin_token_log_probs(*bad(R=0)) == 0
+    g = "myelin_token_log_probs_bwd"
+    with pytest.raises(ValueError, match="null pointer"):
+        _lib.call(g, 16, 0, 10, None, -100, None, 16, None, None, 16, 4, 10, None)
+    with pytest.raises(ValueError, match="row stride"):
+        _lib.call(g, 16, 0, 9, None, -100, 16, 16, None, None, 16, 4, 10, None)
+
+
+def test_log_probs_workspace_is_for_split_rows_only():
+    need = _lib.load().myelin_token_log_probs_workspace_bytes
+    assert need(12800, 10, 0) == 0 and need(8192, 32768, 0) == 0
+    assert need(1, 4096, 5) == 0  # one tile
+    assert need(1, 100000, 0) == 25 * 16 and need(1, 100000, 20) == 25 * (16 + 160)
+
+
+def test_dropout_entry_point_validates():
+    f = "myelin_counter_dropout"
+    with pytest.raises(ValueError, match="unsupported dtype"):
+        _lib.call(f, 16, 5, None, 16, 1, 8, 0, 1.0, 0, 0, None, None)
+    with pytest.raises(ValueError, match="negative size"):
+        _lib.call(f, 16, 0, None, 16, 1, -8, 0, 1.0, 0, 0, None, None)
+    with pytest.raises(ValueError, match="threshold must be"):
+        _lib.call(f, 16, 0, None, 16, 1, 8, 2**32 + 1, 1.0, 0, 0, None, None)
+    with pytest.raises(ValueError, match="null pointer"):
+        _lib.call(f, 16, 0, None, None, 1, 8, 0, 1.0, 0, 0, None, None)
+    assert _lib.load().myelin_counter_dropout(None, 0, None, None, 0, 8, 0, 1.0, 0, 0, None, None) == 0
