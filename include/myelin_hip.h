@@ -645,6 +645,53 @@ int myelin_counter_dropout(const void *x, int dtype, const void *residual,
                            float scale, int64_t seed, int64_t offset,
                            const int64_t *offset_at, myelin_stream_t stream);
 
+/*
+ * Linear attention with a decay for each head:
+ *   S_t = decay[h] S_{t-1} + k_t v_t^T,  o_t = scale S_t^T q_t
+ * q [T, B, H, Dk], k [T, B, Hk, Dk], v [T, B, Hk, Dv], dtype 0 (fp32) or 2
+ * (bf16), each with unit stride in its last dimension and element strides of t,
+ * b and head in `strides` (host memory: q's three, k's, v's, and for the
+ * backward pass grad_out's); H a multiple of Hk, query heads h with key/value
+ * head h / (H / Hk); Dk, Dv in [1, 128].  decay [H] fp32 (0 to 1); states
+ * [B, H, Dk, Dv] contiguous fp32, state NULL for zeros; lengths [B] int32 or
+ * NULL: steps of each batch row (taken into [0, T]); later steps keep the state
+ * and give 0, and their inputs are not read.  out, grad_q, grad_k and grad_v
+ * are contiguous in their inputs' shapes and type; scale finite, not 0.
+ * The backward pass takes grad_out and grad_state_out (or NULL) and writes
+ * grad_state (or NULL) with the others.
+ * workspace: myelin_decay_attention_workspace_elems floats (host only).
+ * _step is one step of it (q [B, H, Dk], ..., six strides); state_out may be
+ * state itself.
+ * No counterpart in myelin.
+ */
+int64_t myelin_decay_attention_workspace_elems(int64_t T, int64_t B, int64_t H,
+                                               int64_t Hk, int64_t Dk,
+                                               int64_t Dv, int backward);
+int myelin_decay_attention_fwd(const void *q, const void *k, const void *v,
+                               int dtype, const int64_t *strides,
+                               const float *decay, const float *state,
+                               const int32_t *lengths, void *out,
+                               float *state_out, int64_t T, int64_t B,
+                               int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
+                               float scale, float *workspace,
+                               int64_t workspace_elems, myelin_stream_t stream);
+int myelin_decay_attention_bwd(const void *q, const void *k, const void *v,
+                               const void *grad_out, int dtype,
+                               const int64_t *strides, const float *decay,
+                               const float *state, const int32_t *lengths,
+                               const float *grad_state_out, void *grad_q,
+                               void *grad_k, void *grad_v, float *grad_state,
+                               int64_t T, int64_t B, int64_t H, int64_t Hk,
+                               int64_t Dk, int64_t Dv, float scale,
+                               float *workspace, int64_t workspace_elems,
+                               myelin_stream_t stream);
+int myelin_decay_attention_step(const void *q, const void *k, const void *v,
+                                int dtype, const int64_t *strides,
+                                const float *decay, const float *state,
+                                void *out, float *state_out, int64_t B,
+                                int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
+                                float scale, myelin_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

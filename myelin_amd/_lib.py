@@ -86,6 +86,9 @@ SIGNATURES: dict[str, list] = {
     "myelin_linear_lif_fwd_narrow_bits": [_P] * 8 + [_I64] * 6 + [_F] * 4 + [_INT, _INT, _P],
     "myelin_token_log_probs": [_P, _INT, _I64, _P, _I64] + [_P] * 5 + [_I64, _I64, _INT, _P, _I64, _P],
     "myelin_token_log_probs_bwd": [_P, _INT, _I64, _P, _I64] + [_P] * 5 + [_I64, _I64, _P],
+    "myelin_decay_attention_fwd": [_P] * 3 + [_INT] + [_P] * 6 + [_I64] * 6 + [_F, _P, _I64, _P],
+    "myelin_decay_attention_bwd": [_P] * 4 + [_INT] + [_P] * 9 + [_I64] * 6 + [_F, _P, _I64, _P],
+    "myelin_decay_attention_step": [_P] * 3 + [_INT] + [_P] * 5 + [_I64] * 5 + [_F, _P],
     "myelin_counter_dropout": [_P, _INT, _P, _P, _I64, _I64, _I64, _F, _I64, _I64, _P, _P],
 }
 
@@ -119,6 +122,8 @@ def load() -> ctypes.CDLL:
             lib.myelin_narrow_bits_fits.restype = ctypes.c_int
             lib.myelin_token_log_probs_workspace_bytes.argtypes = [_I64, _I64, _INT]
             lib.myelin_token_log_probs_workspace_bytes.restype = ctypes.c_int64
+            lib.myelin_decay_attention_workspace_elems.argtypes = [_I64] * 6 + [_INT]
+            lib.myelin_decay_attention_workspace_elems.restype = ctypes.c_int64
             for name, argtypes in SIGNATURES.items():
                 fn = getattr(lib, name)
                 fn.argtypes = argtypes

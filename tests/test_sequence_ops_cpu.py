@@ -63,3 +63,37 @@ def test_dropout_entry_point_validates():
     with pytest.raises(ValueError, match="null pointer"):
         _lib.call(f, 16, 0, None, None, 1, 8, 0, 1.0, 0, 0, None, None)
     assert _lib.load().myelin_counter_dropout(None, 0, None, None, 0, 8, 0, 1.0, 0, 0, None, None) == 0
+
+
+def test_attention_rejects_cpu_tensors():
+    q, d = torch.zeros(3, 2, 2, 4), torch.ones(2)
+    with pytest.raises(ValueError, match="ROCm device"):
+        myelin.decay_attention(q, q, q, d)
+    with pytest.raises(ValueError, match="ROCm device"):
+        myelin.decay_attention_step(q[0], q[0], q[0], d, torch.zeros(2, 2, 4, 4))
+
+
+def test_attention_entry_points_validate():
+    sizes = dict(T=4, B=2, H=4, Hk=2, Dk=8, Dv=8)
+
+    def fwd(q=16, dtype=0, scale=1.0, **kw):
+        z = {**sizes, **kw}
+        _lib.call("myelin_decay_attention_fwd", q, 16, 16, dtype, 16, 16, None, None, 16, 16, *z.values(), scale, None,
+                  0, None)
+
+    for kw, message in ((dict(dtype=3), "unsupported dtype"), (dict(T=0), "positive"), (dict(B=-1), "positive"),
+                        (dict(H=3), "multiple of Hk"), (dict(Dk=129), "Dk and Dv"), (dict(Dv=0), "Dk and Dv"),
+                        (dict(scale=0.0), "not be zero"), (dict(scale=float("nan")), "not be zero"),
+                        (dict(scale=float("inf")), "finite"), (dict(T=2**31), "too many"),
+                        (dict(q=None), "null pointer")):
+        with pytest.raises(ValueError, match=message):
+            fwd(**kw)
+    fwd(q=None, B=0)  # nothing to do
+    bwd = ("myelin_decay_attention_bwd", 16, 16, 16, 16, 0, 16, 16, None, None, None, 16, 16, 16, None)
+    with pytest.raises(ValueError, match="workspace of"):
+        _lib.call(*bwd, *sizes.values(), 1.0, None, 0, None)
+    step = ("myelin_decay_attention_step", 16, 16, 16, 0, 16, 16)
+    with pytest.raises(ValueError, match="null pointer"):
+        _lib.call(*step, None, 16, 16, 2, 4, 2, 8, 8, 1.0, None)
+    with pytest.raises(ValueError, match="Dk and Dv"):
+        _lib.call(*step, 16, 16, 16, 2, 4, 2, 8, 200, 1.0, None)
