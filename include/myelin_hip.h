@@ -659,14 +659,16 @@ int myelin_counter_dropout(const void *x, int dtype, const void *residual,
  * are contiguous in their inputs' shapes and type; scale finite, not 0.
  * The backward pass takes grad_out and grad_state_out (or NULL) and writes
  * grad_state (or NULL) with the others.
- * workspace: myelin_decay_attention_workspace_elems floats (host only).
+ * workspace: myelin_decay_attention_workspace_elems floats (host only), 16-byte
+ * aligned.
  * _step is one step of it (q [B, H, Dk], ..., six strides); state_out may be
  * state itself.
  * No counterpart in myelin.
  */
-int64_t myelin_decay_attention_workspace_elems(int64_t T, int64_t B, int64_t H,
-                                               int64_t Hk, int64_t Dk,
-                                               int64_t Dv, int backward);
+int64_t myelin_decay_attention_workspace_elems(int dtype, int64_t T, int64_t B,
+                                               int64_t H, int64_t Hk,
+                                               int64_t Dk, int64_t Dv,
+                                               int backward);
 int myelin_decay_attention_fwd(const void *q, const void *k, const void *v,
                                int dtype, const int64_t *strides,
                                const float *decay, const float *state,

@@ -122,7 +122,7 @@ def load() -> ctypes.CDLL:
             lib.myelin_narrow_bits_fits.restype = ctypes.c_int
             lib.myelin_token_log_probs_workspace_bytes.argtypes = [_I64, _I64, _INT]
             lib.myelin_token_log_probs_workspace_bytes.restype = ctypes.c_int64
-            lib.myelin_decay_attention_workspace_elems.argtypes = [_I64] * 6 + [_INT]
+            lib.myelin_decay_attention_workspace_elems.argtypes = [_INT] + [_I64] * 6 + [_INT]
             lib.myelin_decay_attention_workspace_elems.restype = ctypes.c_int64
             for name, argtypes in SIGNATURES.items():
                 fn = getattr(lib, name)

@@ -39,9 +39,9 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _workspace(sizes, backward, device):
-    n = _lib.load().myelin_decay_attention_workspace_elems(*sizes, backward)
-    return (torch.empty(n, dtype=torch.float32, device=device) if n else None), n
+def _workspace(q, sizes, backward):
+    n = _lib.load().myelin_decay_attention_workspace_elems(_lib.DT[q.dtype], *sizes, backward)
+    return (torch.empty(n, dtype=torch.float32, device=q.device) if n else None), n
 
 
 def _forward(q, k, v, decay, state, lengths, scale):
@@ -51,7 +51,7 @@ def _forward(q, k, v, decay, state, lengths, scale):
     out = torch.empty((T, B, H, Dv), dtype=q.dtype, device=dev)
     final = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=dev)
     sizes = (T, B, H, Hk, Dk, Dv)
-    ws, n = _workspace(sizes, 0, dev)
+    ws, n = _workspace(q, sizes, 0)
     with _device_of(q):
         _lib.call("myelin_decay_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.DT[q.dtype],
                   _strides(q, k, v), decay.data_ptr(), _lib.ptr(state), _lib.ptr(lengths), out.data_ptr(),
@@ -87,7 +87,7 @@ class HipDecayAttentionFunction(torch.autograd.Function):
         want_state = ctx.needs_input_grad[4]
         g_state = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=dev) if want_state else None
         sizes = (T, B, H, Hk, Dk, Dv)
-        ws, n = _workspace(sizes, 1, dev)
+        ws, n = _workspace(q, sizes, 1)
         with _device_of(q):
             _lib.call("myelin_decay_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), g_out.data_ptr(),
                       _lib.DT[q.dtype], _strides(q, k, v, g_out), decay.data_ptr(), _lib.ptr(state),

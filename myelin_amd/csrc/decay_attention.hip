@@ -21,11 +21,75 @@ using myelin::kWave;
 
 constexpr int kMaxDim = 128;
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+
+// Operand fragments of 16 x 16 products reduced over 32 indices: a lane l has
+// row (or column) l % 16 and, with g = l / 16, the indices 4 g .. 4 g + 3 of
+// each half.  A product's result has column l % 16 and rows 4 g .. 4 g + 3, so
+// two results are a fragment of the transposed product as they are.
 struct F32 {
   using T = float;
+  using Frag = f32x8;
+  static constexpr int VEC = 4;      // elements of 16 bytes
+  static constexpr int C = 32;       // steps of a chunk
+  static constexpr int PARTS = 1;  // fragments that hold an fp32 value
+  // v in PARTS or fewer parts, each the rounded rest of those before
+  template <int N>
+  __device__ static void put(Frag (&part)[N], int i, float v) {
+    part[0][i] = v;
+  }
+  __device__ static void mma(f32x4 &acc, const Frag &a, const Frag &b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
+  }
+  // rows: element `at` of this lane's row and 16 on
+  __device__ static Frag row(const T *at) {
+    const f32x4 a = *reinterpret_cast<const f32x4 *>(at), b = *reinterpret_cast<const f32x4 *>(at + 16);
+    return {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+  // columns: of the matrix of row length ld at `base`, column l % 16 and rows
+  // 4 g .. 4 g + 3 and 16 on
+  __device__ static Frag column(const T *base, int ld, int lane) {
+    const T *p = base + (lane >> 4) * 4 * ld + (lane & 15);
+    return {p[0], p[ld], p[2 * ld], p[3 * ld], p[16 * ld], p[17 * ld], p[18 * ld], p[19 * ld]};
+  }
 };
 struct BF16 {
   using T = __bf16;
+  using Frag = bf16x8;
+  static constexpr int VEC = 8;
+  static constexpr int C = 64;
+  static constexpr int PARTS = 3;
+  template <int N>
+  __device__ static void put(Frag (&part)[N], int i, float v) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      part[k][i] = static_cast<__bf16>(v);
+      v -= static_cast<float>(part[k][i]);
+    }
+  }
+  __device__ static void mma(f32x4 &acc, const Frag &a, const Frag &b) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
+  }
+  __device__ static Frag row(const T *at) {
+    const bf16x4 a = *reinterpret_cast<const bf16x4 *>(at), b = *reinterpret_cast<const bf16x4 *>(at + 16);
+    return {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
+  // the transposing read: lane r of a group of 16 points at row r / 4 and
+  // columns 4 (r % 4) .. + 3 of a 4 x 16 block, lane i receives column i
+  __device__ static Frag column(const T *base, int ld, int lane) {
+    const T *p = base + ((lane >> 4) * 4 + ((lane & 15) >> 2)) * ld + (lane & 3) * 4;
+    const bf16x4 a = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)((lds_void *)p)));
+    const bf16x4 b =
+        __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)((lds_void *)(p + 16 * ld))));
+    return {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  }
 };
 
 // One recurrence over [T, B, H] rows; a, b of KD elements and c, o of VD, each
@@ -42,70 +106,313 @@ struct Problem {
   int ga, gb, gc;  // query heads to a head of a, b, c
   float in_scale, out_scale, o_scale;
   int reverse, o_f32;
+  int va, vb, vc, vo;  // rows of whole 16-byte pieces (vo: of 4 elements)
 };
 
 struct Args {
   Problem p[3];
+  int problems;
   const float *decay;
   const int32_t *lengths;
   int64_t T, B, H;
+  int64_t segments, segment;  // of steps, whole chunks
+  float *ends;                // [problems, B * H, segments - 1] states, as the lanes hold them
 };
 
-// The recurrence step by step: a lane has a column of the state.
-template <class E, int KDP>
-__global__ __launch_bounds__(64) void recurrent(Args args) {
-  using T = typename E::T;
-  const Problem &p = args.p[blockIdx.z];
-  __shared__ float sa[KDP], sb[KDP];
-  const int lane = threadIdx.x;
-  const int64_t b = blockIdx.x / args.H, h = blockIdx.x % args.H;
-  const int v = blockIdx.y * 64 + lane;
-  if (static_cast<int>(blockIdx.y) * 64 >= p.VD) return;
-  const bool on = v < p.VD;
-  const float d = args.decay[h];
-  int64_t n = args.T;
-  if (args.lengths) {
-    n = args.lengths[b];
-    n = n < 0 ? 0 : n > args.T ? args.T : n;
+__device__ __forceinline__ int64_t steps_of(const Args &a, int64_t b) {
+  if (!a.lengths) return a.T;
+  const int64_t n = a.lengths[b];
+  return n < 0 ? 0 : n > a.T ? a.T : n;
+}
+
+// d^n, by squaring in double: 0^0 = 1
+__device__ __forceinline__ float power(float d, int64_t n) {
+  double p = 1.0, s = d;
+  for (; n > 0; n >>= 1) {
+    if (n & 1) p *= s;
+    s *= s;
   }
+  return static_cast<float>(p);
+}
+
+// The recurrence by chunks of C steps.  With X the state before a chunk (after
+// it, reversed), rows i, j of the chunk in the order of the recurrence and e =
+// 1 - reverse:
+//   o_i = d^(i + e) a_i X + sum_{j <= i} d^(i - j) (a_i . b_j) c_j
+//   X'  = d^C X + sum_j d^(C - j - e) b_j c_j^T
+// A workgroup has one (problem, b, h) and a segment of its steps; wave w has
+// columns 16 w .. 16 w + 15 of X in the accumulators of its products, which are
+// also, rounded, the operand of the next chunk's a X.  The 16 x 16 blocks of a
+// b^T are formed transposed, scaled and used as they stand.  C is 64 for bf16
+// and 32 for fp32, whose product with a b^T costs more than its share.
+//
+// Roundings to bf16: the scaled a b^T (then multiplied by the bf16 c, whose
+// products are exact) to one, as good as the result's own; X where it is an
+// operand to two, 16 bits; the scaled c of the state's sum, an fp32 result, to
+// three, which are fp32's 24 bits.
+template <class E, int KT, int NT, bool STATE_ONLY>
+__global__ __launch_bounds__(NT) void chunked(Args args) {
+  using T = typename E::T;
+  using Frag = typename E::Frag;
+  constexpr int C = E::C, VEC = E::VEC, CT = C / 16, CF = C / 32, KF = KT / 2;
+  constexpr int KD = 16 * KT, VD = NT / 4;           // padded
+  constexpr int LK = KD + 16 / sizeof(T), LV = VD + 16 / sizeof(T);  // row lengths in LDS
+  constexpr int PK = KD / VEC, PV = VD / VEC;                        // pieces of a row
+  constexpr int NK = C * PK / NT, NV = C * PV / NT;                  // pieces of a thread
+  static_assert(C * PK % NT == 0 && C * PV % NT == 0, "whole pieces");
+  typedef T piece __attribute__((ext_vector_type(VEC)));
+  __shared__ __attribute__((aligned(16))) T sa[STATE_ONLY ? 1 : C * LK];
+  __shared__ __attribute__((aligned(16))) T sb[C * LK];
+  __shared__ __attribute__((aligned(16))) T sc[C * LV];
+  __shared__ float pw[C + 1];
+
+  // workgroups of one (b, h) run on one XCD, whose L2 the problems share
+  const uint32_t id = blockIdx.x, rest = id >> 3;
+  const Problem &p = args.p[rest % args.problems];
+  const int64_t heads = (args.B * args.H + 7) / 8, r2 = rest / args.problems;
+  const int64_t bh = (r2 % heads) * 8 + (id & 7), seg = r2 / heads;
+  if (bh >= args.B * args.H) return;
+  const int64_t b = bh / args.H, h = bh % args.H;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, l16 = lane & 15;
+  const float d = args.decay[h];
+  const int64_t n = steps_of(args, b);
   const T *pa = static_cast<const T *>(p.a) + b * p.ab + (h / p.ga) * p.ah;
   const T *pb = static_cast<const T *>(p.b) + b * p.bb + (h / p.gb) * p.bh;
   const T *pc = static_cast<const T *>(p.c) + b * p.cb + (h / p.gc) * p.ch;
-  const int64_t state = (b * args.H + h) * p.KD * p.VD;
-  float X[KDP];
+  const int64_t begin = seg * args.segment;
+  const int64_t end = begin + args.segment < args.T ? begin + args.segment : args.T;
+  const int e = 1 - p.reverse;
+  const bool active = 16 * w < p.VD;  // this wave has columns
+
+  if (tid <= C) pw[tid] = power(d, tid);
+
+  // pieces of rows r0 .. r0 + C - 1 (in the recurrence's order) of one operand
+  auto fetch = [&](piece *to, const T *from, int64_t stride, int width, bool whole, int per_row, int count, int64_t r0) {
 #pragma unroll
-  for (int k = 0; k < KDP; ++k)
-    X[k] = (p.s_in && on && k < p.KD) ? p.s_in[state + k * p.sk + v * p.sv] * p.in_scale : 0.0f;
-  for (int64_t r = 0; r < args.T; ++r) {
-    const int64_t t = (p.reverse && r < n) ? n - 1 - r : r;
-    const int64_t o = t * p.ot + b * p.ob + h * p.oh + v;
-    float out = 0.0f;
-    if (r < n) {
-      __syncthreads();
-      for (int k = lane; k < KDP; k += 64) {
-        sa[k] = k < p.KD ? static_cast<float>(pa[t * p.at + k]) : 0.0f;
-        sb[k] = k < p.KD ? static_cast<float>(pb[t * p.bt + k]) : 0.0f;
-      }
-      __syncthreads();
-      const float c = on ? static_cast<float>(pc[t * p.ct + v]) : 0.0f;
+    for (int i = 0; i < count; ++i) {
+      const int at = i * NT + tid, row = at / per_row, col = (at % per_row) * VEC;
+      const int64_t r = r0 + row;
+      const bool on = r < n && r < end;
+      const T *src = from + (p.reverse ? n - 1 - r : r) * stride + col;
+      if (whole) {
+        piece z;
 #pragma unroll
-      for (int k = 0; k < KDP; ++k) {
-        X[k] = __builtin_fmaf(sb[k], c, p.reverse ? X[k] : d * X[k]);
-        out = __builtin_fmaf(sa[k], X[k], out);
-        if (p.reverse) X[k] *= d;
+        for (int q = 0; q < VEC; ++q) z[q] = T(0.0f);
+        if (on && col < width) z = *reinterpret_cast<const piece *>(src);
+        to[i] = z;
+      } else {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) to[i][q] = (on && col + q < width) ? src[q] : T(0.0f);
       }
     }
-    if (on) {
-      if (p.o_f32)
-        static_cast<float *>(p.o)[o] = out * p.o_scale;
-      else
-        static_cast<T *>(p.o)[o] = static_cast<T>(out * p.o_scale);
+  };
+  auto stage = [&](T *to, const piece *from, int per_row, int ld, int count) {
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      const int at = i * NT + tid;
+      *reinterpret_cast<piece *>(to + (at / per_row) * ld + (at % per_row) * VEC) = from[i];
+    }
+  };
+
+  piece na[STATE_ONLY ? 1 : NK], nb[NK], nc[NV];
+  auto prefetch = [&](int64_t r0) {
+    if constexpr (!STATE_ONLY) fetch(na, pa, p.at, p.KD, p.va, PK, NK, r0);
+    fetch(nb, pb, p.bt, p.KD, p.vb, PK, NK, r0);
+    fetch(nc, pc, p.ct, p.VD, p.vc, PV, NV, r0);
+  };
+  prefetch(begin);
+
+  // X: rows 16 t + 4 g + r, column 16 w + l16
+  f32x4 X[KT];
+  const int64_t state = bh * p.KD * p.VD;
+  float *ends = args.ends + ((static_cast<int64_t>(rest % args.problems) * args.B * args.H + bh) * (args.segments - 1)) *
+                                (KD * VD);
+  const int col = 16 * w + l16;
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    if (!STATE_ONLY && seg > 0) {
+      X[t] = *reinterpret_cast<const f32x4 *>(ends + (seg - 1) * (KD * VD) + ((w * KT + t) * 64 + lane) * 4);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = 16 * t + 4 * g + r;
+        X[t][r] = (!STATE_ONLY && p.s_in && k < p.KD && col < p.VD) ? p.s_in[state + k * p.sk + col * p.sv] * p.in_scale
+                                                                  : 0.0f;
+      }
     }
   }
-  if (p.s_out && on) {
+  __syncthreads();
+  // d^(i - j) of a block of a b^T on the diagonal and `k` below it
+  float dec[CT][4];
 #pragma unroll
-    for (int k = 0; k < KDP; ++k)
-      if (k < p.KD) p.s_out[state + k * p.sk + v * p.sv] = X[k] * p.out_scale;
+  for (int r = 0; r < 4; ++r) {
+    const int ij = l16 - 4 * g - r;
+    dec[0][r] = ij >= 0 ? pw[ij] : 0.0f;
+#pragma unroll
+    for (int k = 1; k < CT; ++k) dec[k][r] = pw[16 * k + ij];
+  }
+
+  for (int64_t r0 = begin; r0 < end; r0 += C) {
+    if (r0 >= n) {  // nothing left but zeros to write (the whole workgroup)
+      if constexpr (STATE_ONLY) break;
+      if (active) {
+        for (int i = 0; i < C; i += 4) {
+          const int64_t r = r0 + i + g;
+          if (r < end && col < p.VD) {
+            const int64_t at = r * p.ot + b * p.ob + h * p.oh + col;
+            if (p.o_f32)
+              static_cast<float *>(p.o)[at] = 0.0f;
+            else
+              static_cast<T *>(p.o)[at] = T(0.0f);
+          }
+        }
+      }
+      continue;
+    }
+    const int c = n - r0 < C ? static_cast<int>(n - r0) : C;  // steps of this chunk
+    if constexpr (!STATE_ONLY) stage(sa, na, PK, LK, NK);
+    stage(sb, nb, PK, LK, NK);
+    stage(sc, nc, PV, LV, NV);
+    __syncthreads();
+    if (r0 + C < end) prefetch(r0 + C);
+    if (active) {
+      Frag vf[CF];
+#pragma unroll
+      for (int f = 0; f < CF; ++f) vf[f] = E::column(sc + 32 * f * LV + 16 * w, LV, lane);
+      if constexpr (!STATE_ONLY) {
+        constexpr int XP = E::PARTS < 2 ? E::PARTS : 2;
+        Frag xf[KF][XP];
+#pragma unroll
+        for (int f = 0; f < KF; ++f)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) E::put(xf[f], i, X[2 * f + (i >> 2)][i & 3]);
+#pragma unroll
+        for (int it = 0; it < CT; ++it) {
+          Frag af[KF];
+#pragma unroll
+          for (int f = 0; f < KF; ++f) af[f] = E::row(sa + (16 * it + l16) * LK + 32 * f + 4 * g);
+          // transposed: rows are columns 16 w + 4 g .. of the result, the column its row
+          f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int f = 0; f < KF; ++f)
+#pragma unroll
+            for (int k = 0; k < XP; ++k) E::mma(o, xf[f][k], af[f]);
+          const float lead = pw[16 * it + l16 + e];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[r] *= lead;
+#pragma unroll
+          for (int f = 0; f < CF; ++f) {
+            if (2 * f > it) continue;
+            Frag pf[1];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int jt = 2 * f + half;
+              f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+              if (jt <= it) {
+#pragma unroll
+                for (int q = 0; q < KF; ++q) E::mma(s, E::row(sb + (16 * jt + l16) * LK + 32 * q + 4 * g), af[q]);
+              }
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const float v = jt <= it ? s[r] * dec[jt <= it ? it - jt : 0][r] : 0.0f;
+                E::put(pf, 4 * half + r, v);
+              }
+            }
+            E::mma(o, vf[f], pf[0]);
+          }
+          // row i of the chunk, columns 16 w + 4 g .. + 3
+          const int64_t r = r0 + 16 * it + l16;
+          const int oc = 16 * w + 4 * g;
+          if (r < end) {
+            const int64_t t = (p.reverse && r < n) ? n - 1 - r : r;
+            const int64_t at = t * p.ot + b * p.ob + h * p.oh + oc;
+            if (p.o_f32) {
+              float *to = static_cast<float *>(p.o) + at;
+              if (p.vo && oc < p.VD)
+                *reinterpret_cast<f32x4 *>(to) = o * p.o_scale;
+              else
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  if (oc + q < p.VD) to[q] = o[q] * p.o_scale;
+            } else {
+              T *to = static_cast<T *>(p.o) + at;
+              typedef T four __attribute__((ext_vector_type(4)));
+              four z;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) z[q] = static_cast<T>(o[q] * p.o_scale);
+              if (p.vo && oc < p.VD)
+                *reinterpret_cast<four *>(to) = z;
+              else
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  if (oc + q < p.VD) to[q] = z[q];
+            }
+          }
+        }
+      }
+      // the state: c scaled by d^(c - j - e)
+      Frag vs[CF][E::PARTS];
+#pragma unroll
+      for (int f = 0; f < CF; ++f)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = 32 * f + 16 * (i >> 2) + 4 * g + (i & 3), x = c - j - e;
+          E::put(vs[f], i, static_cast<float>(vf[f][i]) * pw[x > 0 ? x : 0]);
+        }
+      const float fade = pw[c];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) X[t][r] *= fade;
+#pragma unroll
+        for (int f = 0; f < CF; ++f) {
+          const Frag kf = E::column(sb + 32 * f * LK + 16 * t, LK, lane);
+#pragma unroll
+          for (int k = 0; k < E::PARTS; ++k) E::mma(X[t], kf, vs[f][k]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+
+  if (!active) return;
+  if constexpr (STATE_ONLY) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+      *reinterpret_cast<f32x4 *>(ends + seg * (KD * VD) + ((w * KT + t) * 64 + lane) * 4) = X[t];
+  } else if (p.s_out && seg == args.segments - 1 && col < p.VD) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = 16 * t + 4 * g + r;
+        if (k < p.KD) p.s_out[state + k * p.sk + col * p.sv] = X[t][r] * p.out_scale;
+      }
+  }
+}
+
+// Turns the segments' own contributions into the states at their ends: a thread
+// an element of one (problem, b, h).
+template <int KT, int NT>
+__global__ __launch_bounds__(256) void join_segments(Args args) {
+  constexpr int VD = NT / 4, SIZE = 16 * KT * VD;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t bh = blockIdx.y;
+  const Problem &p = args.p[blockIdx.z];
+  const int at = static_cast<int>(i), r = at & 3, lane = (at >> 2) & 63, t = (at >> 8) % KT, w = (at >> 8) / KT;
+  const int k = 16 * t + 4 * (lane >> 4) + r, col = 16 * w + (lane & 15);
+  if (i >= SIZE || 16 * w >= p.VD) return;  // (columns that a wave has no part in were not written)
+  float *x = args.ends + ((blockIdx.z * args.B * args.H + bh) * (args.segments - 1)) * SIZE + at;
+  const float d = args.decay[bh % args.H];
+  const int64_t n = steps_of(args, bh / args.H);
+  float s = (p.s_in && k < p.KD && col < p.VD) ? p.s_in[bh * p.KD * p.VD + k * p.sk + col * p.sv] * p.in_scale : 0.0f;
+  const float whole = power(d, args.segment);
+  for (int64_t seg = 0; seg + 1 < args.segments; ++seg, x += SIZE) {
+    const int64_t left = n - seg * args.segment;
+    const float f = left >= args.segment ? whole : left > 0 ? power(d, left) : 1.0f;
+    s = __builtin_fmaf(f, s, *x);
+    *x = s;
   }
 }
 
@@ -205,18 +512,73 @@ void launch_step(const StepArgs &a, unsigned grid, hipStream_t s) {
   }
 }
 
-template <class E>
-void launch_recurrent(const Args &a, int problems, hipStream_t s) {
-  int kd = 0, vd = 0;
-  for (int i = 0; i < problems; ++i) {
-    kd = a.p[i].KD > kd ? a.p[i].KD : kd;
-    vd = a.p[i].VD > vd ? a.p[i].VD : vd;
+// The padded widths of a call (of its widest problem).
+struct Shape {
+  int kt, nt;
+};
+Shape shape_of(int kd, int vd) { return {kd <= 64 ? 4 : 8, vd <= 64 ? 256 : 512}; }
+
+// Segments of the time axis: as many as give the chip about 512 workgroups,
+// of 4 chunks at least.
+void split(int64_t T, int64_t workgroups, int C, int64_t *segments, int64_t *segment) {
+  const int64_t chunks = (T + C - 1) / C;
+  int64_t n = 512 / workgroups;
+  if (n > chunks / 4) n = chunks / 4;
+  if (n < 1) n = 1;
+  const int64_t per = (chunks + n - 1) / n;
+  *segment = per * C;
+  *segments = (chunks + per - 1) / per;
+}
+
+int chunk_of(int dtype) { return dtype == 0 ? F32::C : BF16::C; }
+
+// Floats of the segments' states.
+int64_t ends_elems(int dtype, int64_t T, int64_t BH, int problems, Shape sh) {
+  int64_t segments, segment;
+  split(T, BH * problems, chunk_of(dtype), &segments, &segment);
+  return (segments - 1) * BH * problems * (16 * sh.kt) * (sh.nt / 4);
+}
+
+template <class E, int KT, int NT>
+void launch_shape(const Args &a, hipStream_t s) {
+  const int64_t heads = (a.B * a.H + 7) / 8 * 8 * a.problems;
+  if (a.segments > 1) {
+    Args before = a;
+    before.segments = a.segments;  // the last segment's end is nobody's start
+    chunked<E, KT, NT, true><<<static_cast<unsigned>(heads * (a.segments - 1)), NT, 0, s>>>(before);
+    const dim3 grid(16 * KT * (NT / 4) / 256, static_cast<unsigned>(a.B * a.H), a.problems);
+    join_segments<KT, NT><<<grid, 256, 0, s>>>(a);
   }
-  const dim3 grid(static_cast<unsigned>(a.B * a.H), (vd + 63) / 64, problems);
-  if (kd <= 64)
-    recurrent<E, 64><<<grid, 64, 0, s>>>(a);
+  chunked<E, KT, NT, false><<<static_cast<unsigned>(heads * a.segments), NT, 0, s>>>(a);
+}
+
+template <class E>
+void launch(Args &a, int problems, float *ends, hipStream_t s) {
+  int kd = 0, vd = 0;
+  a.problems = problems;
+  a.ends = ends;
+  for (int i = 0; i < problems; ++i) {
+    Problem &p = a.p[i];
+    kd = p.KD > kd ? p.KD : kd;
+    vd = p.VD > vd ? p.VD : vd;
+    const auto whole = [](const void *x, int64_t t, int64_t b, int64_t h, int width) {
+      return width % E::VEC == 0 && t % E::VEC == 0 && b % E::VEC == 0 && h % E::VEC == 0 && myelin::aligned(x, 16);
+    };
+    p.va = whole(p.a, p.at, p.ab, p.ah, p.KD);
+    p.vb = whole(p.b, p.bt, p.bb, p.bh, p.KD);
+    p.vc = whole(p.c, p.ct, p.cb, p.ch, p.VD);
+    p.vo = p.VD % 4 == 0 && myelin::aligned(p.o, 16);
+  }
+  split(a.T, a.B * a.H * problems, E::C, &a.segments, &a.segment);
+  const Shape sh = shape_of(kd, vd);
+  if (sh.kt == 4 && sh.nt == 256)
+    launch_shape<E, 4, 256>(a, s);
+  else if (sh.kt == 4)
+    launch_shape<E, 4, 512>(a, s);
+  else if (sh.nt == 256)
+    launch_shape<E, 8, 256>(a, s);
   else
-    recurrent<E, 128><<<grid, 64, 0, s>>>(a);
+    launch_shape<E, 8, 512>(a, s);
 }
 
 int check(const char *what, int dtype, int64_t T, int64_t B, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
@@ -226,9 +588,16 @@ int check(const char *what, int dtype, int64_t T, int64_t B, int64_t H, int64_t 
   if (H % Hk) return myelin::invalid("%s: H must be a multiple of Hk", what);
   if (Dk < 1 || Dk > kMaxDim || Dv < 1 || Dv > kMaxDim)
     return myelin::invalid("%s: Dk and Dv must be in [1, %d]", what, kMaxDim);
-  if (T > 0x7fffffff || B * H > 0x7fffffff) return myelin::invalid("%s: too many rows", what);
+  if (T > 0x7fffffff || B * H > (1 << 28)) return myelin::invalid("%s: too many rows", what);
   if (!(scale > 0.0f) && !(scale < 0.0f)) return myelin::invalid("%s: scale must not be zero", what);
   if (scale - scale != 0.0f) return myelin::invalid("%s: scale must be finite", what);
+  return MYELIN_OK;
+}
+
+int check_workspace(const char *what, const float *workspace, int64_t elems, int64_t need) {
+  if (need && (!workspace || elems < need))
+    return myelin::invalid("%s: workspace of %lld floats needed", what, static_cast<long long>(need));
+  if (need && !myelin::aligned(workspace, 16)) return myelin::invalid("%s: workspace must be 16-byte aligned", what);
   return MYELIN_OK;
 }
 
@@ -250,10 +619,12 @@ Problem problem(const void *a, const int64_t *as, const void *b, const int64_t *
 
 }  // namespace
 
-extern "C" int64_t myelin_decay_attention_workspace_elems(int64_t T, int64_t B, int64_t H, int64_t Hk, int64_t Dk,
-                                                          int64_t Dv, int backward) {
-  if (T < 1 || B < 1 || H < 1 || Hk < 1 || Dk < 1 || Dv < 1) return 0;
-  return backward && H != Hk ? T * B * H * (Dk + Dv) : 0;
+extern "C" int64_t myelin_decay_attention_workspace_elems(int dtype, int64_t T, int64_t B, int64_t H, int64_t Hk,
+                                                          int64_t Dk, int64_t Dv, int backward) {
+  if (T < 1 || B < 1 || H < 1 || Hk < 1 || Dk < 1 || Dv < 1 || Dk > kMaxDim || Dv > kMaxDim) return 0;
+  const int dk = static_cast<int>(Dk), dv = static_cast<int>(Dv), widest = dk > dv ? dk : dv;
+  if (!backward) return ends_elems(dtype, T, B * H, 1, shape_of(dk, dv));
+  return ends_elems(dtype, T, B * H, 3, shape_of(widest, widest)) + (H != Hk ? T * B * H * (Dk + Dv) : 0);
 }
 
 extern "C" int myelin_decay_attention_fwd(const void *q, const void *k, const void *v, int dtype,
@@ -272,10 +643,12 @@ extern "C" int myelin_decay_attention_fwd(const void *q, const void *k, const vo
   p.gb = p.gc = static_cast<int>(H / Hk);
   p.s_in = state, p.s_out = state_out, p.sk = Dv, p.sv = 1;
   p.o_scale = scale;
+  const int64_t need = myelin_decay_attention_workspace_elems(dtype, T, B, H, Hk, Dk, Dv, 0);
+  if (int rc = check_workspace(what, workspace, workspace_elems, need)) return rc;
   if (dtype == 0)
-    launch_recurrent<F32>(a, 1, myelin::as_hip(stream));
+    launch<F32>(a, 1, workspace, myelin::as_hip(stream));
   else
-    launch_recurrent<BF16>(a, 1, myelin::as_hip(stream));
+    launch<BF16>(a, 1, workspace, myelin::as_hip(stream));
   return myelin::launched(what);
 }
 
@@ -290,9 +663,8 @@ extern "C" int myelin_decay_attention_bwd(const void *q, const void *k, const vo
   if (B == 0) return MYELIN_OK;
   if (!q || !k || !v || !grad_out || !strides || !decay || !grad_q || !grad_k || !grad_v)
     return myelin::invalid("%s: null pointer", what);
-  const int64_t need = myelin_decay_attention_workspace_elems(T, B, H, Hk, Dk, Dv, 1);
-  if (need && (!workspace || workspace_elems < need))
-    return myelin::invalid("%s: workspace of %lld floats needed", what, static_cast<long long>(need));
+  const int64_t need = myelin_decay_attention_workspace_elems(dtype, T, B, H, Hk, Dk, Dv, 1);
+  if (int rc = check_workspace(what, workspace, workspace_elems, need)) return rc;
   const int group = static_cast<int>(H / Hk), dk = static_cast<int>(Dk), dv = static_cast<int>(Dv);
   const int64_t *qs = strides, *ks = strides + 3, *vs = strides + 6, *gs = strides + 9;
   Args a{};
@@ -304,8 +676,10 @@ extern "C" int myelin_decay_attention_bwd(const void *q, const void *k, const vo
   pq.s_in = state, pq.sk = 1, pq.sv = Dv;
   // dk = RLA(v, do, scale q), dv = RLA(k, scale q, do), both from dS_T: with
   // the scale taken out of the whole, its share of dS_T is divided by it
-  void *to_k = group > 1 ? static_cast<void *>(workspace) : grad_k;
-  void *to_v = group > 1 ? static_cast<void *>(workspace + T * B * H * Dk) : grad_v;
+  // (the segments' states first: they are read 16 bytes at a time)
+  float *per_head = group > 1 ? workspace + need - T * B * H * (Dk + Dv) : nullptr;
+  void *to_k = group > 1 ? static_cast<void *>(per_head) : grad_k;
+  void *to_v = group > 1 ? static_cast<void *>(per_head + T * B * H * Dk) : grad_v;
   pk = problem(v, vs, grad_out, gs, q, qs, to_k, B, H, dv, dk);
   pk.ga = group;
   pk.s_in = grad_state_out, pk.sk = 1, pk.sv = Dv;
@@ -319,9 +693,9 @@ extern "C" int myelin_decay_attention_bwd(const void *q, const void *k, const vo
   pk.o_f32 = pv.o_f32 = group > 1;
   const hipStream_t s = myelin::as_hip(stream);
   if (dtype == 0)
-    launch_recurrent<F32>(a, 3, s);
+    launch<F32>(a, 3, workspace, s);
   else
-    launch_recurrent<BF16>(a, 3, s);
+    launch<BF16>(a, 3, workspace, s);
   if (group > 1) {
     for (int i = 0; i < 2; ++i) {
       const int D = i ? dv : dk;
