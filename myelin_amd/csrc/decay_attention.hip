@@ -13,6 +13,8 @@
 // for LA(a, b, c): X = d X + b c^T, o = a X, and RLA: X = X + b c^T, o = a X,
 // X = d X.  One kernel computes all four (Problem).
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -21,10 +23,13 @@ using myelin::kWave;
 
 constexpr int kMaxDim = 128;
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
@@ -36,27 +41,29 @@ typedef __attribute__((address_space(3))) void lds_void;
 struct F32 {
   using T = float;
   using Frag = f32x8;
-  static constexpr int VEC = 4;      // elements of 16 bytes
-  static constexpr int C = 32;       // steps of a chunk
+  static constexpr int VEC = 4;    // elements of 16 bytes
+  static constexpr int C = 32;     // steps of a chunk
   static constexpr int PARTS = 1;  // fragments that hold an fp32 value
-  // v in PARTS or fewer parts, each the rounded rest of those before
+  // LDS rows 16 bytes past a multiple of 64 banks: 16 rows' 16-byte pieces are
+  // on distinct banks, and 4 rows 4 apart
+  static constexpr int PAD = 4;
+  __device__ static int at(int row, int col, int ld) { return row * ld + col; }
   template <int N>
-  __device__ static void put(Frag (&part)[N], int i, float v) {
-    part[0][i] = v;
+  __device__ static void parts(Frag (&part)[N], f32x4 a, f32x4 b) {
+    part[0] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
   __device__ static void mma(f32x4 &acc, const Frag &a, const Frag &b) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
   }
-  // rows: element `at` of this lane's row and 16 on
-  __device__ static Frag row(const T *at) {
-    const f32x4 a = *reinterpret_cast<const f32x4 *>(at), b = *reinterpret_cast<const f32x4 *>(at + 16);
+  __device__ static Frag row(const T *p) {
+    const f32x4 a = *reinterpret_cast<const f32x4 *>(p), b = *reinterpret_cast<const f32x4 *>(p + 16);
     return {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
-  // columns: of the matrix of row length ld at `base`, column l % 16 and rows
-  // 4 g .. 4 g + 3 and 16 on
-  __device__ static Frag column(const T *base, int ld, int lane) {
-    const T *p = base + (lane >> 4) * 4 * ld + (lane & 15);
+  // a lane's first row and column of a column block of 32 rows
+  __device__ static int column_row(int lane) { return (lane >> 4) * 4; }
+  __device__ static int column_at(int lane, int ld) { return lane & 15; }
+  __device__ static Frag column(const T *p, int ld) {
     return {p[0], p[ld], p[2 * ld], p[3 * ld], p[16 * ld], p[17 * ld], p[18 * ld], p[19 * ld]};
   }
 };
@@ -66,25 +73,44 @@ struct BF16 {
   static constexpr int VEC = 8;
   static constexpr int C = 64;
   static constexpr int PARTS = 3;
+  // LDS rows 32 bytes past a multiple of 64 banks (an odd multiple of 32 for
+  // the 128-byte rows), so that the transposing read's 8 rows of 32 bytes are
+  // on distinct banks; rows 8 .. 15 of 16 have the two halves of each 32 bytes
+  // exchanged, so that 16 rows' 8-byte pieces are too
+  static constexpr int PAD = 16;
+  __device__ static int at(int row, int col, int ld) { return row * ld + (col ^ (row & 8)); }
+  // a and b in N parts, each the rounded rest of those before
   template <int N>
-  __device__ static void put(Frag (&part)[N], int i, float v) {
+  __device__ static void parts(Frag (&part)[N], f32x4 a, f32x4 b) {
+    float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      part[k][i] = static_cast<__bf16>(v);
-      v -= static_cast<float>(part[k][i]);
+      uint32_t bits[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2 x = {v[2 * i], v[2 * i + 1]};
+        bits[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+        if (k + 1 < N) {
+          v[2 * i] -= __builtin_bit_cast(float, bits[i] << 16);
+          v[2 * i + 1] -= __builtin_bit_cast(float, bits[i] & 0xffff0000u);
+        }
+      }
+      const u32x4 all = {bits[0], bits[1], bits[2], bits[3]};
+      part[k] = __builtin_bit_cast(Frag, all);
     }
   }
   __device__ static void mma(f32x4 &acc, const Frag &a, const Frag &b) {
     acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
   }
-  __device__ static Frag row(const T *at) {
-    const bf16x4 a = *reinterpret_cast<const bf16x4 *>(at), b = *reinterpret_cast<const bf16x4 *>(at + 16);
+  __device__ static Frag row(const T *p) {
+    const bf16x4 a = *reinterpret_cast<const bf16x4 *>(p), b = *reinterpret_cast<const bf16x4 *>(p + 16);
     return {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   }
   // the transposing read: lane r of a group of 16 points at row r / 4 and
   // columns 4 (r % 4) .. + 3 of a 4 x 16 block, lane i receives column i
-  __device__ static Frag column(const T *base, int ld, int lane) {
-    const T *p = base + ((lane >> 4) * 4 + ((lane & 15) >> 2)) * ld + (lane & 3) * 4;
+  __device__ static int column_row(int lane) { return (lane >> 4) * 4 + ((lane & 15) >> 2); }
+  __device__ static int column_at(int lane, int ld) { return at(column_row(lane), (lane & 3) * 4, ld); }
+  __device__ static Frag column(const T *p, int ld) {
     const bf16x4 a = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)((lds_void *)p)));
     const bf16x4 b =
         __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)((lds_void *)(p + 16 * ld))));
@@ -106,7 +132,6 @@ struct Problem {
   int ga, gb, gc;  // query heads to a head of a, b, c
   float in_scale, out_scale, o_scale;
   int reverse, o_f32;
-  int va, vb, vc, vo;  // rows of whole 16-byte pieces (vo: of 4 elements)
 };
 
 struct Args {
@@ -116,7 +141,10 @@ struct Args {
   const int32_t *lengths;
   int64_t T, B, H;
   int64_t segments, segment;  // of steps, whole chunks
-  float *ends;                // [problems, B * H, segments - 1] states, as the lanes hold them
+  // [problems, B * H, segments - 1] states, as the lanes hold them: what each
+  // segment adds, or (joined) the states at their ends
+  float *ends;
+  int joined;
 };
 
 __device__ __forceinline__ int64_t steps_of(const Args &a, int64_t b) {
@@ -142,33 +170,47 @@ __device__ __forceinline__ float power(float d, int64_t n) {
 //   X'  = d^C X + sum_j d^(C - j - e) b_j c_j^T
 // A workgroup has one (problem, b, h) and a segment of its steps; wave w has
 // columns 16 w .. 16 w + 15 of X in the accumulators of its products, which are
-// also, rounded, the operand of the next chunk's a X.  The 16 x 16 blocks of a
-// b^T are formed transposed, scaled and used as they stand.  C is 64 for bf16
-// and 32 for fp32, whose product with a b^T costs more than its share.
+// also, rounded, the operand of the next chunk's a X.  The waves share out the
+// 16 x 16 blocks of a b^T, scale them and put them into LDS.  Everything that
+// reads a chunk's a, b and c comes before the barrier that ends those blocks,
+// so the next chunk's rows, fetched meanwhile, are staged behind it: two
+// barriers a chunk.  C is 64 for bf16 and 32 for fp32.
 //
 // Roundings to bf16: the scaled a b^T (then multiplied by the bf16 c, whose
 // products are exact) to one, as good as the result's own; X where it is an
 // operand to two, 16 bits; the scaled c of the state's sum, an fp32 result, to
 // three, which are fp32's 24 bits.
-template <class E, int KT, int NT, bool STATE_ONLY>
-__global__ __launch_bounds__(NT) void chunked(Args args) {
+//
+// WHOLE: all rows are whole 16-byte pieces.
+
+// Registers bound how many waves a CU holds: with whole rows 8 waves to a
+// workgroup fit 128, so that two of them share it.
+constexpr int waves_per_simd(int waves, bool whole) { return waves == 8 && whole ? 4 : 2; }
+
+template <class E, int KT, int NW, bool WHOLE, bool STATE_ONLY>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, WHOLE)))) void chunked(
+    Args args) {
   using T = typename E::T;
   using Frag = typename E::Frag;
   constexpr int C = E::C, VEC = E::VEC, CT = C / 16, CF = C / 32, KF = KT / 2;
-  constexpr int KD = 16 * KT, VD = NT / 4;           // padded
-  constexpr int LK = KD + 16 / sizeof(T), LV = VD + 16 / sizeof(T);  // row lengths in LDS
-  constexpr int PK = KD / VEC, PV = VD / VEC;                        // pieces of a row
-  constexpr int NK = C * PK / NT, NV = C * PV / NT;                  // pieces of a thread
+  constexpr int NT = 64 * NW, KD = 16 * KT, VD = 16 * NW;             // threads, padded widths
+  constexpr int LK = KD + E::PAD, LV = VD + E::PAD, LP = C + E::PAD;  // row lengths in LDS
+  constexpr int PK = KD / VEC, PV = VD / VEC;                         // pieces of a row
+  constexpr int NK = C * PK / NT, NV = C * PV / NT;                   // pieces of a thread
   static_assert(C * PK % NT == 0 && C * PV % NT == 0, "whole pieces");
   typedef T piece __attribute__((ext_vector_type(VEC)));
+  typedef T four __attribute__((ext_vector_type(4)));
   __shared__ __attribute__((aligned(16))) T sa[STATE_ONLY ? 1 : C * LK];
   __shared__ __attribute__((aligned(16))) T sb[C * LK];
   __shared__ __attribute__((aligned(16))) T sc[C * LV];
-  __shared__ float pw[C + 1];
+  __shared__ __attribute__((aligned(16))) T sp[STATE_ONLY ? 1 : C * LP];  // scaled a b^T
+  __shared__ __attribute__((aligned(16))) float pw[C + 4];                // d^n
+  __shared__ __attribute__((aligned(16))) float weight[C];                // of c_j in a whole chunk
 
   // workgroups of one (b, h) run on one XCD, whose L2 the problems share
   const uint32_t id = blockIdx.x, rest = id >> 3;
-  const Problem &p = args.p[rest % args.problems];
+  const int which = static_cast<int>(rest % args.problems);
+  const Problem &p = args.p[which];
   const int64_t heads = (args.B * args.H + 7) / 8, r2 = rest / args.problems;
   const int64_t bh = (r2 % heads) * 8 + (id & 7), seg = r2 / heads;
   if (bh >= args.B * args.H) return;
@@ -177,242 +219,348 @@ __global__ __launch_bounds__(NT) void chunked(Args args) {
   const int g = lane >> 4, l16 = lane & 15;
   const float d = args.decay[h];
   const int64_t n = steps_of(args, b);
+  // (held in registers: arguments read in the loop cost it a scalar load each)
   const T *pa = static_cast<const T *>(p.a) + b * p.ab + (h / p.ga) * p.ah;
   const T *pb = static_cast<const T *>(p.b) + b * p.bb + (h / p.gb) * p.bh;
   const T *pc = static_cast<const T *>(p.c) + b * p.cb + (h / p.gc) * p.ch;
+  const int64_t at = p.at, bt = p.bt, ct = p.ct, ot = p.ot;
+  const int kd = p.KD, vd = p.VD;
+  const bool o_f32 = p.o_f32;
+  const float o_scale = p.o_scale;
+  char *po = static_cast<char *>(p.o) + (b * p.ob + h * p.oh) * (o_f32 ? 4 : sizeof(T));
   const int64_t begin = seg * args.segment;
   const int64_t end = begin + args.segment < args.T ? begin + args.segment : args.T;
-  const int e = 1 - p.reverse;
-  const bool active = 16 * w < p.VD;  // this wave has columns
+  const int64_t last = n < end ? n : end;  // the segment's steps end here
+  const bool reverse = p.reverse;
+  const bool active = 16 * w < vd;  // this wave has columns
+  const int e = reverse ? 0 : 1;
 
   if (tid <= C) pw[tid] = power(d, tid);
+  if (tid < C) weight[tid] = power(d, C - tid - e);
+  if constexpr (!STATE_ONLY)  // blocks right of the diagonal stay zero
+    for (int i = tid; i < C * LP; i += NT) sp[i] = T(0.0f);
 
-  // pieces of rows r0 .. r0 + C - 1 (in the recurrence's order) of one operand
-  auto fetch = [&](piece *to, const T *from, int64_t stride, int width, bool whole, int per_row, int count, int64_t r0) {
+  // Rows r0 .. r0 + C - 1 (in the recurrence's order) of one operand, `per`
+  // pieces a row, in pieces or (not WHOLE) element by element, a row's to
+  // consecutive lanes.  Rows past the last step and columns past the width are
+  // zero; their loads go to the nearest element that there is (r0 < last, width
+  // > 0).
+  auto fetch = [&](auto per, auto &to, const T *from, int64_t stride, int width, int64_t r0) {
+    constexpr int PER = decltype(per)::value;
+    const int c = last - r0 < C ? static_cast<int>(last - r0) : C;
+    if constexpr (WHOLE) {
+      // a uniform address and 32-bit offsets, of rows back from the chunk's
+      // last one if reversed
+      constexpr int N = C * PER / NT;
+      const int row0 = tid / PER, col = (tid % PER) * VEC;
+      const T *base = from + (reverse ? n - r0 - c : r0) * stride;
+      const int at = col < width ? col : 0;
 #pragma unroll
-    for (int i = 0; i < count; ++i) {
-      const int at = i * NT + tid, row = at / per_row, col = (at % per_row) * VEC;
-      const int64_t r = r0 + row;
-      const bool on = r < n && r < end;
-      const T *src = from + (p.reverse ? n - 1 - r : r) * stride + col;
-      if (whole) {
-        piece z;
+      for (int i = 0; i < N; ++i) {
+        int row = i * (NT / PER) + row0;
+        row = reverse ? c - 1 - row : row;
+        row = row < 0 ? 0 : row >= c ? c - 1 : row;
+        const uint32_t off = (static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) + at) * sizeof(T);
+        to[i] = *reinterpret_cast<const piece *>(reinterpret_cast<const char *>(base) + off);
+      }
+      if (c < C || width < PER * VEC) {
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) z[q] = T(0.0f);
-        if (on && col < width) z = *reinterpret_cast<const piece *>(src);
-        to[i] = z;
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int q = 0; q < VEC; ++q)
+            to[i][q] = (col < width && i * (NT / PER) + row0 < c) ? to[i][q] : T(0.0f);
+      }
+    } else {
+      // a lane's first address, the others whole rows on
+      constexpr int ROW = PER * VEC, N = C * ROW / NT;
+      const int row0 = tid / ROW, col = tid % ROW;
+      const bool in = col < width;
+      const int64_t step = reverse ? -stride : stride;
+      const T *base = from + (reverse ? n - 1 - r0 : r0) * stride;
+      const int at = in ? col : width - 1;
+      if (c == C) {
+        const int64_t mine = row0 * step + at;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const T v = base[i * (NT / ROW) * step + mine];
+          to[i / VEC][i % VEC] = in ? v : T(0.0f);
+        }
       } else {
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) to[i][q] = (on && col + q < width) ? src[q] : T(0.0f);
+        for (int i = 0; i < N; ++i) {
+          const int row = i * (NT / ROW) + row0;
+          const T v = base[(row < c ? row : c - 1) * step + at];
+          to[i / VEC][i % VEC] = (in && row < c) ? v : T(0.0f);
+        }
       }
     }
   };
-  auto stage = [&](T *to, const piece *from, int per_row, int ld, int count) {
+  auto stage = [&](auto per, T *to, const auto &from, int ld) {
+    constexpr int PER = decltype(per)::value, N = C * PER / NT;
+    if constexpr (WHOLE) {
 #pragma unroll
-    for (int i = 0; i < count; ++i) {
-      const int at = i * NT + tid;
-      *reinterpret_cast<piece *>(to + (at / per_row) * ld + (at % per_row) * VEC) = from[i];
+      for (int i = 0; i < N; ++i)
+        *reinterpret_cast<piece *>(to + E::at(i * (NT / PER) + tid / PER, (tid % PER) * VEC, ld)) = from[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N * VEC; ++i)
+        to[E::at((i * NT + tid) / (PER * VEC), tid % (PER * VEC), ld)] = from[i / VEC][i % VEC];
     }
   };
-
+  const std::integral_constant<int, PK> wide{};
+  const std::integral_constant<int, PV> narrow{};
   piece na[STATE_ONLY ? 1 : NK], nb[NK], nc[NV];
-  auto prefetch = [&](int64_t r0) {
-    if constexpr (!STATE_ONLY) fetch(na, pa, p.at, p.KD, p.va, PK, NK, r0);
-    fetch(nb, pb, p.bt, p.KD, p.vb, PK, NK, r0);
-    fetch(nc, pc, p.ct, p.VD, p.vc, PV, NV, r0);
+  auto fetch_a = [&](int64_t r0) {
+    if constexpr (!STATE_ONLY) fetch(wide, na, pa, at, kd, r0);
   };
-  prefetch(begin);
+  auto fetch_bc = [&](int64_t r0) {
+    fetch(wide, nb, pb, bt, kd, r0);
+    fetch(narrow, nc, pc, ct, vd, r0);
+  };
+  auto stage_all = [&]() {
+    if constexpr (!STATE_ONLY) stage(wide, sa, na, LK);
+    stage(wide, sb, nb, LK);
+    stage(narrow, sc, nc, LV);
+  };
+  if (begin < last) {
+    fetch_a(begin);
+    fetch_bc(begin);
+  }
 
   // X: rows 16 t + 4 g + r, column 16 w + l16
   f32x4 X[KT];
-  const int64_t state = bh * p.KD * p.VD;
-  float *ends = args.ends + ((static_cast<int64_t>(rest % args.problems) * args.B * args.H + bh) * (args.segments - 1)) *
-                                (KD * VD);
   const int col = 16 * w + l16;
+  const int64_t state = bh * p.KD * p.VD;
+  float *ends = args.ends + ((which * args.B * args.H + bh) * (args.segments - 1)) * (KD * VD);
+  const auto at_end = [&](int t) { return ((w * KT + t) * 64 + lane) * 4; };
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
-    if (!STATE_ONLY && seg > 0) {
-      X[t] = *reinterpret_cast<const f32x4 *>(ends + (seg - 1) * (KD * VD) + ((w * KT + t) * 64 + lane) * 4);
-    } else {
+    X[t] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (!STATE_ONLY) {
+      if (seg > 0 && args.joined) {
+        X[t] = *reinterpret_cast<const f32x4 *>(ends + (seg - 1) * (KD * VD) + at_end(t));
+      } else if (p.s_in) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int k = 16 * t + 4 * g + r;
-        X[t][r] = (!STATE_ONLY && p.s_in && k < p.KD && col < p.VD) ? p.s_in[state + k * p.sk + col * p.sv] * p.in_scale
-                                                                  : 0.0f;
+        for (int r = 0; r < 4; ++r) {
+          const int k = 16 * t + 4 * g + r;
+          if (k < p.KD && col < p.VD) X[t][r] = p.s_in[state + k * p.sk + col * p.sv] * p.in_scale;
+        }
       }
     }
-  }
-  __syncthreads();
-  // d^(i - j) of a block of a b^T on the diagonal and `k` below it
-  float dec[CT][4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int ij = l16 - 4 * g - r;
-    dec[0][r] = ij >= 0 ? pw[ij] : 0.0f;
-#pragma unroll
-    for (int k = 1; k < CT; ++k) dec[k][r] = pw[16 * k + ij];
   }
 
-  for (int64_t r0 = begin; r0 < end; r0 += C) {
-    if (r0 >= n) {  // nothing left but zeros to write (the whole workgroup)
-      if constexpr (STATE_ONLY) break;
-      if (active) {
-        for (int i = 0; i < C; i += 4) {
-          const int64_t r = r0 + i + g;
-          if (r < end && col < p.VD) {
-            const int64_t at = r * p.ot + b * p.ob + h * p.oh + col;
-            if (p.o_f32)
-              static_cast<float *>(p.o)[at] = 0.0f;
-            else
-              static_cast<T *>(p.o)[at] = T(0.0f);
-          }
-        }
+  if constexpr (!STATE_ONLY) {
+    if (!args.joined) {
+      const float whole = power(d, args.segment);
+      for (int64_t q = 0; q < seg; ++q) {
+        const int64_t left = n - q * args.segment;
+        const float f = left >= args.segment ? whole : left > 0 ? power(d, left) : 1.0f;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+          X[t] = f * X[t] + *reinterpret_cast<const f32x4 *>(ends + q * (KD * VD) + at_end(t));
       }
-      continue;
     }
-    const int c = n - r0 < C ? static_cast<int>(n - r0) : C;  // steps of this chunk
-    if constexpr (!STATE_ONLY) stage(sa, na, PK, LK, NK);
-    stage(sb, nb, PK, LK, NK);
-    stage(sc, nc, PV, LV, NV);
+  }
+
+  // where a lane's fragments start: of row l16, and of a column block
+  const int at_row = E::at(l16, 4 * g, 0), at_col = E::column_at(lane, 0);
+  const int row_k = l16 * LK + at_row, col_k = E::column_row(lane) * LK + at_col;
+  const int row_p = l16 * LP + at_row, col_v = E::column_row(lane) * LV + at_col;
+
+  if (begin < last) stage_all();
+  for (int64_t r0 = begin; r0 < last; r0 += C) {
+    const int c = last - r0 < C ? static_cast<int>(last - r0) : C;  // steps of this chunk
     __syncthreads();
-    if (r0 + C < end) prefetch(r0 + C);
+    if (r0 + C < last) fetch_bc(r0 + C);
+    if constexpr (!STATE_ONLY) {
+      // blocks (it, jt), jt <= it, of a b^T, transposed: rows j, column i
+      for (int q = w; q < CT * (CT + 1) / 2; q += NW) {
+        int it = 0, jt = q;
+        while (jt > it) jt -= ++it;
+        Frag x[KF], y[KF];
+#pragma unroll
+        for (int f = 0; f < KF; ++f) {
+          x[f] = E::row(sb + 16 * jt * LK + 32 * f + row_k);
+          y[f] = E::row(sa + 16 * it * LK + 32 * f + row_k);
+        }
+        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s;
+#pragma unroll
+        for (int f = 0; f < KF; f += 2) {
+          E::mma(s, x[f], y[f]);
+          E::mma(s1, x[f + 1], y[f + 1]);
+        }
+        s = (s + s1) * o_scale;
+        four z;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int ij = 16 * (it - jt) + l16 - 4 * g - r;
+          z[r] = static_cast<T>(ij >= 0 ? s[r] * pw[ij >= 0 ? ij : 0] : 0.0f);
+        }
+        *reinterpret_cast<four *>(sp + 16 * it * LP + 16 * jt + row_p) = z;
+      }
+    }
+    Frag vf[CF];
+    f32x4 o[CT];
     if (active) {
-      Frag vf[CF];
 #pragma unroll
-      for (int f = 0; f < CF; ++f) vf[f] = E::column(sc + 32 * f * LV + 16 * w, LV, lane);
+      for (int f = 0; f < CF; ++f) vf[f] = E::column(sc + 32 * f * LV + 16 * w + col_v, LV);
       if constexpr (!STATE_ONLY) {
+        // a X, transposed: rows are columns of the result, the column its row
         constexpr int XP = E::PARTS < 2 ? E::PARTS : 2;
-        Frag xf[KF][XP];
+        Frag af[2][CT];
+        auto read = [&](int f) {
 #pragma unroll
-        for (int f = 0; f < KF; ++f)
+          for (int it = 0; it < CT; ++it) af[f & 1][it] = E::row(sa + 16 * it * LK + 32 * f + row_k);
+        };
+        read(0);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) E::put(xf[f], i, X[2 * f + (i >> 2)][i & 3]);
+        for (int it = 0; it < CT; ++it) o[it] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int it = 0; it < CT; ++it) {
-          Frag af[KF];
+        for (int f = 0; f < KF; ++f) {
+          Frag xf[XP];
+          E::parts(xf, X[2 * f], X[2 * f + 1]);
+          if (f + 1 < KF) read(f + 1);
 #pragma unroll
-          for (int f = 0; f < KF; ++f) af[f] = E::row(sa + (16 * it + l16) * LK + 32 * f + 4 * g);
-          // transposed: rows are columns 16 w + 4 g .. of the result, the column its row
-          f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int k = 0; k < XP; ++k)
 #pragma unroll
-          for (int f = 0; f < KF; ++f)
+            for (int it = 0; it < CT; ++it) E::mma(o[it], xf[k], af[f & 1][it]);
+        }
 #pragma unroll
-            for (int k = 0; k < XP; ++k) E::mma(o, xf[f][k], af[f]);
-          const float lead = pw[16 * it + l16 + e];
+        for (int it = 0; it < CT; ++it) o[it] *= pw[16 * it + l16 + e] * o_scale;
+      }
+      // (a's rows later than the others: the registers of a X are free here)
+      if (r0 + C < last) fetch_a(r0 + C);
+      // the state: c scaled by d^(c - j - e)
+      const float fade = pw[c];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] *= lead;
+      for (int t = 0; t < KT; ++t) X[t] *= fade;
 #pragma unroll
-          for (int f = 0; f < CF; ++f) {
-            if (2 * f > it) continue;
-            Frag pf[1];
+      for (int f = 0; f < CF; ++f) {
+        f32x4 wt[2];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int jt = 2 * f + half;
-              f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-              if (jt <= it) {
+        for (int half = 0; half < 2; ++half) {
+          const int j0 = 32 * f + 16 * half + 4 * g;
+          if (c == C) {
+            wt[half] = *reinterpret_cast<const f32x4 *>(weight + j0);
+          } else {
 #pragma unroll
-                for (int q = 0; q < KF; ++q) E::mma(s, E::row(sb + (16 * jt + l16) * LK + 32 * q + 4 * g), af[q]);
-              }
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const float v = jt <= it ? s[r] * dec[jt <= it ? it - jt : 0][r] : 0.0f;
-                E::put(pf, 4 * half + r, v);
-              }
-            }
-            E::mma(o, vf[f], pf[0]);
-          }
-          // row i of the chunk, columns 16 w + 4 g .. + 3
-          const int64_t r = r0 + 16 * it + l16;
-          const int oc = 16 * w + 4 * g;
-          if (r < end) {
-            const int64_t t = (p.reverse && r < n) ? n - 1 - r : r;
-            const int64_t at = t * p.ot + b * p.ob + h * p.oh + oc;
-            if (p.o_f32) {
-              float *to = static_cast<float *>(p.o) + at;
-              if (p.vo && oc < p.VD)
-                *reinterpret_cast<f32x4 *>(to) = o * p.o_scale;
-              else
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  if (oc + q < p.VD) to[q] = o[q] * p.o_scale;
-            } else {
-              T *to = static_cast<T *>(p.o) + at;
-              typedef T four __attribute__((ext_vector_type(4)));
-              four z;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) z[q] = static_cast<T>(o[q] * p.o_scale);
-              if (p.vo && oc < p.VD)
-                *reinterpret_cast<four *>(to) = z;
-              else
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  if (oc + q < p.VD) to[q] = z[q];
+            for (int r = 0; r < 4; ++r) {
+              const int x = c - j0 - r - e;
+              wt[half][r] = pw[x > 0 ? x : 0];
             }
           }
         }
+        Frag vs[E::PARTS];
+        f32x4 lo, hi;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          lo[r] = static_cast<float>(vf[f][r]) * wt[0][r];
+          hi[r] = static_cast<float>(vf[f][4 + r]) * wt[1][r];
+        }
+        E::parts(vs, lo, hi);
+        // (two blocks at a time, so that a product does not wait for the one before)
+#pragma unroll
+        for (int t0 = 0; t0 < KT; t0 += 2) {
+          Frag kf[2];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) kf[t] = E::column(sb + 32 * f * LK + 16 * (t0 + t) + col_k, LK);
+#pragma unroll
+          for (int k = 0; k < E::PARTS; ++k)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) E::mma(X[t0 + t], kf[t], vs[k]);
+        }
       }
-      // the state: c scaled by d^(c - j - e)
-      Frag vs[CF][E::PARTS];
+    } else if (r0 + C < last) {
+      fetch_a(r0 + C);
+    }
+    __syncthreads();
+    if (r0 + C < last) stage_all();
+    if (!STATE_ONLY && active) {
 #pragma unroll
       for (int f = 0; f < CF; ++f)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = 32 * f + 16 * (i >> 2) + 4 * g + (i & 3), x = c - j - e;
-          E::put(vs[f], i, static_cast<float>(vf[f][i]) * pw[x > 0 ? x : 0]);
-        }
-      const float fade = pw[c];
+        for (int it = 2 * f; it < CT; ++it) E::mma(o[it], vf[f], E::row(sp + 16 * it * LP + 32 * f + row_p));
+      // row i of the chunk, columns 16 w + 4 g .. + 3
+      char *out = po + (reverse ? n - r0 - c : r0) * ot * (o_f32 ? 4 : sizeof(T));
+      const int oc = 16 * w + 4 * g;
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
+      for (int it = 0; it < CT; ++it) {
+        const int i = 16 * it + l16;
+        if (i >= c) continue;
+        if constexpr (WHOLE) {
+          // a uniform address and a 32-bit offset
+          const uint32_t at = static_cast<uint32_t>(reverse ? c - 1 - i : i) * static_cast<uint32_t>(ot) + oc;
+          if (oc >= vd) continue;
+          if (o_f32)
+            *reinterpret_cast<f32x4 *>(out + at * 4) = o[it];
+          else
+            *reinterpret_cast<four *>(out + at * sizeof(T)) = __builtin_convertvector(o[it], four);
+        } else {
+          const int64_t at = static_cast<int64_t>(reverse ? c - 1 - i : i) * ot + oc;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) X[t][r] *= fade;
-#pragma unroll
-        for (int f = 0; f < CF; ++f) {
-          const Frag kf = E::column(sb + 32 * f * LK + 16 * t, LK, lane);
-#pragma unroll
-          for (int k = 0; k < E::PARTS; ++k) E::mma(X[t], kf, vs[f][k]);
+          for (int q = 0; q < 4; ++q) {
+            if (oc + q >= vd) continue;
+            if (o_f32)
+              reinterpret_cast<float *>(out)[at + q] = o[it][q];
+            else
+              reinterpret_cast<T *>(out)[at + q] = static_cast<T>(o[it][q]);
+          }
         }
       }
     }
-    __syncthreads();
   }
-
-  if (!active) return;
   if constexpr (STATE_ONLY) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t)
-      *reinterpret_cast<f32x4 *>(ends + seg * (KD * VD) + ((w * KT + t) * 64 + lane) * 4) = X[t];
-  } else if (p.s_out && seg == args.segments - 1 && col < p.VD) {
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int k = 16 * t + 4 * g + r;
-        if (k < p.KD) p.s_out[state + k * p.sk + col * p.sv] = X[t][r] * p.out_scale;
+    for (int t = 0; t < KT; ++t) *reinterpret_cast<f32x4 *>(ends + seg * (KD * VD) + at_end(t)) = X[t];
+  } else {
+    // steps past the length give zeros
+    for (int64_t r = last > begin ? last : begin; r < end; ++r) {
+      for (int i = tid; i < vd; i += NT) {
+        if (o_f32)
+          reinterpret_cast<float *>(po)[r * ot + i] = 0.0f;
+        else
+          reinterpret_cast<T *>(po)[r * ot + i] = T(0.0f);
       }
+    }
+    if (p.s_out && seg == args.segments - 1 && col < p.VD) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int k = 16 * t + 4 * g + r;
+          if (k < p.KD) p.s_out[state + k * p.sk + col * p.sv] = X[t][r] * p.out_scale;
+        }
+    }
   }
 }
 
 // Turns the segments' own contributions into the states at their ends: a thread
-// an element of one (problem, b, h).
-template <int KT, int NT>
+// an element of one (problem, b, h), segments read ahead of the chain.
+template <int KT, int VD>
 __global__ __launch_bounds__(256) void join_segments(Args args) {
-  constexpr int VD = NT / 4, SIZE = 16 * KT * VD;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  constexpr int SIZE = 16 * KT * VD, AHEAD = 8;
+  const int at = static_cast<int>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t bh = blockIdx.y;
   const Problem &p = args.p[blockIdx.z];
-  const int at = static_cast<int>(i), r = at & 3, lane = (at >> 2) & 63, t = (at >> 8) % KT, w = (at >> 8) / KT;
-  const int k = 16 * t + 4 * (lane >> 4) + r, col = 16 * w + (lane & 15);
-  if (i >= SIZE || 16 * w >= p.VD) return;  // (columns that a wave has no part in were not written)
+  const int r = at & 3, lane = (at >> 2) & 63, t = (at >> 8) % KT, block = (at >> 8) / KT;
+  const int k = 16 * t + 4 * (lane >> 4) + r, col = 16 * block + (lane & 15);
   float *x = args.ends + ((blockIdx.z * args.B * args.H + bh) * (args.segments - 1)) * SIZE + at;
   const float d = args.decay[bh % args.H];
   const int64_t n = steps_of(args, bh / args.H);
   float s = (p.s_in && k < p.KD && col < p.VD) ? p.s_in[bh * p.KD * p.VD + k * p.sk + col * p.sv] * p.in_scale : 0.0f;
   const float whole = power(d, args.segment);
-  for (int64_t seg = 0; seg + 1 < args.segments; ++seg, x += SIZE) {
-    const int64_t left = n - seg * args.segment;
-    const float f = left >= args.segment ? whole : left > 0 ? power(d, left) : 1.0f;
-    s = __builtin_fmaf(f, s, *x);
-    *x = s;
+  for (int64_t seg = 0; seg + 1 < args.segments; seg += AHEAD, x += AHEAD * SIZE) {
+    const int m = args.segments - 1 - seg < AHEAD ? static_cast<int>(args.segments - 1 - seg) : AHEAD;
+    float y[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) y[i] = i < m ? x[static_cast<int64_t>(i) * SIZE] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int64_t left = n - (seg + i) * args.segment;
+      const float f = left >= args.segment ? whole : left > 0 ? power(d, left) : 1.0f;
+      s = __builtin_fmaf(f, s, y[i]);
+      if (i < m) x[static_cast<int64_t>(i) * SIZE] = s;
+    }
   }
 }
 
@@ -514,9 +662,9 @@ void launch_step(const StepArgs &a, unsigned grid, hipStream_t s) {
 
 // The padded widths of a call (of its widest problem).
 struct Shape {
-  int kt, nt;
+  int kt, vd;
 };
-Shape shape_of(int kd, int vd) { return {kd <= 64 ? 4 : 8, vd <= 64 ? 256 : 512}; }
+Shape shape_of(int kd, int vd) { return {kd <= 64 ? 4 : 8, vd <= 64 ? 64 : 128}; }
 
 // Segments of the time axis: as many as give the chip about 512 workgroups,
 // of 4 chunks at least.
@@ -536,20 +684,21 @@ int chunk_of(int dtype) { return dtype == 0 ? F32::C : BF16::C; }
 int64_t ends_elems(int dtype, int64_t T, int64_t BH, int problems, Shape sh) {
   int64_t segments, segment;
   split(T, BH * problems, chunk_of(dtype), &segments, &segment);
-  return (segments - 1) * BH * problems * (16 * sh.kt) * (sh.nt / 4);
+  return (segments - 1) * BH * problems * (16 * sh.kt) * sh.vd;
 }
 
-template <class E, int KT, int NT>
+template <class E, int KT, int NW, bool WHOLE>
 void launch_shape(const Args &a, hipStream_t s) {
   const int64_t heads = (a.B * a.H + 7) / 8 * 8 * a.problems;
   if (a.segments > 1) {
-    Args before = a;
-    before.segments = a.segments;  // the last segment's end is nobody's start
-    chunked<E, KT, NT, true><<<static_cast<unsigned>(heads * (a.segments - 1)), NT, 0, s>>>(before);
-    const dim3 grid(16 * KT * (NT / 4) / 256, static_cast<unsigned>(a.B * a.H), a.problems);
-    join_segments<KT, NT><<<grid, 256, 0, s>>>(a);
+    // (the last segment's end is nobody's start)
+    chunked<E, KT, NW, WHOLE, true><<<static_cast<unsigned>(heads * (a.segments - 1)), 64 * NW, 0, s>>>(a);
+    if (a.joined) {
+      const dim3 grid(KT * NW, static_cast<unsigned>(a.B * a.H), a.problems);
+      join_segments<KT, 16 * NW><<<grid, 256, 0, s>>>(a);
+    }
   }
-  chunked<E, KT, NT, false><<<static_cast<unsigned>(heads * a.segments), NT, 0, s>>>(a);
+  chunked<E, KT, NW, WHOLE, false><<<static_cast<unsigned>(heads * a.segments), 64 * NW, 0, s>>>(a);
 }
 
 template <class E>
@@ -557,28 +706,43 @@ void launch(Args &a, int problems, float *ends, hipStream_t s) {
   int kd = 0, vd = 0;
   a.problems = problems;
   a.ends = ends;
+  // rows of whole 16-byte pieces everywhere, and a chunk of them within 2^31 bytes
+  bool whole = true;
   for (int i = 0; i < problems; ++i) {
-    Problem &p = a.p[i];
+    const Problem &p = a.p[i];
     kd = p.KD > kd ? p.KD : kd;
     vd = p.VD > vd ? p.VD : vd;
-    const auto whole = [](const void *x, int64_t t, int64_t b, int64_t h, int width) {
-      return width % E::VEC == 0 && t % E::VEC == 0 && b % E::VEC == 0 && h % E::VEC == 0 && myelin::aligned(x, 16);
+    const auto rows = [](const void *x, int64_t t, int64_t b, int64_t h, int width) {
+      return width % E::VEC == 0 && t % E::VEC == 0 && b % E::VEC == 0 && h % E::VEC == 0 && myelin::aligned(x, 16) &&
+             t >= 0 && t < (1 << 23);
     };
-    p.va = whole(p.a, p.at, p.ab, p.ah, p.KD);
-    p.vb = whole(p.b, p.bt, p.bb, p.bh, p.KD);
-    p.vc = whole(p.c, p.ct, p.cb, p.ch, p.VD);
-    p.vo = p.VD % 4 == 0 && myelin::aligned(p.o, 16);
+    whole = whole && rows(p.a, p.at, p.ab, p.ah, p.KD) && rows(p.b, p.bt, p.bb, p.bh, p.KD) &&
+            rows(p.c, p.ct, p.cb, p.ch, p.VD) && rows(p.o, p.ot, p.ob, p.oh, p.VD);
   }
   split(a.T, a.B * a.H * problems, E::C, &a.segments, &a.segment);
+  // Where they are few each segment adds up those before it (2048 steps of 8 x 16
+  // heads of 128, 4 segments: training 396 -> 381 us); where they are many that
+  // reads more than joining them does (32768 steps of 16 heads, 32 segments: 253
+  // against 242 us).
+  a.joined = a.segments > 8;
   const Shape sh = shape_of(kd, vd);
-  if (sh.kt == 4 && sh.nt == 256)
-    launch_shape<E, 4, 256>(a, s);
+  const auto go = [&](auto kt, auto waves) {
+    constexpr int KT = decltype(kt)::value, NW = decltype(waves)::value;
+    if (whole)
+      launch_shape<E, KT, NW, true>(a, s);
+    else
+      launch_shape<E, KT, NW, false>(a, s);
+  };
+  const std::integral_constant<int, 4> four{};
+  const std::integral_constant<int, 8> eight{};
+  if (sh.kt == 4 && sh.vd == 64)
+    go(four, four);
   else if (sh.kt == 4)
-    launch_shape<E, 4, 512>(a, s);
-  else if (sh.nt == 256)
-    launch_shape<E, 8, 256>(a, s);
+    go(four, eight);
+  else if (sh.vd == 64)
+    go(eight, four);
   else
-    launch_shape<E, 8, 512>(a, s);
+    go(eight, eight);
 }
 
 int check(const char *what, int dtype, int64_t T, int64_t B, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
@@ -622,8 +786,12 @@ Problem problem(const void *a, const int64_t *as, const void *b, const int64_t *
 extern "C" int64_t myelin_decay_attention_workspace_elems(int dtype, int64_t T, int64_t B, int64_t H, int64_t Hk,
                                                           int64_t Dk, int64_t Dv, int backward) {
   if (T < 1 || B < 1 || H < 1 || Hk < 1 || Dk < 1 || Dv < 1 || Dk > kMaxDim || Dv > kMaxDim) return 0;
-  const int dk = static_cast<int>(Dk), dv = static_cast<int>(Dv), widest = dk > dv ? dk : dv;
+  const int dk = static_cast<int>(Dk), dv = static_cast<int>(Dv);
   if (!backward) return ends_elems(dtype, T, B * H, 1, shape_of(dk, dv));
+  // one launch for the three problems, of the wider shape (a launch for each
+  // shape would need more segments to fill the chip: 501 steps of 16 x 8 heads
+  // of 50 and 75, fp32, 290 against 263 us)
+  const int widest = dk > dv ? dk : dv;
   return ends_elems(dtype, T, B * H, 3, shape_of(widest, widest)) + (H != Hk ? T * B * H * (Dk + Dv) : 0);
 }
 
