@@ -19,7 +19,7 @@ import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
-from myelin_amd import _lib
+from myelin_amd import _lib, autograd
 from myelin_amd.packing import _device_of
 
 MAX_DIM = 128
@@ -181,6 +181,9 @@ def decay_attention(
         lengths = lengths.contiguous()
     scale = _scale(scale, q)
     q, k, v, decay = _rows(q), _rows(k), _rows(v), decay.contiguous()
+    if autograd.plain(q, k, v) and (initial_state is None or autograd.plain(initial_state)):
+        state, out = autograd.native().decay_attention(q, k, v, decay, initial_state, lengths, scale)
+        return state, out
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, initial_state)):
         return HipDecayAttentionFunction.apply(q, k, v, decay, initial_state, lengths, scale)
     return _forward(q, k, v, decay, initial_state, lengths, scale)
@@ -208,27 +211,19 @@ def decay_attention_step(
     scale = _scale(scale, q)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
         raise ValueError("decay_attention_step has no gradient; use decay_attention, or torch.no_grad()")
-    B, H, Dk = q.shape
-    Hk, Dv = v.shape[-2:]
-    if out_state is None:
-        out_state = torch.empty((B, H, Dk, Dv), dtype=torch.float32, device=q.device)
-    else:
+    state = state.contiguous()
+    if out_state is not None:
         _check_state(out_state, q, v, "out_state")
         if not out_state.is_contiguous():
             raise ValueError("out_state must be contiguous")
         if out_state.requires_grad:
             raise ValueError("out_state is written in place and must not require a gradient")
-    state = state.contiguous()
-    a, b, size = state.data_ptr(), out_state.data_ptr(), 4 * state.numel()
-    if a != b and a < b + size and b < a + size:
-        raise ValueError("out_state must be state itself or not overlap it")
-    q, k, v, decay = _rows(q), _rows(k), _rows(v), decay.contiguous()
-    out = torch.empty((B, H, Dv), dtype=q.dtype, device=q.device)
-    with _device_of(q):
-        _lib.call("myelin_decay_attention_step", q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.DT[q.dtype],
-                  _strides(q, k, v), decay.data_ptr(), a, out.data_ptr(), b, B, H, Hk, Dk, Dv, scale,
-                  _lib.stream(q.device))
-    return out_state, out
+        a, b, size = state.data_ptr(), out_state.data_ptr(), 4 * state.numel()
+        if a != b and a < b + size and b < a + size:
+            raise ValueError("out_state must be state itself or not overlap it")
+    new, out = autograd.native().decay_attention_step(_rows(q), _rows(k), _rows(v), decay.contiguous(), state,
+                                                      out_state, scale)
+    return (new if out_state is None else out_state), out
 
 
 class DecayAttention(nn.Module):

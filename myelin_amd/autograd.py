@@ -50,6 +50,10 @@ def native():
                 for n in ("myelin_lif_fwd_f32", "myelin_lif_bwd_f32", "myelin_alif_fwd_f32", "myelin_alif_bwd_f32",
                           "myelin_last_error")]
         _autograd.bind(*addr, _lib.MyelinHipError)
+        _autograd.bind_sequence({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
+            "myelin_token_log_probs_workspace_bytes", "myelin_token_log_probs", "myelin_token_log_probs_bwd",
+            "myelin_counter_dropout", "myelin_decay_attention_workspace_elems", "myelin_decay_attention_fwd",
+            "myelin_decay_attention_bwd", "myelin_decay_attention_step", "myelin_last_error")}, _lib.MyelinHipError)
         _native = _autograd
     return _native
 

@@ -2,8 +2,8 @@
 
 Run ``python -m myelin_amd.build``.  Every source is compiled with hipcc
 (``--offload-arch=gfx950``) into ``myelin_amd/_build/`` and linked into one
-shared library next to this file; ``csrc/autograd.cpp`` becomes the extension
-module ``myelin_amd/_autograd.so`` (host compiler, torch's headers).  Extra ``-D`` defines (kernel tuning
+shared library next to this file; ``csrc/*.cpp`` become the extension module
+``myelin_amd/_autograd.so`` (host compiler, torch's headers).  Extra ``-D`` defines (kernel tuning
 knobs) can be passed with ``MYELIN_HIPCC_DEFINES="-DNAME=VALUE ..."`` and the
 output path with ``MYELIN_LIB_OUT``.
 """
@@ -64,11 +64,21 @@ def build_autograd() -> pathlib.Path:
     includes = [root / "include", root / "include/torch/csrc/api/include", rocm / "include",
                 sysconfig.get_paths()["include"]]
     tmp = AUTOGRAD.with_suffix(".so.tmp")
-    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_autograd",
-          "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-          *(f"-isystem{i}" for i in includes), str(CSRC / "autograd.cpp"), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch",
-          "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-ltorch_python"])
+    cxx = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC"]
+    defines = ["-DTORCH_EXTENSION_NAME=_autograd", "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__=1",
+               "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    BUILD.mkdir(exist_ok=True)
+
+    def compile_one(src: pathlib.Path) -> None:
+        _run([*cxx, *defines, *(f"-isystem{i}" for i in includes), "-c", str(src), "-o",
+              str(BUILD / f"autograd.{src.stem}.o")])
+
+    sources = sorted(CSRC.glob("*.cpp"))
+    objs = [str(BUILD / f"autograd.{src.stem}.o") for src in sources]
+    with ThreadPoolExecutor(max_workers=2) as pool:
+        list(pool.map(compile_one, sources))
+    _run([*cxx, "-shared", *objs, "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_hip",
+          "-lc10", "-lc10_hip", "-ltorch_python"])
     os.replace(tmp, AUTOGRAD)
     return AUTOGRAD
 

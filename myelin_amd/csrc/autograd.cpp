@@ -18,6 +18,7 @@
 #include <string>
 
 #include "../../include/myelin_hip.h"
+#include "sequence_autograd.h"
 
 namespace {
 
@@ -159,4 +160,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                    double beta, double reset, double slope, int64_t rule, int64_t code, int64_t chunk) {
     return apply<true>(Params{decay, rho, threshold, beta, reset, slope, rule, code, chunk, false}, x, m0, a0);
   }, nogil);
+  register_sequence_operators(m);
 }

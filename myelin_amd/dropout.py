@@ -14,7 +14,7 @@ import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
-from myelin_amd import _lib
+from myelin_amd import _lib, autograd
 from myelin_amd.packing import _device_of
 
 _TYPES = (torch.float32, torch.bfloat16)
@@ -103,6 +103,9 @@ def counter_dropout(
     steps = x.shape[0] if time_shared else 1
     threshold = int(p * 2**32)
     scale = 0.0 if p == 1.0 else 1.0 / (1.0 - p)
+    if autograd.plain(x) and (residual is None or autograd.plain(residual)):
+        at, number = (offset, 0) if isinstance(offset, torch.Tensor) else (None, offset)
+        return autograd.native().counter_dropout(x, residual, at, steps, threshold, scale, seed, number)
     if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         return HipCounterDropoutFunction.apply(x, residual, steps, threshold, scale, seed, offset)
     return _launch(x, residual, steps, threshold, scale, seed, offset)

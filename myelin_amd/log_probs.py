@@ -9,7 +9,7 @@ from typing import Any, NamedTuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from myelin_amd import _lib
+from myelin_amd import _lib, autograd
 from myelin_amd.packing import _device_of
 
 MAX_TOP = 64
@@ -112,15 +112,23 @@ def token_log_probs(
             raise ValueError("targets must be on the same device as logits")
         if targets.dtype not in (torch.int64, torch.int32):
             raise ValueError(f"targets must be int64 or int32; got {targets.dtype}")
-        targets = targets.reshape(-1).to(torch.int64).contiguous()
-    x = logits if logits.stride(-1) == 1 or V == 1 else logits.contiguous()
-    x = x.reshape(-1, V)
+        if targets.ndim != 1:
+            targets = targets.reshape(-1)
+        targets = targets.to(torch.int64).contiguous()
+    x = logits if logits.ndim == 2 else logits.reshape(-1, V)
     if (x.shape[0] > 1 and x.stride(0) < V) or x.stride(1) != 1:
         x = x.contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
+    if autograd.plain(x):
+        results = iter(autograd.native().token_log_probs(x, targets, top, ignore_index))
+        log_probs = None if targets is None else next(results)
+        entropy = next(results)
+        top_lp, top_tok = (next(results), next(results)) if top else (None, None)
+    elif torch.is_grad_enabled() and x.requires_grad:
         log_probs, entropy, top_lp, top_tok = HipTokenLogProbsFunction.apply(x, targets, top, ignore_index)
     else:
         log_probs, entropy, _, top_lp, top_tok = _forward(x, targets, top, ignore_index)
+    if len(lead) == 1:
+        return TokenLogProbs(log_probs, entropy, top_lp, top_tok)
     return TokenLogProbs(
         None if log_probs is None else log_probs.view(lead),
         entropy.view(lead),
