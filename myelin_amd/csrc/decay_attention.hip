@@ -73,10 +73,13 @@ struct BF16 {
   static constexpr int VEC = 8;
   static constexpr int C = 64;
   static constexpr int PARTS = 3;
-  // LDS rows 32 bytes past a multiple of 64 banks (an odd multiple of 32 for
-  // the 128-byte rows), so that the transposing read's 8 rows of 32 bytes are
-  // on distinct banks; rows 8 .. 15 of 16 have the two halves of each 32 bytes
-  // exchanged, so that 16 rows' 8-byte pieces are too
+  // LDS rows an odd multiple of 32 bytes long, which puts the transposing read's
+  // 4 rows of 32 bytes on distinct banks (16 lanes take 128 bytes a cycle).  Of
+  // 16 rows' 8-byte pieces two share a bank; exchanging the halves of each 32
+  // bytes in rows 8 .. 15 keeps it at two.  (A permutation of 8-byte slots by
+  // the row's low four bits has no conflicts either way, but its addresses cost
+  // the registers that hold two workgroups to a CU: 2048 steps of 8 x 16 heads of
+  // 128, training, 380 -> 625 us.)
   static constexpr int PAD = 16;
   __device__ static int at(int row, int col, int ld) { return row * ld + (col ^ (row & 8)); }
   // a and b in N parts, each the rounded rest of those before
@@ -136,12 +139,12 @@ struct Problem {
 
 struct Args {
   Problem p[3];
-  int problems;
+  int problems, slices;  // slices of the widest problem's columns
   const float *decay;
   const int32_t *lengths;
   int64_t T, B, H;
   int64_t segments, segment;  // of steps, whole chunks
-  // [problems, B * H, segments - 1] states, as the lanes hold them: what each
+  // [problems, slices, B * H, segments - 1] states, as the lanes hold them: what each
   // segment adds, or (joined) the states at their ends
   float *ends;
   int joined;
@@ -168,8 +171,9 @@ __device__ __forceinline__ float power(float d, int64_t n) {
 // 1 - reverse:
 //   o_i = d^(i + e) a_i X + sum_{j <= i} d^(i - j) (a_i . b_j) c_j
 //   X'  = d^C X + sum_j d^(C - j - e) b_j c_j^T
-// A workgroup has one (problem, b, h) and a segment of its steps; wave w has
-// columns 16 w .. 16 w + 15 of X in the accumulators of its products, which are
+// A workgroup has one (problem, b, h), a slice of 16 columns of X for each of
+// its NW waves and a segment of the steps; wave w has columns 16 w .. 16 w + 15
+// of the slice in the accumulators of its products, which are
 // also, rounded, the operand of the next chunk's a X.  The waves share out the
 // 16 x 16 blocks of a b^T, scale them and put them into LDS.  Everything that
 // reads a chunk's a, b and c comes before the barrier that ends those blocks,
@@ -184,8 +188,8 @@ __device__ __forceinline__ float power(float d, int64_t n) {
 // WHOLE: all rows are whole 16-byte pieces.
 
 // Registers bound how many waves a CU holds: with whole rows 8 waves to a
-// workgroup fit 128, so that two of them share it.
-constexpr int waves_per_simd(int waves, bool whole) { return waves == 8 && whole ? 4 : 2; }
+// workgroup fit 128, so that two of them share it, and 4 fit 168, for three.
+constexpr int waves_per_simd(int waves, bool whole) { return whole ? (waves == 8 ? 4 : 3) : 2; }
 
 template <class E, int KT, int NW, bool WHOLE, bool STATE_ONLY>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, WHOLE)))) void chunked(
@@ -211,8 +215,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
   const uint32_t id = blockIdx.x, rest = id >> 3;
   const int which = static_cast<int>(rest % args.problems);
   const Problem &p = args.p[which];
-  const int64_t heads = (args.B * args.H + 7) / 8, r2 = rest / args.problems;
+  const int64_t heads = (args.B * args.H + 7) / 8, r1 = rest / args.problems, r2 = r1 / args.slices;
+  const int slice = static_cast<int>(r1 % args.slices), first = slice * VD;  // its first column
   const int64_t bh = (r2 % heads) * 8 + (id & 7), seg = r2 / heads;
+  if (first >= p.VD) return;
   if (bh >= args.B * args.H) return;
   const int64_t b = bh / args.H, h = bh % args.H;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -222,12 +228,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
   // (held in registers: arguments read in the loop cost it a scalar load each)
   const T *pa = static_cast<const T *>(p.a) + b * p.ab + (h / p.ga) * p.ah;
   const T *pb = static_cast<const T *>(p.b) + b * p.bb + (h / p.gb) * p.bh;
-  const T *pc = static_cast<const T *>(p.c) + b * p.cb + (h / p.gc) * p.ch;
+  const T *pc = static_cast<const T *>(p.c) + b * p.cb + (h / p.gc) * p.ch + first;
   const int64_t at = p.at, bt = p.bt, ct = p.ct, ot = p.ot;
-  const int kd = p.KD, vd = p.VD;
+  const int kd = p.KD, vd = p.VD - first < VD ? p.VD - first : VD;
   const bool o_f32 = p.o_f32;
   const float o_scale = p.o_scale;
-  char *po = static_cast<char *>(p.o) + (b * p.ob + h * p.oh) * (o_f32 ? 4 : sizeof(T));
+  char *po = static_cast<char *>(p.o) + (b * p.ob + h * p.oh + first) * (o_f32 ? 4 : sizeof(T));
   const int64_t begin = seg * args.segment;
   const int64_t end = begin + args.segment < args.T ? begin + args.segment : args.T;
   const int64_t last = n < end ? n : end;  // the segment's steps end here
@@ -327,11 +333,12 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
     fetch_bc(begin);
   }
 
-  // X: rows 16 t + 4 g + r, column 16 w + l16
+  // X: rows 16 t + 4 g + r, column 16 w + l16 of the slice
   f32x4 X[KT];
-  const int col = 16 * w + l16;
+  const int col = first + 16 * w + l16;
   const int64_t state = bh * p.KD * p.VD;
-  float *ends = args.ends + ((which * args.B * args.H + bh) * (args.segments - 1)) * (KD * VD);
+  float *ends =
+      args.ends + (((which * args.slices + slice) * args.B * args.H + bh) * (args.segments - 1)) * (KD * VD);
   const auto at_end = [&](int t) { return ((w * KT + t) * 64 + lane) * 4; };
 #pragma unroll
   for (int t = 0; t < KT; ++t) {
@@ -407,23 +414,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
       if constexpr (!STATE_ONLY) {
         // a X, transposed: rows are columns of the result, the column its row
         constexpr int XP = E::PARTS < 2 ? E::PARTS : 2;
-        Frag af[2][CT];
-        auto read = [&](int f) {
-#pragma unroll
-          for (int it = 0; it < CT; ++it) af[f & 1][it] = E::row(sa + 16 * it * LK + 32 * f + row_k);
-        };
-        read(0);
 #pragma unroll
         for (int it = 0; it < CT; ++it) o[it] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int f = 0; f < KF; ++f) {
           Frag xf[XP];
           E::parts(xf, X[2 * f], X[2 * f + 1]);
-          if (f + 1 < KF) read(f + 1);
+          Frag af[CT];
+#pragma unroll
+          for (int it = 0; it < CT; ++it) af[it] = E::row(sa + 16 * it * LK + 32 * f + row_k);
 #pragma unroll
           for (int k = 0; k < XP; ++k)
 #pragma unroll
-            for (int it = 0; it < CT; ++it) E::mma(o[it], xf[k], af[f & 1][it]);
+            for (int it = 0; it < CT; ++it) E::mma(o[it], xf[k], af[it]);
         }
 #pragma unroll
         for (int it = 0; it < CT; ++it) o[it] *= pw[16 * it + l16 + e] * o_scale;
@@ -536,14 +539,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
 
 // Turns the segments' own contributions into the states at their ends: a thread
 // an element of one (problem, b, h), segments read ahead of the chain.
-template <int KT, int VD>
+template <int KT, int NW>
 __global__ __launch_bounds__(256) void join_segments(Args args) {
-  constexpr int SIZE = 16 * KT * VD, AHEAD = 8;
+  constexpr int VD = 16 * NW, SIZE = 16 * KT * VD, AHEAD = 8;
   const int at = static_cast<int>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t bh = blockIdx.y;
-  const Problem &p = args.p[blockIdx.z];
+  const Problem &p = args.p[blockIdx.z / args.slices];
+  const int first = static_cast<int>(blockIdx.z % args.slices) * VD;
   const int r = at & 3, lane = (at >> 2) & 63, t = (at >> 8) % KT, block = (at >> 8) / KT;
-  const int k = 16 * t + 4 * (lane >> 4) + r, col = 16 * block + (lane & 15);
+  const int k = 16 * t + 4 * (lane >> 4) + r, col = first + 16 * block + (lane & 15);
   float *x = args.ends + ((blockIdx.z * args.B * args.H + bh) * (args.segments - 1)) * SIZE + at;
   const float d = args.decay[bh % args.H];
   const int64_t n = steps_of(args, bh / args.H);
@@ -660,17 +664,26 @@ void launch_step(const StepArgs &a, unsigned grid, hipStream_t s) {
   }
 }
 
-// The padded widths of a call (of its widest problem).
+// How a call is cut, by its widest problem: the padded KD (16 kt), slices of 16
+// nw columns, and the workgroups that the chip holds of it.  For bf16 of both
+// widths past 64 one workgroup of 8 waves has all columns, since each forms the
+// whole of a b^T; the others' smaller workgroups fill the chip more evenly, and
+// three share a CU (501 steps of 16 x 8 heads of 50 and 75, fp32, training: 258
+// -> 220 us; 1021 of 8 x 16 heads of 64 and 96, bf16: 59 -> 56 us; but 2048 of 8
+// x 16 heads of 128, bf16, training: 380 -> 390 us).
 struct Shape {
-  int kt, vd;
+  int kt, nw, slices, places;
 };
-Shape shape_of(int kd, int vd) { return {kd <= 64 ? 4 : 8, vd <= 64 ? 64 : 128}; }
+Shape shape_of(int dtype, int kd, int vd) {
+  if (dtype != 0 && kd > 64 && vd > 64) return {8, 8, 1, 512};
+  return {kd <= 64 ? 4 : 8, 4, (vd + 63) / 64, 768};
+}
 
-// Segments of the time axis: as many as give the chip about 512 workgroups,
+// Segments of the time axis: as many as fill the workgroups' places,
 // of 4 chunks at least.
-void split(int64_t T, int64_t workgroups, int C, int64_t *segments, int64_t *segment) {
+void split(int64_t T, int64_t workgroups, int places, int C, int64_t *segments, int64_t *segment) {
   const int64_t chunks = (T + C - 1) / C;
-  int64_t n = 512 / workgroups;
+  int64_t n = places / workgroups;
   if (n > chunks / 4) n = chunks / 4;
   if (n < 1) n = 1;
   const int64_t per = (chunks + n - 1) / n;
@@ -683,22 +696,22 @@ int chunk_of(int dtype) { return dtype == 0 ? F32::C : BF16::C; }
 // Floats of the segments' states.
 int64_t ends_elems(int dtype, int64_t T, int64_t BH, int problems, Shape sh) {
   int64_t segments, segment;
-  split(T, BH * problems, chunk_of(dtype), &segments, &segment);
-  return (segments - 1) * BH * problems * (16 * sh.kt) * sh.vd;
+  split(T, BH * problems * sh.slices, sh.places, chunk_of(dtype), &segments, &segment);
+  return (segments - 1) * BH * problems * sh.slices * (16 * sh.kt) * (16 * sh.nw);
 }
 
 template <class E, int KT, int NW, bool WHOLE>
 void launch_shape(const Args &a, hipStream_t s) {
-  const int64_t heads = (a.B * a.H + 7) / 8 * 8 * a.problems;
+  const int64_t groups = (a.B * a.H + 7) / 8 * 8 * a.problems * a.slices;
   if (a.segments > 1) {
     // (the last segment's end is nobody's start)
-    chunked<E, KT, NW, WHOLE, true><<<static_cast<unsigned>(heads * (a.segments - 1)), 64 * NW, 0, s>>>(a);
+    chunked<E, KT, NW, WHOLE, true><<<static_cast<unsigned>(groups * (a.segments - 1)), 64 * NW, 0, s>>>(a);
     if (a.joined) {
-      const dim3 grid(KT * NW, static_cast<unsigned>(a.B * a.H), a.problems);
-      join_segments<KT, 16 * NW><<<grid, 256, 0, s>>>(a);
+      const dim3 grid(KT * NW, static_cast<unsigned>(a.B * a.H), a.problems * a.slices);
+      join_segments<KT, NW><<<grid, 256, 0, s>>>(a);
     }
   }
-  chunked<E, KT, NW, WHOLE, false><<<static_cast<unsigned>(heads * a.segments), 64 * NW, 0, s>>>(a);
+  chunked<E, KT, NW, WHOLE, false><<<static_cast<unsigned>(groups * a.segments), 64 * NW, 0, s>>>(a);
 }
 
 template <class E>
@@ -719,13 +732,14 @@ void launch(Args &a, int problems, float *ends, hipStream_t s) {
     whole = whole && rows(p.a, p.at, p.ab, p.ah, p.KD) && rows(p.b, p.bt, p.bb, p.bh, p.KD) &&
             rows(p.c, p.ct, p.cb, p.ch, p.VD) && rows(p.o, p.ot, p.ob, p.oh, p.VD);
   }
-  split(a.T, a.B * a.H * problems, E::C, &a.segments, &a.segment);
+  const Shape sh = shape_of(sizeof(typename E::T) == 4 ? 0 : 2, kd, vd);
+  a.slices = sh.slices;
+  split(a.T, a.B * a.H * problems * a.slices, sh.places, E::C, &a.segments, &a.segment);
   // Where they are few each segment adds up those before it (2048 steps of 8 x 16
   // heads of 128, 4 segments: training 396 -> 381 us); where they are many that
   // reads more than joining them does (32768 steps of 16 heads, 32 segments: 253
   // against 242 us).
   a.joined = a.segments > 8;
-  const Shape sh = shape_of(kd, vd);
   const auto go = [&](auto kt, auto waves) {
     constexpr int KT = decltype(kt)::value, NW = decltype(waves)::value;
     if (whole)
@@ -735,13 +749,11 @@ void launch(Args &a, int problems, float *ends, hipStream_t s) {
   };
   const std::integral_constant<int, 4> four{};
   const std::integral_constant<int, 8> eight{};
-  if (sh.kt == 4 && sh.vd == 64)
+  if (sh.kt == 4)
     go(four, four);
-  else if (sh.kt == 4)
-    go(four, eight);
-  else if (sh.vd == 64)
+  else if (sh.nw == 4)
     go(eight, four);
-  else
+  else if constexpr (sizeof(typename E::T) == 2)
     go(eight, eight);
 }
 
@@ -787,12 +799,12 @@ extern "C" int64_t myelin_decay_attention_workspace_elems(int dtype, int64_t T, 
                                                           int64_t Dk, int64_t Dv, int backward) {
   if (T < 1 || B < 1 || H < 1 || Hk < 1 || Dk < 1 || Dv < 1 || Dk > kMaxDim || Dv > kMaxDim) return 0;
   const int dk = static_cast<int>(Dk), dv = static_cast<int>(Dv);
-  if (!backward) return ends_elems(dtype, T, B * H, 1, shape_of(dk, dv));
+  if (!backward) return ends_elems(dtype, T, B * H, 1, shape_of(dtype, dk, dv));
   // one launch for the three problems, of the wider shape (a launch for each
   // shape would need more segments to fill the chip: 501 steps of 16 x 8 heads
   // of 50 and 75, fp32, 290 against 263 us)
   const int widest = dk > dv ? dk : dv;
-  return ends_elems(dtype, T, B * H, 3, shape_of(widest, widest)) + (H != Hk ? T * B * H * (Dk + Dv) : 0);
+  return ends_elems(dtype, T, B * H, 3, shape_of(dtype, widest, widest)) + (H != Hk ? T * B * H * (Dk + Dv) : 0);
 }
 
 extern "C" int myelin_decay_attention_fwd(const void *q, const void *k, const void *v, int dtype,
