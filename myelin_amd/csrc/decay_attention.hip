@@ -182,17 +182,26 @@ __device__ __forceinline__ float power(float d, int64_t n) {
 //
 // Roundings to bf16: the scaled a b^T (then multiplied by the bf16 c, whose
 // products are exact) to one, as good as the result's own; X where it is an
-// operand to two, 16 bits; the scaled c of the state's sum, an fp32 result, to
-// three, which are fp32's 24 bits.
+// operand to two, 16 bits; the scaled c of the state's sum to three, which are
+// fp32's 24 bits, where that sum is a result, and to two where it is not.
 //
 // WHOLE: all rows are whole 16-byte pieces.
 
+template <class E>
+constexpr int lds_bytes(int kt, int waves) {
+  return E::C * (2 * (16 * kt + E::PAD) + 16 * waves + E::PAD + E::C + E::PAD + 2) *
+         static_cast<int>(sizeof(typename E::T));
+}
+
 // Registers bound how many waves a CU holds: with whole rows 8 waves to a
 // workgroup fit 128, so that two of them share it, and 4 fit 168, for three.
-constexpr int waves_per_simd(int waves, bool whole) { return whole ? (waves == 8 ? 4 : 3) : 2; }
+constexpr int waves_per_simd(int waves, int lds, bool whole) {
+  return !whole ? 2 : waves == 8 ? 4 : 160 * 1024 / lds < 3 ? 2 : 3;
+}
 
-template <class E, int KT, int NW, bool WHOLE, bool STATE_ONLY>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, WHOLE)))) void chunked(
+// EXACT: the last segment's X is a result.
+template <class E, int KT, int NW, bool WHOLE, bool STATE_ONLY, bool EXACT>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOLE)))) void chunked(
     Args args) {
   using T = typename E::T;
   using Frag = typename E::Frag;
@@ -453,7 +462,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
             }
           }
         }
-        Frag vs[E::PARTS];
+        // (16 bits of X where it is only an operand)
+        constexpr int VP = EXACT || E::PARTS < 3 ? E::PARTS : 2;
+        Frag vs[VP];
         f32x4 lo, hi;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -468,7 +479,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
 #pragma unroll
           for (int t = 0; t < 2; ++t) kf[t] = E::column(sb + 32 * f * LK + 16 * (t0 + t) + col_k, LK);
 #pragma unroll
-          for (int k = 0; k < E::PARTS; ++k)
+          for (int k = 0; k < VP; ++k)
 #pragma unroll
             for (int t = 0; t < 2; ++t) E::mma(X[t0 + t], kf[t], vs[k]);
         }
@@ -705,13 +716,22 @@ void launch_shape(const Args &a, hipStream_t s) {
   const int64_t groups = (a.B * a.H + 7) / 8 * 8 * a.problems * a.slices;
   if (a.segments > 1) {
     // (the last segment's end is nobody's start)
-    chunked<E, KT, NW, WHOLE, true><<<static_cast<unsigned>(groups * (a.segments - 1)), 64 * NW, 0, s>>>(a);
+    chunked<E, KT, NW, WHOLE, true, true><<<static_cast<unsigned>(groups * (a.segments - 1)), 64 * NW, 0, s>>>(a);
     if (a.joined) {
       const dim3 grid(KT * NW, static_cast<unsigned>(a.B * a.H), a.problems * a.slices);
       join_segments<KT, NW><<<grid, 256, 0, s>>>(a);
     }
   }
-  chunked<E, KT, NW, WHOLE, false><<<static_cast<unsigned>(groups * a.segments), 64 * NW, 0, s>>>(a);
+  const unsigned grid = static_cast<unsigned>(groups * a.segments);
+  bool exact = false;
+  for (int i = 0; i < a.problems; ++i) exact = exact || a.p[i].s_out;
+  if constexpr (E::PARTS == 3) {
+    if (!exact) {
+      chunked<E, KT, NW, WHOLE, false, false><<<grid, 64 * NW, 0, s>>>(a);
+      return;
+    }
+  }
+  chunked<E, KT, NW, WHOLE, false, true><<<grid, 64 * NW, 0, s>>>(a);
 }
 
 template <class E>
