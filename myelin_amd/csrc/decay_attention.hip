@@ -195,7 +195,7 @@ constexpr int lds_bytes(int kt, int waves) {
 
 // Registers bound how many waves a CU holds: with whole rows 8 waves to a
 // workgroup fit 128, so that two of them share it, and 4 fit 168, for three.
-constexpr int waves_per_simd(int waves, int lds, bool whole) {
+[[maybe_unused]] constexpr int waves_per_simd(int waves, int lds, bool whole) {
   return !whole ? 2 : waves == 8 ? 4 : 160 * 1024 / lds < 3 ? 2 : 3;
 }
 
@@ -607,7 +607,9 @@ struct StepArgs {
 
 // A workgroup has a (b, h); LX lanes to a row of the state, VEC columns a lane,
 // the other 256 / LX threads the next rows.  It reads the state once and writes
-// it once, which is nearly all that a step moves.
+// it once, which is nearly all that a step moves; the read passes the caches
+// (nontemporal), which leaves them to the states written: 256 x 16 states of 128
+// x 128 109 -> 88 us (6.1 TB/s).
 template <class E, int VEC, int LX>
 __global__ __launch_bounds__(256) void step_kernel(StepArgs a) {
   using T = typename E::T;
@@ -638,7 +640,7 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs a) {
   if (on) {
 #pragma unroll 8
     for (int r = ry; r < a.Dk; r += RY) {
-      vec s = *reinterpret_cast<const vec *>(a.state + base + static_cast<int64_t>(r) * a.Dv);
+      vec s = __builtin_nontemporal_load(reinterpret_cast<const vec *>(a.state + base + static_cast<int64_t>(r) * a.Dv));
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         s[i] = __builtin_fmaf(sk[r], c[i], d * s[i]);

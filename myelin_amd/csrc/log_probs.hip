@@ -6,6 +6,9 @@
 //   top: the n largest x_i - lse, equal ones by the lower index
 //   dx_i = g_lp (1[i = target] - p_i) - g_ent p_i (log p_i + entropy)
 //
+// The rows are read and the gradient written past the caches (nontemporal):
+// 8192 x 32768 bf16, forward and backward, 290 -> 263 us (1.55 GB, 5.9 TB/s).
+//
 // One pass: a lane keeps the running maximum m of its elements, s = sum
 // e^(x - m) and u = sum e^(x - m) (x - m); a larger maximum m' rescales them by
 // f = e^(m - m') as s' = f s, u' = f (u + (m - m') s).  Then log p = (x - m) -
@@ -270,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void wide_rows(Args a) {
     for (int j = 0; j < NV; ++j) {
       const int64_t i = at + (static_cast<int64_t>(j) * kThreads + tid) * VEC;
       if (i >= begin && i + VEC <= end) {
-        const vec p = *reinterpret_cast<const vec *>(x + i);
+        const vec p = __builtin_nontemporal_load(reinterpret_cast<const vec *>(x + i));
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
           v[j * VEC + q] = E::get(p[q]);
@@ -473,11 +476,11 @@ __global__ __launch_bounds__(256) void grad_wide(BwdArgs a) {
 #pragma unroll
         for (int q = 0; q < VEC; ++q) o[q] = E::put(0.0f);
       } else {
-        const vec p = *reinterpret_cast<const vec *>(x + i);
+        const vec p = __builtin_nontemporal_load(reinterpret_cast<const vec *>(x + i));
 #pragma unroll
         for (int q = 0; q < VEC; ++q) o[q] = E::put(grad_of(g, E::get(p[q]), i + q));
       }
-      *reinterpret_cast<vec *>(dx + i) = o;
+      __builtin_nontemporal_store(o, reinterpret_cast<vec *>(dx + i));
     } else {
       dx[i] = g.zero ? E::put(0.0f) : E::put(grad_of(g, E::get(x[i]), i));
     }
