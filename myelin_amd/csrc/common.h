@@ -25,6 +25,19 @@ inline bool aligned(const void *p, int bytes) {
 
 constexpr int kWave = 64;
 
+// Results of at least this many bytes (a quarter of the 256 MB cache in front
+// of the memory) are written past the caches by the kernels that ask: they
+// would push out what others read, and what reads them finds little of them.
+constexpr int64_t kStreamBytes = int64_t{64} << 20;
+
+template <bool STREAM, class V>
+__device__ __forceinline__ void store(V v, V *to) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(v, to);
+  else
+    *to = v;
+}
+
 // 1/b rounded to nearest, for b >= 1: the hardware reciprocal refined by
 // one Newton step (e = 1 - b*r exact in an fma, r + r*e rounded once).  On
 // gfx950 this equals the IEEE quotient 1.0f / b for every fp32 significand

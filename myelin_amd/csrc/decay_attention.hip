@@ -607,10 +607,9 @@ struct StepArgs {
 
 // A workgroup has a (b, h); LX lanes to a row of the state, VEC columns a lane,
 // the other 256 / LX threads the next rows.  It reads the state once and writes
-// it once, which is nearly all that a step moves; the read passes the caches
-// (nontemporal), which leaves them to the states written: 256 x 16 states of 128
-// x 128 109 -> 88 us (6.1 TB/s).
-template <class E, int VEC, int LX>
+// it once, which is nearly all that a step moves, both past the caches where the
+// states are large: 256 x 16 states of 128 x 128 109 -> 99 us (5.5 TB/s).
+template <class E, int VEC, int LX, bool STREAM>
 __global__ __launch_bounds__(256) void step_kernel(StepArgs a) {
   using T = typename E::T;
   constexpr int RY = 256 / LX;
@@ -646,7 +645,7 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs a) {
         s[i] = __builtin_fmaf(sk[r], c[i], d * s[i]);
         out[i] = __builtin_fmaf(sq[r], s[i], out[i]);
       }
-      *reinterpret_cast<vec *>(a.state_out + base + static_cast<int64_t>(r) * a.Dv) = s;
+      myelin::store<STREAM>(s, reinterpret_cast<vec *>(a.state_out + base + static_cast<int64_t>(r) * a.Dv));
     }
   }
 #pragma unroll
@@ -662,19 +661,26 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs a) {
 template <class E>
 void launch_step(const StepArgs &a, unsigned grid, hipStream_t s) {
   const bool vector = a.Dv % 4 == 0 && myelin::aligned(a.state, 16) && myelin::aligned(a.state_out, 16);
-  if (vector) {
+  if (!vector) {
     if (a.Dv <= 32)
-      step_kernel<E, 4, 8><<<grid, 256, 0, s>>>(a);
-    else if (a.Dv <= 64)
-      step_kernel<E, 4, 16><<<grid, 256, 0, s>>>(a);
+      step_kernel<E, 1, 32, false><<<grid, 256, 0, s>>>(a);
     else
-      step_kernel<E, 4, 32><<<grid, 256, 0, s>>>(a);
-  } else {
-    if (a.Dv <= 32)
-      step_kernel<E, 1, 32><<<grid, 256, 0, s>>>(a);
-    else
-      step_kernel<E, 1, 128><<<grid, 256, 0, s>>>(a);
+      step_kernel<E, 1, 128, false><<<grid, 256, 0, s>>>(a);
+    return;
   }
+  const auto go = [&](auto stream) {
+    constexpr bool STREAM = decltype(stream)::value;
+    if (a.Dv <= 32)
+      step_kernel<E, 4, 8, STREAM><<<grid, 256, 0, s>>>(a);
+    else if (a.Dv <= 64)
+      step_kernel<E, 4, 16, STREAM><<<grid, 256, 0, s>>>(a);
+    else
+      step_kernel<E, 4, 32, STREAM><<<grid, 256, 0, s>>>(a);
+  };
+  if (static_cast<int64_t>(grid) * a.Dk * a.Dv * 4 >= myelin::kStreamBytes)
+    go(std::true_type{});
+  else
+    go(std::false_type{});
 }
 
 // How a call is cut, by its widest problem: the padded KD (16 kt), slices of 16

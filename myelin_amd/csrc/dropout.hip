@@ -9,9 +9,9 @@
 //   y = x * scale (+ residual) where kept, 0 (+ residual) elsewhere
 // in fp32, rounded once; a dropped NaN or infinity is dropped.
 //
-// Bound by memory: x and the residual are read past the caches (nontemporal; the
-// result, usually read next, is not): forward and backward of 26 M fp32 with a
-// shared mask 83 -> 71 us (5.9 TB/s), of 38 M bf16 with a residual 76 -> 71.
+// Bound by memory: x and the residual are read past the caches (nontemporal),
+// and large results written so: forward and backward of 26 M fp32 with a shared
+// mask 83 -> 76 us (5.5 TB/s), of 38 M bf16 with a residual 74 -> 71.
 //
 // x is [steps, n]: one mask of n elements for all steps (a spiking layer keeps
 // its mask over time), or steps = 1 and a mask element for each of x.
@@ -60,7 +60,7 @@ __device__ __forceinline__ void philox(uint64_t group, uint64_t offset, uint32_t
 
 // A thread has VEC mask elements, for `per` steps of them.  VECTOR: rows start
 // on multiples of 16 bytes and hold whole vectors.
-template <class E, bool VECTOR>
+template <class E, bool VECTOR, bool STREAM>
 __global__ __launch_bounds__(256) void dropout_kernel(Args a) {
   using T = typename E::T;
   constexpr int VEC = E::VEC;
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(Args a) {
         o[q] = static_cast<T>(f);
       }
       if constexpr (VECTOR) {
-        *reinterpret_cast<vec *>(y) = o;
+        myelin::store<STREAM>(o, reinterpret_cast<vec *>(y));
       } else {
 #pragma unroll
         for (int q = 0; q < VEC; ++q) y[q] = o[q];
@@ -128,10 +128,12 @@ int launch(Args &a, hipStream_t s) {
   const bool rows = a.steps == 1 ? a.n % E::VEC == 0 : (a.n * sizeof(typename E::T)) % 16 == 0;
   const bool vector = rows && myelin::aligned(a.x, 16) && myelin::aligned(a.y, 16) && myelin::aligned(a.residual, 16);
   const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(by));
-  if (vector)
-    dropout_kernel<E, true><<<grid, 256, 0, s>>>(a);
+  if (!vector)
+    dropout_kernel<E, false, false><<<grid, 256, 0, s>>>(a);
+  else if (a.steps * a.n * static_cast<int64_t>(sizeof(typename E::T)) >= myelin::kStreamBytes)
+    dropout_kernel<E, true, true><<<grid, 256, 0, s>>>(a);
   else
-    dropout_kernel<E, false><<<grid, 256, 0, s>>>(a);
+    dropout_kernel<E, true, false><<<grid, 256, 0, s>>>(a);
   return myelin::launched("counter_dropout");
 }
 

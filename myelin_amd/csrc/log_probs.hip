@@ -6,8 +6,8 @@
 //   top: the n largest x_i - lse, equal ones by the lower index
 //   dx_i = g_lp (1[i = target] - p_i) - g_ent p_i (log p_i + entropy)
 //
-// The rows are read and the gradient written past the caches (nontemporal):
-// 8192 x 32768 bf16, forward and backward, 290 -> 263 us (1.55 GB, 5.9 TB/s).
+// The rows are read past the caches (nontemporal) and a large gradient written
+// so: 8192 x 32768 bf16, forward and backward, 290 -> 263 us (1.55 GB, 5.9 TB/s).
 //
 // One pass: a lane keeps the running maximum m of its elements, s = sum
 // e^(x - m) and u = sum e^(x - m) (x - m); a larger maximum m' rescales them by
@@ -456,7 +456,7 @@ __global__ __launch_bounds__(256) void grad_flat(BwdArgs a) {
   static_cast<typename E::T *>(a.dx)[at] = g.zero ? E::put(0.0f) : E::put(grad_of(g, E::get(x[row * a.ld + i]), i));
 }
 
-template <class E, bool VECTOR>
+template <class E, bool VECTOR, bool STREAM>
 __global__ __launch_bounds__(256) void grad_wide(BwdArgs a) {
   using T = typename E::T;
   constexpr int VEC = VECTOR ? E::VEC : 1, NV = kPerThread / VEC;
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(256) void grad_wide(BwdArgs a) {
 #pragma unroll
         for (int q = 0; q < VEC; ++q) o[q] = E::put(grad_of(g, E::get(p[q]), i + q));
       }
-      __builtin_nontemporal_store(o, reinterpret_cast<vec *>(dx + i));
+      myelin::store<STREAM>(o, reinterpret_cast<vec *>(dx + i));
     } else {
       dx[i] = g.zero ? E::put(0.0f) : E::put(grad_of(g, E::get(x[i]), i));
     }
@@ -545,10 +545,12 @@ void launch_bwd(BwdArgs &a, hipStream_t s) {
                       myelin::aligned(a.dx, 16);
   a.per_row = (a.V + kTile - 1) / kTile;
   const unsigned grid = static_cast<unsigned>(a.R * a.per_row);
-  if (vector)
-    grad_wide<E, true><<<grid, 256, 0, s>>>(a);
+  if (!vector)
+    grad_wide<E, false, false><<<grid, 256, 0, s>>>(a);
+  else if (total * static_cast<int64_t>(sizeof(typename E::T)) >= myelin::kStreamBytes)
+    grad_wide<E, true, true><<<grid, 256, 0, s>>>(a);
   else
-    grad_wide<E, false><<<grid, 256, 0, s>>>(a);
+    grad_wide<E, true, false><<<grid, 256, 0, s>>>(a);
 }
 
 }  // namespace
