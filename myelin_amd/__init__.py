@@ -3,7 +3,9 @@
 ``import myelin_amd as myelin`` gives the names callers of djsaunde/myelin
 use on this path (kernels, packing, neuron types, surrogates, checkpoint
 policy, and the streamed-synapse / rate modules); every compute call runs a
-hand-written gfx950 HIP kernel from ``libmyelin_hip.so``.
+hand-written gfx950 HIP kernel from ``libmyelin_hip.so``.  Beside them are the
+operators of a spiking sequence model, which myelin does not have:
+``decay_attention`` and its step, ``counter_dropout`` and ``token_log_probs``.
 """
 
 from myelin_amd.attention import DecayAttention, decay_attention, decay_attention_step

@@ -378,6 +378,11 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
     }
   }
 
+  // Blocks of 32 rows of X past the width.  fp32's products take long enough for
+  // this to pay (100 steps of 4 x 4 heads of 32: 19.2 -> 17.0 us); in the bf16
+  // kernels the branches cost more than the products.
+  const auto past = [&](int f) { return E::PARTS == 1 && 32 * f >= kd; };
+
   // where a lane's fragments start: of row l16, and of a column block
   const int at_row = E::at(l16, 4 * g, 0), at_col = E::column_at(lane, 0);
   const int row_k = l16 * LK + at_row, col_k = E::column_row(lane) * LK + at_col;
@@ -396,14 +401,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
         Frag x[KF], y[KF];
 #pragma unroll
         for (int f = 0; f < KF; ++f) {
+          if (past(f)) continue;
           x[f] = E::row(sb + 16 * jt * LK + 32 * f + row_k);
           y[f] = E::row(sa + 16 * it * LK + 32 * f + row_k);
         }
         f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f}, s1 = s;
 #pragma unroll
         for (int f = 0; f < KF; f += 2) {
-          E::mma(s, x[f], y[f]);
-          E::mma(s1, x[f + 1], y[f + 1]);
+          if (!past(f)) E::mma(s, x[f], y[f]);
+          if (!past(f + 1)) E::mma(s1, x[f + 1], y[f + 1]);
         }
         s = (s + s1) * o_scale;
         four z;
@@ -427,6 +433,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
         for (int it = 0; it < CT; ++it) o[it] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int f = 0; f < KF; ++f) {
+          if (past(f)) continue;
           Frag xf[XP];
           E::parts(xf, X[2 * f], X[2 * f + 1]);
           Frag af[CT];
@@ -475,6 +482,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(waves_p
         // (two blocks at a time, so that a product does not wait for the one before)
 #pragma unroll
         for (int t0 = 0; t0 < KT; t0 += 2) {
+          if (past(t0 / 2)) continue;
           Frag kf[2];
 #pragma unroll
           for (int t = 0; t < 2; ++t) kf[t] = E::column(sb + 32 * f * LK + 16 * (t0 + t) + col_k, LK);
