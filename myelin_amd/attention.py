@@ -17,7 +17,6 @@ from typing import Any, Sequence
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from myelin_amd import _lib, autograd
 from myelin_amd.packing import _device_of
@@ -71,7 +70,7 @@ class HipDecayAttentionFunction(torch.autograd.Function):
         return _forward(q, k, v, decay, state, lengths, scale)
 
     @staticmethod
-    @once_differentiable
+    @autograd.differentiated_once
     def backward(ctx: Any, g_final, g_out):
         if g_final is None and g_out is None:
             return (None,) * 7

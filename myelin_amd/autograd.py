@@ -15,6 +15,7 @@ re-reads ``x`` once to recompute each chunk.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Any
 
@@ -87,6 +88,26 @@ def alif(x, m0, a0, decay, rho, threshold, beta, reset, slope, rule, sid):
         return native().alif(x, m0, a0, decay, rho, threshold, beta, reset, slope, rule, sid, BWD_CHUNK)
     with torch.cuda.device(x.device):
         return HipALIFFunction.apply(x, m0, a0, decay, rho, threshold, beta, reset, slope, rule, sid)
+
+
+def differentiated_once(backward):
+    """For a Function's ``backward`` that has no derivative of its own: under
+    ``create_graph`` its gradients carry a node that raises when it is
+    differentiated.  (torch's ``once_differentiable`` does so only where the
+    incoming gradients ask for one; otherwise a second derivative would miss
+    the saved tensors' part without a word.)"""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        with torch.no_grad():
+            outputs = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return outputs
+        error = torch._C._functions.DelayedError(
+            b"trying to differentiate twice a function that was marked with @once_differentiable", len(outputs))
+        return error(*[None if t is None else t.detach().requires_grad_() for t in outputs])
+
+    return wrapper
 
 
 def _chunks(T: int) -> int:

@@ -12,7 +12,6 @@ from typing import Any
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from myelin_amd import _lib, autograd
 from myelin_amd.packing import _device_of
@@ -46,7 +45,7 @@ class HipCounterDropoutFunction(torch.autograd.Function):
         return _launch(x, residual, steps, threshold, scale, seed, offset)
 
     @staticmethod
-    @once_differentiable
+    @autograd.differentiated_once
     def backward(ctx: Any, g):
         gx = None
         if g is not None and ctx.needs_input_grad[0]:

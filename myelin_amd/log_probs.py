@@ -7,7 +7,6 @@ from __future__ import annotations
 from typing import Any, NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from myelin_amd import _lib, autograd
 from myelin_amd.packing import _device_of
@@ -60,7 +59,7 @@ class HipTokenLogProbsFunction(torch.autograd.Function):
         return log_probs, entropy, top_lp, top_tok
 
     @staticmethod
-    @once_differentiable
+    @autograd.differentiated_once
     def backward(ctx: Any, g_lp, g_ent, _g_top=None, _g_tok=None):
         if g_lp is None and g_ent is None:
             return None, None, None, None
