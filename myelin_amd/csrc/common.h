@@ -25,6 +25,17 @@ inline bool aligned(const void *p, int bytes) {
 
 constexpr int kWave = 64;
 
+// A launch has fewer than 2^32 threads in x.  Up to kGridX workgroups of 256 (a
+// multiple of the XCDs) go there, more into y, whose last row may be past the end.
+constexpr int64_t kGridX = int64_t{1} << 23;
+
+inline dim3 grid_of(int64_t blocks) {
+  const int64_t y = (blocks + kGridX - 1) / kGridX;
+  return dim3(static_cast<unsigned>(y > 1 ? kGridX : blocks), static_cast<unsigned>(y));
+}
+
+__device__ __forceinline__ int64_t block_id() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 // Results of at least this many bytes (a quarter of the 256 MB cache in front
 // of the memory) are written past the caches by the kernels that ask: they
 // would push out what others read, and what reads them finds little of them.

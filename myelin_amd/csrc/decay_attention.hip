@@ -603,7 +603,7 @@ __global__ __launch_bounds__(256) void join_segments(Args args) {
 template <class E>
 __global__ __launch_bounds__(256) void sum_groups(const float *__restrict__ from, void *__restrict__ to, int64_t n,
                                                   int group, int D) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t i = myelin::block_id() * 256 + threadIdx.x;
   if (i >= n) return;
   const int64_t head = i / D;
   const float *f = from + head * group * D + (i - head * D);
@@ -811,7 +811,8 @@ int check(const char *what, int dtype, int64_t T, int64_t B, int64_t H, int64_t 
   if (H % Hk) return myelin::invalid("%s: H must be a multiple of Hk", what);
   if (Dk < 1 || Dk > kMaxDim || Dv < 1 || Dv > kMaxDim)
     return myelin::invalid("%s: Dk and Dv must be in [1, %d]", what, kMaxDim);
-  if (T > 0x7fffffff || B * H > (1 << 28)) return myelin::invalid("%s: too many rows", what);
+  // (six workgroups of 256 threads for a head, fewer than 2^32 threads in all)
+  if (T > 0x7fffffff || B > (1 << 21) / H) return myelin::invalid("%s: too many rows", what);
   if (!(scale > 0.0f) && !(scale < 0.0f)) return myelin::invalid("%s: scale must not be zero", what);
   if (scale - scale != 0.0f) return myelin::invalid("%s: scale must be finite", what);
   return MYELIN_OK;
@@ -927,7 +928,7 @@ extern "C" int myelin_decay_attention_bwd(const void *q, const void *k, const vo
     for (int i = 0; i < 2; ++i) {
       const int D = i ? dv : dk;
       const int64_t n = T * B * Hk * D;
-      const unsigned grid = static_cast<unsigned>((n + 255) / 256);
+      const dim3 grid = myelin::grid_of((n + 255) / 256);
       const float *from = static_cast<const float *>(i ? to_v : to_k);
       void *to = i ? grad_v : grad_k;
       if (dtype == 0)

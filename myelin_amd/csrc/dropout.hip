@@ -118,8 +118,9 @@ __global__ __launch_bounds__(256) void dropout_kernel(Args a) {
 
 template <class E>
 int launch(Args &a, hipStream_t s) {
+  // (fewer than 2^32 threads in x)
   const int64_t threads = (a.n + E::VEC - 1) / E::VEC, bx = (threads + 255) / 256;
-  if (bx > 0x7fffffff) return myelin::invalid("counter_dropout: too many elements");
+  if (bx > 0xffffff) return myelin::invalid("counter_dropout: too many elements");
   // steps to a workgroup: as many as leave 2048 workgroups
   int64_t by = bx >= 2048 ? 1 : (2048 + bx - 1) / bx;
   if (by > a.steps) by = a.steps;

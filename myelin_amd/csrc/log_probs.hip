@@ -109,6 +109,7 @@ struct Args {
   int top;
   int parts;
   int64_t part;  // elements of a part
+  int64_t rows;  // of a launch in x
   Stats *part_stats;
   uint64_t *part_keys;
 };
@@ -159,7 +160,7 @@ __device__ __forceinline__ bool ignored(const Args &a, int64_t row) {
 // kNarrow.  12800 rows of 10: 3.8 us, a launch's latency.
 template <class E, int LANES>
 __global__ __launch_bounds__(256) void narrow_rows(Args a) {
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LANES;
+  const int64_t row = (myelin::block_id() * 256 + threadIdx.x) / LANES;
   const int l = threadIdx.x % LANES;
   if (row >= a.R) return;  // whole groups of lanes
   if (ignored(a, row)) {
@@ -252,7 +253,8 @@ __global__ __launch_bounds__(kThreads) void wide_rows(Args a) {
   __shared__ uint64_t bound_of[kWaves];
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid >> 6;
-  const int64_t row = blockIdx.x / a.parts;
+  const int64_t row = blockIdx.x / a.parts + blockIdx.y * a.rows;
+  if (row >= a.R) return;  // the whole workgroup
   const int part = static_cast<int>(blockIdx.x % a.parts);
   const int64_t begin = part * a.part;
   const int64_t end = begin + a.part < a.V ? begin + a.part : a.V;
@@ -424,6 +426,7 @@ struct BwdArgs {
   void *dx;  // [R, V] contiguous
   int64_t R, V;
   int64_t per_row;  // workgroups of a row
+  int64_t rows;     // of a launch in x
 };
 
 struct RowGrad {
@@ -456,7 +459,7 @@ __device__ __forceinline__ float grad_of(const RowGrad &g, float x, int64_t i) {
 
 template <class E>
 __global__ __launch_bounds__(256) void grad_flat(BwdArgs a) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t at = myelin::block_id() * 256 + threadIdx.x;
   if (at >= a.R * a.V) return;
   const int64_t row = at / a.V, i = at - row * a.V;
   const RowGrad g = row_grad(a, row);
@@ -469,7 +472,8 @@ __global__ __launch_bounds__(256) void grad_wide(BwdArgs a) {
   using T = typename E::T;
   constexpr int VEC = VECTOR ? E::VEC : 1, NV = kPerThread / VEC;
   typedef T vec __attribute__((ext_vector_type(VEC)));
-  const int64_t row = blockIdx.x / a.per_row;
+  const int64_t row = blockIdx.x / a.per_row + blockIdx.y * a.rows;
+  if (row >= a.R) return;
   const int64_t at = (blockIdx.x % a.per_row) * kTile;
   const RowGrad g = row_grad(a, row);
   const T *x = static_cast<const T *>(a.x) + row * a.ld;
@@ -520,16 +524,22 @@ int check(const char *what, const void *x, int dtype, int64_t ld, int64_t R, int
   return MYELIN_OK;
 }
 
+// `per_row` workgroups for each of R rows, whole rows in x.
+dim3 row_grid(int64_t R, int64_t per_row, int64_t *rows) {
+  *rows = R < myelin::kGridX / per_row ? R : myelin::kGridX / per_row;
+  return dim3(static_cast<unsigned>(*rows * per_row), static_cast<unsigned>((R + *rows - 1) / *rows));
+}
+
 template <class E>
 void launch_fwd(Args &a, hipStream_t s) {
   if (narrow(a.V, a.top)) {
     if (a.V <= 32)
-      narrow_rows<E, 8><<<static_cast<unsigned>((a.R * 8 + 255) / 256), 256, 0, s>>>(a);
+      narrow_rows<E, 8><<<myelin::grid_of((a.R * 8 + 255) / 256), 256, 0, s>>>(a);
     else
-      narrow_rows<E, 64><<<static_cast<unsigned>((a.R * 64 + 255) / 256), 256, 0, s>>>(a);
+      narrow_rows<E, 64><<<myelin::grid_of((a.R * 64 + 255) / 256), 256, 0, s>>>(a);
     return;
   }
-  const unsigned grid = static_cast<unsigned>(a.R * a.parts);
+  const dim3 grid = row_grid(a.R, a.parts, &a.rows);
   if (a.top)
     wide_rows<E, true><<<grid, kThreads, 0, s>>>(a);
   else
@@ -546,13 +556,13 @@ template <class E>
 void launch_bwd(BwdArgs &a, hipStream_t s) {
   const int64_t total = a.R * a.V;
   if (a.V < 256) {
-    grad_flat<E><<<static_cast<unsigned>((total + 255) / 256), 256, 0, s>>>(a);
+    grad_flat<E><<<myelin::grid_of((total + 255) / 256), 256, 0, s>>>(a);
     return;
   }
   const bool vector = a.V % E::VEC == 0 && (a.ld * sizeof(typename E::T)) % 16 == 0 && myelin::aligned(a.x, 16) &&
                       myelin::aligned(a.dx, 16);
   a.per_row = (a.V + kTile - 1) / kTile;
-  const unsigned grid = static_cast<unsigned>(a.R * a.per_row);
+  const dim3 grid = row_grid(a.R, a.per_row, &a.rows);
   if (!vector)
     grad_wide<E, false, false><<<grid, 256, 0, s>>>(a);
   else if (total * static_cast<int64_t>(sizeof(typename E::T)) >= myelin::kStreamBytes)
@@ -582,7 +592,7 @@ extern "C" int myelin_token_log_probs(const void *logits, int dtype, int64_t ld,
   if (!entropy || !stats || (top && (!top_log_probs || !top_tokens)) || (targets && !log_probs))
     return myelin::invalid("%s: null pointer", what);
   Args a{logits, ld, targets, ignore_index, targets ? log_probs : nullptr, entropy, stats, top_log_probs, top_tokens,
-         R, V, top, 1, V, nullptr, nullptr};
+         R, V, top, 1, V, R, nullptr, nullptr};
   if (!narrow(V, top)) {
     int64_t parts;
     split(R, V, &parts, &a.part);
@@ -615,7 +625,7 @@ extern "C" int myelin_token_log_probs_bwd(const void *logits, int dtype, int64_t
   if (R * ((V + kTile - 1) / kTile) > 0x7fffffff || (V < 256 && R * V / 256 >= 0x7fffffff))
     return myelin::invalid("%s: too many rows", what);
   BwdArgs a{logits, ld, targets, ignore_index, stats, entropy, targets ? grad_log_probs : nullptr, grad_entropy,
-            grad_logits, R, V, 1};
+            grad_logits, R, V, 1, R};
   if (dtype == 0)
     launch_bwd<F32>(a, myelin::as_hip(stream));
   else

@@ -331,3 +331,29 @@ def test_other_stream_and_graph_replays():
         for a, b in zip(held, eager):
             assert torch.equal(a, b)
         _ = float((x.detach().float() * 2.0).sum())
+
+
+@pytest.mark.parametrize("V", [62, 300])
+def test_more_rows_than_one_launch_dimension(V):
+    """Over 2^32 threads: rows past the first 2^32 / V are the same rows as alone."""
+
+    R = (2**32 if V < 256 else 2**32 // 256 * V) // V + 5
+    _case(test="log_probs_rows", R=R, V=V)
+    x = torch.zeros(R, V, dtype=torch.bfloat16, device=DEV)
+    rows = torch.tensor([0, 1, R // 2, R - 6, R - 5, R - 1], device=DEV)
+    x[rows] = _logits(len(rows), V, "bf16")[0]
+    targets = torch.zeros(R, dtype=torch.int64, device=DEV)
+    targets[rows] = torch.arange(len(rows), device=DEV) * 7
+    few = x[rows].clone().requires_grad_()
+    want = myelin.token_log_probs(few, targets[rows])
+    x.requires_grad_()
+    got = myelin.token_log_probs(x, targets)
+    (g,) = torch.autograd.grad(got[0].sum() + got[1].sum(), x)
+    (w,) = torch.autograd.grad(want[0].sum() + want[1].sum(), few)
+    for a, b in zip(got[:2], want[:2]):
+        a = a.detach().abs()
+        assert torch.equal(a[rows], b.abs())
+        a[rows] = math.log(V)
+        # every other row is uniform: log V, of terms that are exact but for its rounding
+        assert bool(((a - math.log(V)).abs() < 1e-5 + 1e-6 * math.log(V)).all())
+    assert torch.equal(g[rows], w)

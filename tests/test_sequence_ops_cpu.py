@@ -97,3 +97,15 @@ def test_attention_entry_points_validate():
         _lib.call(*step, None, 16, 16, 2, 4, 2, 8, 8, 1.0, None)
     with pytest.raises(ValueError, match="Dk and Dv"):
         _lib.call(*step, 16, 16, 16, 2, 4, 2, 8, 200, 1.0, None)
+
+
+def test_more_rows_than_a_launch_has_are_refused():
+    args = ("myelin_decay_attention_fwd", 16, 16, 16, 0, 16, 16, None, None, 16, 16)
+    with pytest.raises(ValueError, match="too many rows"):
+        _lib.call(*args, 1, 2**20 + 1, 2, 1, 8, 8, 1.0, None, 0, None)
+    step = ("myelin_decay_attention_step", 16, 16, 16, 0, 16, 16, 16, 16, 16)
+    with pytest.raises(ValueError, match="too many rows"):
+        _lib.call(*step, 2**21 + 1, 1, 1, 8, 8, 1.0, None)
+    # 2^34 elements are 2^24 workgroups of 4 a thread
+    with pytest.raises(ValueError, match="too many elements"):
+        _lib.call("myelin_counter_dropout", 16, 0, None, 16, 1, 2**34, 0, 1.0, 0, 0, None, None)
