@@ -399,3 +399,38 @@ def test_refusals():
     room = torch.zeros(s.numel() + 4, device=DEV)
     with pytest.raises(ValueError, match="not overlap"):
         g(*one, d, room[: s.numel()].view_as(s), out_state=room[4:].view_as(s))
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("which", ["q", "k", "v", "go"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,Dk,Dv", [(100, 20, 36), (300, 128, 128)])
+def test_a_value_reaches_no_step_before_it(T, Dk, Dv, dtype, which, bad):
+    """A NaN or an infinity in one step: outputs before it, and gradients that it
+    is not part of, are those of the formula, also within its chunk."""
+
+    _case(test="attention_causal", T=T, Dk=Dk, Dv=Dv, dtype=dtype, which=which, bad=bad)
+    q, k, v, d, s, go, gs = _inputs(T, 1, 2, 1, Dk, Dv, dtype)
+    clean = dict(q=q, k=k, v=v, go=go)
+    dirty = {n: t.clone() for n, t in clean.items()}
+    at = 77
+    dirty[which][at, 0, 0, Dk // 3] = bad
+    leaves = [dirty[n].requires_grad_() for n in ("q", "k", "v")] + [s.clone().requires_grad_()]
+    final, out = myelin.decay_attention(*leaves[:3], d, leaves[3])
+    got = (final, out, *torch.autograd.grad((final, out), leaves, (gs, dirty["go"])))
+    scale = Dk**-0.5
+    want = _reference(*leaves[:3], d, s, None, scale, dirty["go"], gs)
+    size = _reference(q.abs(), k.abs(), v.abs(), d, s.abs(), None, scale, go.abs(), gs.abs())
+    for name, a, w, z in zip(NAMES, got, want, size):
+        a = a.detach().double().cpu()
+        if "state" not in name:
+            # the formula's sums over a whole step: NaN in all that it is part of
+            w = torch.where(w.isfinite().all(-1, keepdim=True), w, math.nan) if name[0] == "g" else w
+        ok = w.isfinite()
+        _close(name, torch.where(ok, a, 0.0), torch.where(ok, w, 0.0), z, dtype)
+    first = dict(q=(1, slice(0, at)), k=(1, slice(0, at)), v=(1, slice(0, at)), go=(3, slice(at + 1, T)))[which]
+    assert bool(got[first[0]][first[1]].isfinite().all())
+    if which in ("q", "go"):  # gradients of later steps, and of every other step's q
+        assert bool(got[3][at + 1 :].isfinite().all()) and bool(got[4][at + 1 :].isfinite().all())
+    if which in ("k", "v"):
+        assert bool(got[2][:at].isfinite().all())
