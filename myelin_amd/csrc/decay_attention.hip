@@ -447,6 +447,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
     if constexpr (NW == 8) __builtin_amdgcn_s_setprio(1);
     Frag vf[CF];
     f32x4 o[CT];
+    bool strange = false;  // c holds an infinity or a NaN
     if (active) {
 #pragma unroll
       for (int f = 0; f < CF; ++f) vf[f] = E::column(sc + 32 * f * LV + 16 * w + col_v, LV);
@@ -470,6 +471,10 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
         }
 #pragma unroll
         for (int it = 0; it < CT; ++it) o[it] *= pw[16 * it + l16 + e] * o_scale;
+        float zero = 0.0f;
+#pragma unroll
+        for (int f = 0; f < CF; ++f) zero = E::zero_of(vf[f], zero);
+        strange = __any(zero != 0.0f);
       }
       // (a's rows later than the others: the registers of a X are free here)
       if (r0 + C < last) fetch_a(r0 + C);
@@ -525,12 +530,10 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
     if (!STATE_ONLY && active) {
       // A product takes 0 for the steps after its row: an infinity or a NaN in one of
       // them would reach the row as 0 * inf.  Where c has any they leave the product,
-      // and rows from their step on become NaN.  (2048 steps of 8 x 16 heads of 128,
-      // training, 374 -> 395 us; 32768 steps of 16 heads 235 -> 238.)
-      float zero = 0.0f;
-#pragma unroll
-      for (int f = 0; f < CF; ++f) zero = E::zero_of(vf[f], zero);
-      if (__builtin_expect(__any(zero != 0.0f), 0)) {
+      // and rows from their step on become NaN.  (Told by the dot products
+      // beside those of the state: behind the barrier 2048 steps of 8 x 16 heads of 128,
+      // training, took 395 us for 362.)
+      if (__builtin_expect(strange, 0)) {
         int ahead = l16 - 4 * g;  // (computed here: its operands would be kept over the loop)
         asm volatile("" : "+v"(ahead));
 #pragma unroll
