@@ -113,12 +113,22 @@ def counter_dropout(
 class CounterDropout(nn.Module):
     """``counter_dropout`` with a new mask for each training call.
 
-    The count of calls is a buffer (``offset``), saved with the module and
-    advanced on the device, so that a captured training step draws a new mask at
-    each replay.  In evaluation mode the input passes, plus ``residual``.
+    Without a ``seed`` each call takes its offset from torch's generator of the
+    input's device, as ``nn.Dropout`` takes its mask: ``torch.manual_seed``
+    decides the masks, modules have masks of their own, a captured graph draws a
+    new one at each replay, and ``torch.utils.checkpoint``, which puts the
+    generator back, computes the forward pass again under the same mask.
+
+    With a ``seed`` the masks are those of the calls 1, 2, ... of this seed,
+    whatever else draws random numbers; modules that must not share masks have
+    seeds of their own, as have the ranks of a data-parallel run.  The count of
+    calls is a buffer (``offset``), saved with the module and advanced on the
+    device, so that a captured training step draws a new mask at each replay.
+
+    In evaluation mode the input passes, plus ``residual``.
     """
 
-    def __init__(self, p: float, seed: int = 0, time_shared: bool = False) -> None:
+    def __init__(self, p: float, seed: int | None = None, time_shared: bool = False) -> None:
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p must be in [0, 1]; got {p}")
@@ -130,7 +140,10 @@ class CounterDropout(nn.Module):
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         if not self.training:
             return x if residual is None else x + residual
-        # a tensor of this call's own: the backward pass reads it again
-        offset = self.offset + 1
-        self.offset.copy_(offset)
-        return counter_dropout(x, self.p, self.seed, offset, residual=residual, time_shared=self.time_shared)
+        # the offset is a tensor of this call's own: the backward pass reads it again
+        if self.seed is None:
+            seed, offset = 0, torch.randint(2**63 - 1, (1,), device=x.device)
+        else:
+            seed, offset = self.seed, self.offset + 1
+            self.offset.copy_(offset)
+        return counter_dropout(x, self.p, seed, offset, residual=residual, time_shared=self.time_shared)
