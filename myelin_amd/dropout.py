@@ -124,6 +124,8 @@ class CounterDropout(nn.Module):
     seeds of their own, as have the ranks of a data-parallel run.  The count of
     calls is a buffer (``offset``), saved with the module and advanced on the
     device, so that a captured training step draws a new mask at each replay.
+    A forward pass that a backward pass computes again would draw the next mask
+    and is refused: checkpointed layers take no seed.
 
     In evaluation mode the input passes, plus ``residual``.
     """
@@ -144,6 +146,10 @@ class CounterDropout(nn.Module):
         if self.seed is None:
             seed, offset = 0, torch.randint(2**63 - 1, (1,), device=x.device)
         else:
+            if torch._C._current_graph_task_id() != -1:
+                raise RuntimeError("CounterDropout with a seed counts its calls, and this one computes a forward pass "
+                                   "again within a backward pass, which would change its mask; leave the seed out, or "
+                                   "call counter_dropout with the first pass's offset")
             seed, offset = self.seed, self.offset + 1
             self.offset.copy_(offset)
         return counter_dropout(x, self.p, seed, offset, residual=residual, time_shared=self.time_shared)

@@ -8,6 +8,7 @@ import math
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import myelin_amd as myelin
 from myelin_amd import dropout
@@ -72,3 +73,35 @@ def test_evaluation_draws_nothing(seed, host_dropout):
     before = torch.get_rng_state()
     assert torch.equal(drop(x), x) and torch.equal(drop(x, r), x + r)
     assert not host_dropout and int(drop.offset) == 0 and torch.equal(torch.get_rng_state(), before)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_checkpointed_layer_keeps_its_mask(reentrant, host_dropout):
+    """Two checkpointed calls of one module, then the backward pass of both, which
+    computes the second first: the gradient is the forward pass's own.  (Whole
+    numbers, whose sums are exact in any order.)"""
+
+    torch.manual_seed(5)
+    drop = myelin.CounterDropout(0.5)
+    x = torch.arange(1.0, 101.0).requires_grad_()
+    square = lambda t: drop(t * t)  # noqa: E731
+    a = torch.utils.checkpoint.checkpoint(square, x, use_reentrant=reentrant)
+    b = torch.utils.checkpoint.checkpoint(square, x, use_reentrant=reentrant)
+    (a.sum() + 3.0 * b.sum()).backward()
+    first, second = host_dropout[:2]
+    assert not torch.equal(first, second)
+    assert torch.equal(x.grad, 4.0 * x.detach() * first + 12.0 * x.detach() * second)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_counted_mask_is_not_drawn_again(reentrant, host_dropout):
+    drop = myelin.CounterDropout(0.5, seed=8)
+    x = torch.randn(100, requires_grad=True)
+    y = torch.utils.checkpoint.checkpoint(lambda t: drop(t * t), x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="leave the seed out"):
+        y.sum().backward()
+    assert int(drop.offset) == 1
+    drop.eval()  # passes in a backward pass too
+    y = torch.utils.checkpoint.checkpoint(lambda t: drop(t * t), x, use_reentrant=reentrant)
+    y.sum().backward()
+    assert torch.equal(x.grad, 2.0 * x.detach())

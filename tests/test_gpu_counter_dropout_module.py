@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import myelin_amd as myelin
 
@@ -64,3 +65,38 @@ def test_a_captured_graph_draws_at_each_replay():
     for i, a in enumerate(masks):
         for b in masks[:i]:
             assert abs(int((a == b).sum()) - n // 2) <= 5 * 128
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_checkpointed_layer_keeps_its_mask(reentrant):
+    """The same bits as without checkpointing."""
+
+    print(f"case: test=counter_dropout_checkpoint reentrant={reentrant}", flush=True)
+    x, w = torch.randn(64, 512, device=DEV), torch.randn(512, 512, device=DEV)
+    drops = [myelin.CounterDropout(0.5).to(DEV) for _ in range(2)]
+
+    def layer(drop, t, weight):
+        return drop(torch.tanh(t @ weight), t)
+
+    def step(call):
+        torch.manual_seed(6)
+        leaves = [t.clone().requires_grad_() for t in (x, w)]
+        y = call(drops[1], call(drops[0], leaves[0], leaves[1]), leaves[1])
+        y.square().sum().backward()
+        return y.detach(), [t.grad for t in leaves]
+
+    y0, g0 = step(layer)
+    y1, g1 = step(lambda *a: torch.utils.checkpoint.checkpoint(layer, *a, use_reentrant=reentrant))
+    assert torch.equal(y0, y1)
+    for a, b in zip(g0, g1):
+        assert torch.equal(a, b)
+
+
+def test_a_counted_mask_is_not_drawn_again():
+    print("case: test=counter_dropout_checkpoint_counted", flush=True)
+    drop = myelin.CounterDropout(0.5, seed=8).to(DEV)
+    x = torch.randn(100, device=DEV, requires_grad=True)
+    y = torch.utils.checkpoint.checkpoint(lambda t: drop(t * t), x, use_reentrant=False)
+    with pytest.raises(RuntimeError, match="leave the seed out"):
+        y.sum().backward()
+    assert int(drop.offset) == 1
