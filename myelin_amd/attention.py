@@ -183,9 +183,7 @@ def decay_attention(
     if autograd.plain(q, k, v) and (initial_state is None or autograd.plain(initial_state)):
         state, out = autograd.native().decay_attention(q, k, v, decay, initial_state, lengths, scale)
         return state, out
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, initial_state)):
-        return HipDecayAttentionFunction.apply(q, k, v, decay, initial_state, lengths, scale)
-    return _forward(q, k, v, decay, initial_state, lengths, scale)
+    return HipDecayAttentionFunction.apply(q, k, v, decay, initial_state, lengths, scale)
 
 
 def decay_attention_step(
@@ -210,6 +208,7 @@ def decay_attention_step(
     scale = _scale(scale, q)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
         raise ValueError("decay_attention_step has no gradient; use decay_attention, or torch.no_grad()")
+    autograd.refuse_tangents("decay_attention_step", q, k, v, decay, state)
     state = state.contiguous()
     if out_state is not None:
         _check_state(out_state, q, v, "out_state")

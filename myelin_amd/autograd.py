@@ -72,6 +72,13 @@ def plain(*tensors: torch.Tensor) -> bool:
             and all(type(t) in _PLAIN for t in tensors))
 
 
+def refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
+    """For calls without a Function: a forward-mode tangent would be lost."""
+
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} has no forward-mode derivative")
+
+
 def lif(x, m0, decay, threshold, reset, slope, rule, sid):
     """(final membrane, spikes) of HipLIFFunction."""
 

@@ -105,9 +105,7 @@ def counter_dropout(
     if autograd.plain(x) and (residual is None or autograd.plain(residual)):
         at, number = (offset, 0) if isinstance(offset, torch.Tensor) else (None, offset)
         return autograd.native().counter_dropout(x, residual, at, steps, threshold, scale, seed, number)
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return HipCounterDropoutFunction.apply(x, residual, steps, threshold, scale, seed, offset)
-    return _launch(x, residual, steps, threshold, scale, seed, offset)
+    return HipCounterDropoutFunction.apply(x, residual, steps, threshold, scale, seed, offset)
 
 
 class CounterDropout(nn.Module):

@@ -122,10 +122,8 @@ def token_log_probs(
         log_probs = None if targets is None else next(results)
         entropy = next(results)
         top_lp, top_tok = (next(results), next(results)) if top else (None, None)
-    elif torch.is_grad_enabled() and x.requires_grad:
-        log_probs, entropy, top_lp, top_tok = HipTokenLogProbsFunction.apply(x, targets, top, ignore_index)
     else:
-        log_probs, entropy, _, top_lp, top_tok = _forward(x, targets, top, ignore_index)
+        log_probs, entropy, top_lp, top_tok = HipTokenLogProbsFunction.apply(x, targets, top, ignore_index)
     if len(lead) == 1:
         return TokenLogProbs(log_probs, entropy, top_lp, top_tok)
     return TokenLogProbs(
