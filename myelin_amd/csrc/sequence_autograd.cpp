@@ -299,6 +299,8 @@ variable_list decay_attention_step(const Tensor &q, const Tensor &k, const Tenso
   check(lib.attention_step(at(q), at(k), at(v), code_of(q), strides_of({q, k, v}).data(), f32(decay), f32(state),
                            at(out), f32(to), B, H, Hk, Dk, Dv, static_cast<float>(scale), stream_of(q)),
         "myelin_decay_attention_step");
+  // autograd notices where it keeps out_state for a backward pass
+  if (out_state.has_value() && !to.is_inference()) to.unsafeGetTensorImpl()->bump_version();
   return {to, out};
 }
 

@@ -434,3 +434,30 @@ def test_a_value_reaches_no_step_before_it(T, Dk, Dv, dtype, which, bad):
         assert bool(got[3][at + 1 :].isfinite().all()) and bool(got[4][at + 1 :].isfinite().all())
     if which in ("k", "v"):
         assert bool(got[2][:at].isfinite().all())
+
+
+@pytest.mark.parametrize("kind", [torch.Tensor, torch.nn.Parameter])
+def test_a_state_advanced_in_place_is_noticed(kind):
+    """The backward pass of a sequence reads its initial state again."""
+
+    _case(test="attention_state_version", kind=kind.__name__)
+    q, k, v, d, s, go, _ = _inputs(20, 2, 2, 2, 8, 8, "fp32")
+    if kind is torch.nn.Parameter:
+        s = torch.nn.Parameter(s, requires_grad=False)
+    q.requires_grad_()
+    _, out = myelin.decay_attention(q, k, v, d, s)
+    _, kept = myelin.decay_attention(q, k, v, d, s[:, :])
+    with torch.no_grad():
+        other, _ = myelin.decay_attention_step(q[0], k[0], v[0], d, s)  # a new tensor: nothing has changed
+        assert other is not s
+        torch.autograd.grad(out, q, go, retain_graph=True)
+        myelin.decay_attention_step(q[0], k[0], v[0], d, s, out_state=s)
+    for o in (out, kept):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(o, q, go)
+    with torch.inference_mode():  # tensors without a version
+        a, b = (t.clone() for t in (s.detach(), s.detach()))
+        one = (q[0].clone(), k[0].clone(), v[0].clone(), d.clone())
+        new, _ = myelin.decay_attention_step(*one, a)
+        myelin.decay_attention_step(*one, b, out_state=b)
+        assert torch.equal(new, b)
