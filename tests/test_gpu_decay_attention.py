@@ -461,3 +461,18 @@ def test_a_state_advanced_in_place_is_noticed(kind):
         new, _ = myelin.decay_attention_step(*one, a)
         myelin.decay_attention_step(*one, b, out_state=b)
         assert torch.equal(new, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,H,Hk,Dk,Dv", [(300, 2, 2, 128, 128), (2100, 2, 1, 64, 40)])
+def test_gradients_do_not_depend_on_which_are_asked_for(T, H, Hk, Dk, Dv, dtype):
+    _case(test="attention_which_gradients", T=T, Dk=Dk, Dv=Dv, dtype=dtype)
+    q, k, v, d, s, go, gs = _inputs(T, 2, H, Hk, Dk, Dv, dtype)
+    every = None
+    for wanted in ((0, 1, 2, 3), (0, 1, 2), (0,), (1, 3)):
+        leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate((q, k, v, s))]
+        final, out = myelin.decay_attention(*leaves[:3], d, leaves[3])
+        grads = dict(zip(wanted, torch.autograd.grad((final, out), [leaves[i] for i in wanted], (gs, go))))
+        every = every or grads
+        for i, g in grads.items():
+            assert torch.equal(g, every[i]), NAMES[2 + i]
