@@ -148,7 +148,7 @@ struct Problem {
   int64_t sk, sv;
   int KD, VD;
   int ga, gb, gc;  // query heads to a head of a, b, c
-  float in_scale, out_scale, o_scale;
+  float s_scale, x_scale, c_scale;  // of a b^T, of a X, of the c that are added to X
   int reverse, o_f32;
 };
 
@@ -184,8 +184,10 @@ __device__ __forceinline__ float power(float d, int64_t n) {
 // The recurrence by chunks of C steps.  With X the state before a chunk (after
 // it, reversed), rows i, j of the chunk in the order of the recurrence and e =
 // 1 - reverse:
-//   o_i = d^(i + e) a_i X + sum_{j <= i} d^(i - j) (a_i . b_j) c_j
-//   X'  = d^C X + sum_j d^(C - j - e) b_j c_j^T
+//   o_i = x d^(i + e) a_i X + s sum_{j <= i} d^(i - j) (a_i . b_j) c_j
+//   X'  = d^C X + c sum_j d^(C - j - e) b_j c_j^T
+// with the scales (s, x, c) = (scale, scale, 1) where X is the state and (scale, 1,
+// scale) where it is the state's gradient.
 // A workgroup has one (problem, b, h), a slice of 16 columns of X for each of
 // its NW waves and a segment of the steps; wave w has columns 16 w .. 16 w + 15
 // of the slice in the accumulators of its products, which are
@@ -242,7 +244,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
   __shared__ __attribute__((aligned(16))) T sc[C * LV];
   __shared__ __attribute__((aligned(16))) T sp[STATE_ONLY ? 1 : C * LP];  // scaled a b^T
   __shared__ __attribute__((aligned(16))) float pw[C + 4];                // d^n
-  __shared__ __attribute__((aligned(16))) float weight[C];                // of c_j in a whole chunk
+  __shared__ __attribute__((aligned(16))) float weight[C];                // of c_j in a whole chunk: c d^(C - j - e)
 
   // workgroups of one (b, h) run on one XCD, whose L2 the problems share
   const uint32_t id = blockIdx.x, rest = id >> 3;
@@ -265,7 +267,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
   const int64_t at = p.at, bt = p.bt, ct = p.ct, ot = p.ot;
   const int kd = p.KD, vd = p.VD - first < VD ? p.VD - first : VD;
   const bool o_f32 = p.o_f32;
-  const float o_scale = p.o_scale;
+  const float s_scale = p.s_scale, x_scale = p.x_scale;
   char *po = static_cast<char *>(p.o) + (b * p.ob + h * p.oh + first) * (o_f32 ? 4 : sizeof(T));
   const int64_t begin = seg * args.segment;
   const int64_t end = begin + args.segment < args.T ? begin + args.segment : args.T;
@@ -275,7 +277,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
   const int e = reverse ? 0 : 1;
 
   if (tid <= C) pw[tid] = power(d, tid);
-  if (tid < C) weight[tid] = power(d, C - tid - e);
+  if (tid < C) weight[tid] = power(d, C - tid - e) * p.c_scale;
   if constexpr (!STATE_ONLY)  // blocks right of the diagonal stay zero
     for (int i = tid; i < C * LP; i += NT) sp[i] = T(0.0f);
 
@@ -383,7 +385,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int k = 16 * t + 4 * g + r;
-          if (k < p.KD && col < p.VD) X[t][r] = p.s_in[state + k * p.sk + col * p.sv] * p.in_scale;
+          if (k < p.KD && col < p.VD) X[t][r] = p.s_in[state + k * p.sk + col * p.sv];
         }
       }
     }
@@ -435,7 +437,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
           if (!past(f)) E::mma(s, x[f], y[f]);
           if (!past(f + 1)) E::mma(s1, x[f + 1], y[f + 1]);
         }
-        s = (s + s1) * o_scale;
+        s = (s + s1) * s_scale;
         four z;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -473,7 +475,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
             for (int it = 0; it < CT; ++it) E::mma(o[it], xf[k], af[it]);
         }
 #pragma unroll
-        for (int it = 0; it < CT; ++it) o[it] *= pw[16 * it + l16 + e] * o_scale;
+        for (int it = 0; it < CT; ++it) o[it] *= pw[16 * it + l16 + e] * x_scale;
         float zero = 0.0f;
 #pragma unroll
         for (int f = 0; f < CF; ++f) zero = E::zero_of(vf[f], zero);
@@ -496,8 +498,8 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const int x = c - j0 - r - e;
-              wt[half][r] = pw[x > 0 ? x : 0];
+              const int x = C - c + j0 + r;  // (rows past the last step are zero)
+              wt[half][r] = weight[x < C ? x : C - 1];
             }
           }
         }
@@ -613,7 +615,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int k = 16 * t + 4 * g + r;
-          if (k < p.KD) p.s_out[state + k * p.sk + col * p.sv] = X[t][r] * p.out_scale;
+          if (k < p.KD) p.s_out[state + k * p.sk + col * p.sv] = X[t][r];
         }
     }
   }
@@ -634,7 +636,7 @@ __global__ __launch_bounds__(256) void join_segments(Args args) {
   float *x = args.ends + ((blockIdx.z * args.B * args.H + bh) * (args.segments - 1)) * SIZE + at;
   const float d = args.decay[bh % args.H];
   const int64_t n = steps_of(args, bh / args.H);
-  float s = (p.s_in && k < p.KD && col < p.VD) ? p.s_in[bh * p.KD * p.VD + k * p.sk + col * p.sv] * p.in_scale : 0.0f;
+  float s = (p.s_in && k < p.KD && col < p.VD) ? p.s_in[bh * p.KD * p.VD + k * p.sk + col * p.sv] : 0.0f;
   const float whole = power(d, args.segment);
   for (int64_t seg = 0; seg + 1 < args.segments; seg += AHEAD, x += AHEAD * SIZE) {
     const int m = args.segments - 1 - seg < AHEAD ? static_cast<int>(args.segments - 1 - seg) : AHEAD;
@@ -888,7 +890,7 @@ Problem problem(const void *a, const int64_t *as, const void *b, const int64_t *
   p.ot = B * H * VD, p.ob = H * VD, p.oh = VD;
   p.KD = KD, p.VD = VD;
   p.ga = p.gb = p.gc = 1;
-  p.in_scale = p.out_scale = p.o_scale = 1.0f;
+  p.s_scale = p.x_scale = p.c_scale = 1.0f;
   return p;
 }
 
@@ -921,7 +923,7 @@ extern "C" int myelin_decay_attention_fwd(const void *q, const void *k, const vo
   p = problem(q, strides, k, strides + 3, v, strides + 6, out, B, H, static_cast<int>(Dk), static_cast<int>(Dv));
   p.gb = p.gc = static_cast<int>(H / Hk);
   p.s_in = state, p.s_out = state_out, p.sk = Dv, p.sv = 1;
-  p.o_scale = scale;
+  p.s_scale = p.x_scale = scale;
   const int64_t need = myelin_decay_attention_workspace_elems(dtype, T, B, H, Hk, Dk, Dv, 0);
   if (int rc = check_workspace(what, workspace, workspace_elems, need)) return rc;
   if (dtype == 0)
@@ -953,9 +955,8 @@ extern "C" int myelin_decay_attention_bwd(const void *q, const void *k, const vo
   pq = problem(grad_out, gs, v, vs, k, ks, grad_q, B, H, dv, dk);
   pq.gb = pq.gc = group;
   pq.s_in = state, pq.sk = 1, pq.sv = Dv;
-  // dk = RLA(v, do, scale q), dv = RLA(k, scale q, do), both from dS_T: with
-  // the scale taken out of the whole, its share of dS_T is divided by it
-  // (the segments' states first: they are read 16 bytes at a time)
+  // dk = RLA(v, do, scale q), dv = RLA(k, scale q, do), both from dS_T
+  // (in the workspace the segments' states come first: they are read 16 bytes at a time)
   float *per_head = group > 1 ? workspace + need - T * B * H * (Dk + Dv) : nullptr;
   void *to_k = group > 1 ? static_cast<void *>(per_head) : grad_k;
   void *to_v = group > 1 ? static_cast<void *>(per_head + T * B * H * Dk) : grad_v;
@@ -965,9 +966,8 @@ extern "C" int myelin_decay_attention_bwd(const void *q, const void *k, const vo
   pv = problem(k, ks, q, qs, grad_out, gs, to_v, B, H, dk, dv);
   pv.ga = group;
   pv.s_in = grad_state_out, pv.s_out = grad_state, pv.sk = Dv, pv.sv = 1;
-  pq.o_scale = pk.o_scale = pv.o_scale = scale;
-  pk.in_scale = pv.in_scale = 1.0f / scale;
-  pv.out_scale = scale;
+  pq.s_scale = pk.s_scale = pv.s_scale = scale;
+  pq.x_scale = pk.c_scale = pv.c_scale = scale;
   pk.reverse = pv.reverse = 1;
   pk.o_f32 = pv.o_f32 = group > 1;
   const hipStream_t s = myelin::as_hip(stream);

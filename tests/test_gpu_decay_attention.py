@@ -476,3 +476,16 @@ def test_gradients_do_not_depend_on_which_are_asked_for(T, H, Hk, Dk, Dv, dtype)
         every = every or grads
         for i, g in grads.items():
             assert torch.equal(g, every[i]), NAMES[2 + i]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [1e-30, 1e-39, -3e-42])
+@pytest.mark.parametrize("T", [70, 1300])
+def test_small_scales(T, scale, dtype):
+    """Nothing is divided by the scale: a state's gradient of 1e9 passes through at
+    any.  (Terms that the scale makes smaller than 2^-126 may be lost: 1e-38 of
+    sums that are held to 1e-30.)"""
+
+    _case(test="attention_small_scale", T=T, scale=scale, dtype=dtype)
+    q, k, v, d, s, go, gs = _inputs(T, 2, 2, 1, 24, 40, dtype)
+    _check(q, k, v, d, s, None, dtype, go, gs * 1e9, scale=scale)
