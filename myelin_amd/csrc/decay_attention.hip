@@ -405,9 +405,11 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
   }
 
   // Blocks of 32 rows of X past the width.  fp32's products take long enough for
-  // this to pay (100 steps of 4 x 4 heads of 32: 19.2 -> 17.0 us); in the bf16
-  // kernels the branches cost more than the products.
-  const auto past = [&](int f) { return E::PARTS == 1 && 32 * f >= kd; };
+  // this to pay (100 steps of 4 x 4 heads of 32: 19.2 -> 17.0 us; 501 of 16 x 8
+  // heads of 50 and 75, training, 351 -> 296 us); in the bf16 kernels the branches
+  // cost more than the products, and in fp32's of whole rows past 64 they cost 114
+  // spilled registers (1024 steps of 4 x 16 heads of 128, training, 317 -> 488 us).
+  const auto past = [&](int f) { return E::PARTS == 1 && (KT == 4 || !WHOLE) && 32 * f >= kd; };
 
   // where a lane's fragments start: of row l16, and of a column block
   const int at_row = E::at(l16, 4 * g, 0), at_col = E::column_at(lane, 0);
