@@ -246,15 +246,19 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
   __shared__ __attribute__((aligned(16))) float pw[C + 4];                // d^n
   __shared__ __attribute__((aligned(16))) float weight[C];                // of c_j in a whole chunk: c d^(C - j - e)
 
-  // workgroups of one (b, h) run on one XCD, whose L2 the problems share
+  // Workgroups go to the 8 XCDs in turn.  Those of one (b, h) and segment run on one
+  // of them, whose L2 the problems and slices share; (b, h) and segments together
+  // are dealt out evenly (32768 steps of 128, bf16, 1 head 56 us, 12 heads 190; by
+  // (b, h) alone 124 and 247).
   const uint32_t id = blockIdx.x, rest = id >> 3;
   const int which = static_cast<int>(rest % args.problems);
   const Problem &p = args.p[which];
-  const int64_t heads = (args.B * args.H + 7) / 8, r1 = rest / args.problems, r2 = r1 / args.slices;
+  const uint32_t heads = static_cast<uint32_t>(args.B * args.H), r1 = rest / args.problems;
   const int slice = static_cast<int>(r1 % args.slices), first = slice * VD;  // its first column
-  const int64_t bh = (r2 % heads) * 8 + (id & 7), seg = r2 / heads;
+  const uint32_t unit = r1 / args.slices * 8 + (id & 7);
+  const int64_t bh = __builtin_amdgcn_readfirstlane(unit % heads), seg = __builtin_amdgcn_readfirstlane(unit / heads);
   if (first >= p.VD) return;
-  if (bh >= args.B * args.H) return;
+  if (seg >= args.segments - (STATE_ONLY ? 1 : 0)) return;
   const int64_t b = bh / args.H, h = bh % args.H;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, l16 = lane & 15;
@@ -571,7 +575,12 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
         for (int it = 2 * f; it < CT; ++it) E::mma(o[it], vf[f], E::row(sp + 16 * it * LP + 32 * f + row_p));
       // row i of the chunk, columns 16 w + 4 g .. + 3
       char *out = po + (reverse ? n - r0 - c : r0) * ot * (o_f32 ? 4 : sizeof(T));
-      const int oc = 16 * w + 4 * g;
+      // (16 w + 4 g, counted anew: kept over the loop it is spilled in the 8-wave
+      // kernels, and its load back waits for the rows that are on their way: 2048
+      // steps of 8 x 16 heads of 128, training, 372 us for 337)
+      uint32_t all = ~0u;
+      asm volatile("" : "+v"(all));
+      const int oc = 16 * w + 4 * static_cast<int>(__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0)) >> 4);
 #pragma unroll
       for (int it = 0; it < CT; ++it) {
         const int i = 16 * it + l16;
@@ -797,16 +806,18 @@ int64_t ends_elems(int dtype, int64_t T, int64_t BH, int problems, Shape sh) {
 
 template <class E, int KT, int NW, bool WHOLE>
 void launch_shape(const Args &a, bool exact, hipStream_t s) {
-  const int64_t groups = (a.B * a.H + 7) / 8 * 8 * a.problems * a.slices;
+  const auto groups = [&](int64_t segments) {
+    return static_cast<unsigned>((a.B * a.H * segments + 7) / 8 * 8 * a.problems * a.slices);
+  };
   if (a.segments > 1) {
     // (the last segment's end is nobody's start)
-    chunked<E, KT, NW, WHOLE, true, true><<<static_cast<unsigned>(groups * (a.segments - 1)), 64 * NW, 0, s>>>(a);
+    chunked<E, KT, NW, WHOLE, true, true><<<groups(a.segments - 1), 64 * NW, 0, s>>>(a);
     if (a.joined) {
       const dim3 grid(KT * NW, static_cast<unsigned>(a.B * a.H), a.problems * a.slices);
       join_segments<KT, NW><<<grid, 256, 0, s>>>(a);
     }
   }
-  const unsigned grid = static_cast<unsigned>(groups * a.segments);
+  const unsigned grid = groups(a.segments);
   if constexpr (E::PARTS == 3) {
     if (!exact) {
       chunked<E, KT, NW, WHOLE, false, false><<<grid, 64 * NW, 0, s>>>(a);

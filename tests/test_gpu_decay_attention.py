@@ -489,3 +489,29 @@ def test_small_scales(T, scale, dtype):
     _case(test="attention_small_scale", T=T, scale=scale, dtype=dtype)
     q, k, v, d, s, go, gs = _inputs(T, 2, 2, 1, 24, 40, dtype)
     _check(q, k, v, d, s, None, dtype, go, gs * 1e9, scale=scale)
+
+
+def test_few_heads_use_the_whole_chip():
+    """A long prompt of 2 heads has an eighth of the work of 16, which fill the
+    chip, and more of its time in launches: held to 0.4 of theirs (0.26 measured;
+    on two of the eight XCDs 0.54)."""
+
+    _case(test="attention_few_heads")
+
+    def microseconds(heads):
+        q, k, v, d, _, _, _ = _inputs(32768, 1, heads, heads, 128, 128, "bf16", state=False)
+        times = []
+        for _ in range(8):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            for _ in range(10):
+                myelin.decay_attention(q, k, v, d)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(start.elapsed_time(end) * 100.0)
+        return min(times)
+
+    with torch.no_grad():
+        few, many = microseconds(2), microseconds(16)
+    print(f"2 heads {few:.0f} us, 16 heads {many:.0f} us", flush=True)
+    assert few <= 0.4 * many
