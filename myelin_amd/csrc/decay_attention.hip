@@ -221,7 +221,7 @@ constexpr int lds_bytes(int kt, int waves) {
 
 // Registers bound how many waves a CU holds: with whole rows 8 waves to a
 // workgroup fit 128, so that two of them share it, and 4 fit 168, for three.
-[[maybe_unused]] constexpr int waves_per_simd(int waves, int lds, bool whole) {
+constexpr int waves_per_simd(int waves, int lds, bool whole) {
   return !whole ? 2 : waves == 8 ? 4 : 160 * 1024 / lds < 3 ? 2 : 3;
 }
 
@@ -771,16 +771,20 @@ void launch_step(const StepArgs &a, unsigned grid, hipStream_t s) {
 // How a call is cut, by its widest problem: the padded KD (16 kt), slices of 16
 // nw columns, and the workgroups that the chip holds of it.  For bf16 of both
 // widths past 64 one workgroup of 8 waves has all columns, since each forms the
-// whole of a b^T; the others' smaller workgroups fill the chip more evenly, and
-// three share a CU (501 steps of 16 x 8 heads of 50 and 75, fp32, training: 258
-// -> 220 us; 1021 of 8 x 16 heads of 64 and 96, bf16: 59 -> 56 us; but 2048 of 8
-// x 16 heads of 128, bf16, training: 380 -> 390 us).
+// whole of a b^T; the others' smaller workgroups fill the chip more evenly (501
+// steps of 16 x 8 heads of 50 and 75, fp32, training: 258 -> 220 us; 1021 of 8 x
+// 16 heads of 64 and 96, bf16: 59 -> 56 us; but 2048 of 8 x 16 heads of 128, bf16,
+// training: 380 -> 390 us), three to a CU where its LDS holds them, else two.
+// (Element-wise kernels are counted as the others, though their registers hold
+// two: whether rows are whole is not known where the workspace is asked for.)
 struct Shape {
   int kt, nw, slices, places;
 };
 Shape shape_of(int dtype, int kd, int vd) {
-  if (dtype != 0 && kd > 64 && vd > 64) return {8, 8, 1, 512};
-  return {kd <= 64 ? 4 : 8, 4, (vd + 63) / 64, 768};
+  const bool all = dtype != 0 && kd > 64 && vd > 64;
+  const int kt = kd <= 64 ? 4 : 8, nw = all ? 8 : 4;
+  const int lds = dtype == 0 ? lds_bytes<F32>(kt, nw) : lds_bytes<BF16>(kt, nw);
+  return {kt, nw, all ? 1 : (vd + 63) / 64, 256 * 4 * waves_per_simd(nw, lds, true) / nw};
 }
 
 // Segments of the time axis: as many as fill the workgroups' places,

@@ -109,3 +109,19 @@ def test_more_rows_than_a_launch_has_are_refused():
     # 2^34 elements are 2^24 workgroups of 4 a thread
     with pytest.raises(ValueError, match="too many elements"):
         _lib.call("myelin_counter_dropout", 16, 0, None, 16, 1, 2**34, 0, 1.0, 0, 0, None, None)
+
+
+def test_attention_is_cut_for_the_workgroups_that_fit():
+    """Segments' states in the workspace: one less than the workgroups that the 256
+    CUs hold of a (b, h).  Two of 57,600 bytes of LDS share a CU (bf16, keys past 64,
+    values not), three of 41,216 and 47,360, two of 8 waves."""
+
+    def segments(dtype, Dk, Dv, heads):
+        kt, vt = (64 if Dk <= 64 else 128), (128 if dtype and Dk > 64 and Dv > 64 else 64)
+        n = _lib.load().myelin_decay_attention_workspace_elems(dtype, 3 * 2**18, 1, heads, heads, Dk, Dv, 0)
+        assert n % (heads * kt * vt) == 0
+        return n // (heads * kt * vt) + 1
+
+    assert segments(2, 128, 64, 1) == 512 and segments(2, 64, 64, 1) == 768 and segments(2, 128, 128, 1) == 512
+    assert segments(0, 64, 64, 1) == 768 and segments(0, 128, 64, 1) == 768
+    assert segments(2, 128, 64, 4) == 128
