@@ -228,8 +228,8 @@ class DecayAttention(nn.Module):
     """The decays of a layer's heads, and attention with them.
 
     ``taus`` gives each head's time constant in steps (``decay = 1 - 1 / tau``,
-    as ``LIFParams``; ``math.inf`` never forgets).  ``forward`` takes whole
-    sequences, ``step`` one step.
+    as ``LIFParams``; ``math.inf`` never forgets), kept in float32 whatever type the
+    module is cast to.  ``forward`` takes whole sequences, ``step`` one step.
     """
 
     def __init__(self, taus: Sequence[float], scale: float | None = None) -> None:
@@ -239,6 +239,13 @@ class DecayAttention(nn.Module):
         self.scale = scale
         decay = torch.tensor([1.0 - 1.0 / t for t in taus], dtype=torch.float64)
         self.register_buffer("decay", decay.to(torch.float32))
+
+    def _apply(self, fn, recurse: bool = True):
+        decay = self.decay
+        super()._apply(fn, recurse)
+        if self.decay.dtype != decay.dtype:  # in bfloat16 a decay of 1 - 1 / 1024 is 1
+            self.decay = decay.to(self.decay.device)
+        return self
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, initial_state: torch.Tensor | None = None,
                 lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:

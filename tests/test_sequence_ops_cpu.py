@@ -125,3 +125,13 @@ def test_attention_is_cut_for_the_workgroups_that_fit():
     assert segments(2, 128, 64, 1) == 512 and segments(2, 64, 64, 1) == 768 and segments(2, 128, 128, 1) == 512
     assert segments(0, 64, 64, 1) == 768 and segments(0, 128, 64, 1) == 768
     assert segments(2, 128, 64, 4) == 128
+
+
+def test_a_cast_module_keeps_its_decays():
+    want = torch.tensor([0.75, 1 - 1 / 1024, 1.0])
+    for cast in (lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.double(),
+                 lambda m: m.to(torch.bfloat16).float()):
+        model = cast(torch.nn.Sequential(myelin.DecayAttention([4.0, 1024.0, float("inf")]), torch.nn.Linear(2, 2)))
+        assert torch.equal(model[0].decay, want) and "0.decay" in model.state_dict()
+    assert model.to("meta")[0].decay.device.type == "meta"
+    assert model.to(torch.bfloat16)[0].decay.dtype == torch.float32
