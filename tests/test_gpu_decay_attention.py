@@ -515,3 +515,28 @@ def test_few_heads_use_the_whole_chip():
         few, many = microseconds(2), microseconds(16)
     print(f"2 heads {few:.0f} us, 16 heads {many:.0f} us", flush=True)
     assert few <= 0.4 * many
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("which", ["q", "k", "v", "go"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,Dk,Dv", [(100, 20, 36), (300, 128, 128)])
+def test_a_value_is_not_lost(T, Dk, Dv, dtype, which, bad):
+    """A NaN or an infinity in one step: wherever the formula has one, in its own
+    chunk and in later ones, the results have."""
+
+    _case(test="attention_not_lost", T=T, Dk=Dk, Dv=Dv, dtype=dtype, which=which, bad=bad)
+    q, k, v, d, s, go, gs = _inputs(T, 1, 2, 1, Dk, Dv, dtype)
+    dirty = {n: t.clone() for n, t in dict(q=q, k=k, v=v, go=go).items()}
+    at = 77
+    dirty[which][at, 0, 0, Dk // 3] = bad
+    leaves = [dirty[n].requires_grad_() for n in ("q", "k", "v")] + [s.clone().requires_grad_()]
+    final, out = myelin.decay_attention(*leaves[:3], d, leaves[3])
+    got = (final, out, *torch.autograd.grad((final, out), leaves, (gs, dirty["go"])))
+    want = _reference(*leaves[:3], d, s, None, Dk**-0.5, dirty["go"], gs)
+    reached = {"q": ("out", "gk", "gv", "gstate"), "k": ("state", "out", "gq", "gv"), "v": ("state", "out", "gq", "gk"),
+               "go": ("gq", "gk", "gv", "gstate")}[which]
+    for name, a, w in zip(NAMES, got, want):
+        strange = ~w.isfinite()
+        assert bool(strange.any()) == (name in reached), name
+        assert not bool((a.detach().cpu().isfinite() & strange).any()), name
