@@ -657,6 +657,8 @@ int myelin_counter_dropout(const void *x, int dtype, const void *residual,
  * NULL: steps of each batch row (taken into [0, T]); later steps keep the state
  * and give 0, and their inputs are not read.  out, grad_q, grad_k and grad_v
  * are contiguous in their inputs' shapes and type; scale finite, not 0.
+ * An infinity or a NaN makes the results that it is part of infinite or NaN (NaN
+ * also where the formula has infinities), and no others.
  * The backward pass takes grad_out and grad_state_out (or NULL) and writes
  * grad_state (or NULL) with the others.
  * workspace: myelin_decay_attention_workspace_elems floats (host only), 16-byte

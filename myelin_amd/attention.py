@@ -162,6 +162,11 @@ def decay_attention(
     Returns ``(final state [B, H, Dk, Dv] float32, out [T, B, H, Dv])``,
     differentiable in q, k, v and the initial state.  States and sums are
     float32.
+
+    An infinity or a NaN in a step makes the results that it is part of (of its
+    own step and later ones, states, gradients) infinite or NaN, and no others.
+    Which of the two is not the formula's where that has infinities: the
+    bfloat16 kernel works in parts, whose infinities cancel.
     """
 
     _check(q, k, v, decay, 4, "[T, B, heads, width]")
