@@ -126,8 +126,8 @@ int launch(Args &a, hipStream_t s) {
   if (by > a.steps) by = a.steps;
   a.per = (a.steps + by - 1) / by;
   by = (a.steps + a.per - 1) / a.per;
-  const bool rows = a.steps == 1 ? a.n % E::VEC == 0 : (a.n * sizeof(typename E::T)) % 16 == 0;
-  const bool vector = rows && myelin::aligned(a.x, 16) && myelin::aligned(a.y, 16) && myelin::aligned(a.residual, 16);
+  const bool vector = a.n % E::VEC == 0 && myelin::aligned(a.x, 16) && myelin::aligned(a.y, 16) &&
+                      myelin::aligned(a.residual, 16);
   const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(by));
   if (!vector)
     dropout_kernel<E, false, false><<<grid, 256, 0, s>>>(a);
