@@ -43,7 +43,8 @@ struct F32 {
   using Frag = f32x8;
   static constexpr int VEC = 4;    // elements of 16 bytes
   static constexpr int C = 32;     // steps of a chunk
-  static constexpr int PARTS = 1;  // fragments that hold an fp32 value
+  static constexpr int PARTS = 1;   // fragments that hold an fp32 value
+  static constexpr int HALVES = 1;  // that hold 16 bits of one
   // LDS rows 16 bytes past a multiple of 64 banks: 16 rows' 16-byte pieces are
   // on distinct banks, and 4 rows 4 apart
   static constexpr int PAD = 4;
@@ -79,6 +80,7 @@ struct BF16 {
   static constexpr int VEC = 8;
   static constexpr int C = 64;
   static constexpr int PARTS = 3;
+  static constexpr int HALVES = 2;
   // LDS rows an odd multiple of 32 bytes long, which puts the transposing read's
   // 4 rows of 32 bytes on distinct banks (16 lanes take 128 bytes a cycle).  Of
   // 16 rows' 8-byte pieces two share a bank; exchanging the halves of each 32
@@ -197,9 +199,10 @@ __device__ __forceinline__ float power(float d, int64_t n) {
 // so the next chunk's rows, fetched meanwhile, are staged behind it: two
 // barriers a chunk.  C is 64 for bf16 and 32 for fp32.
 //
-// Roundings to bf16: the scaled a b^T (then multiplied by the bf16 c, whose
-// products are exact) to one, as good as the result's own; X where it is an
-// operand to two, 16 bits; the scaled c of the state's sum to three, which are
+// Roundings to bf16: the scaled a b^T, multiplied by the bf16 c, and X where it is
+// an operand to two parts each, 16 bits, so that the result has no error but its own
+// rounding's (1.66e-3 of its norm; with one part of a b^T 1.85e-3, for 3 to 6 % less
+// time); the scaled c of the state's sum to three, which are
 // fp32's 24 bits, in the forward pass and in the gradients of a call with an
 // initial state, and to two in the others, whose sums are only operands (2048
 // steps of 8 x 16 heads of 128, training, 389 -> 363 us).  Which it is does not
@@ -215,7 +218,7 @@ __device__ __forceinline__ float power(float d, int64_t n) {
 
 template <class E>
 constexpr int lds_bytes(int kt, int waves) {
-  return E::C * (2 * (16 * kt + E::PAD) + 16 * waves + E::PAD + E::C + E::PAD + 2) *
+  return E::C * (2 * (16 * kt + E::PAD) + 16 * waves + E::PAD + E::HALVES * (E::C + E::PAD) + 2) *
          static_cast<int>(sizeof(typename E::T));
 }
 
@@ -242,7 +245,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
   __shared__ __attribute__((aligned(16))) T sa[STATE_ONLY ? 1 : C * LK];
   __shared__ __attribute__((aligned(16))) T sb[C * LK];
   __shared__ __attribute__((aligned(16))) T sc[C * LV];
-  __shared__ __attribute__((aligned(16))) T sp[STATE_ONLY ? 1 : C * LP];  // scaled a b^T
+  __shared__ __attribute__((aligned(16))) T sp[STATE_ONLY ? 1 : E::HALVES * C * LP];  // scaled a b^T
   __shared__ __attribute__((aligned(16))) float pw[C + 4];                // d^n
   __shared__ __attribute__((aligned(16))) float weight[C];                // of c_j in a whole chunk: c d^(C - j - e)
 
@@ -282,7 +285,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
 
   if (tid <= C) pw[tid] = power(d, tid);
   if (tid < C) weight[tid] = power(d, C - tid - e) * p.c_scale;
-  if constexpr (!STATE_ONLY)  // blocks right of the diagonal stay zero
+  if constexpr (!STATE_ONLY && E::HALVES == 1)  // blocks right of the diagonal stay zero
     for (int i = tid; i < C * LP; i += NT) sp[i] = T(0.0f);
 
   // Rows r0 .. r0 + C - 1 (in the recurrence's order) of one operand, `per`
@@ -340,16 +343,24 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
       }
     }
   };
-  auto stage = [&](auto per, T *to, const auto &from, int ld) {
+  // The lane, counted where it is asked for: what is kept over the loop is spilled
+  // in the 8-wave kernels, and its load back waits for the rows that are on their
+  // way (2048 steps of 8 x 16 heads of 128, training, 372 us for 337).
+  const auto lane_anew = []() {
+    uint32_t all = ~0u;
+    asm volatile("" : "+v"(all));
+    return static_cast<int>(__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0)));
+  };
+  auto stage = [&](auto per, T *to, const auto &from, int ld, int t) {
     constexpr int PER = decltype(per)::value, N = C * PER / NT;
     if constexpr (WHOLE) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        *reinterpret_cast<piece *>(to + E::at(i * (NT / PER) + tid / PER, (tid % PER) * VEC, ld)) = from[i];
+        *reinterpret_cast<piece *>(to + E::at(i * (NT / PER) + t / PER, (t % PER) * VEC, ld)) = from[i];
     } else {
 #pragma unroll
       for (int i = 0; i < N * VEC; ++i)
-        to[E::at((i * NT + tid) / (PER * VEC), tid % (PER * VEC), ld)] = from[i / VEC][i % VEC];
+        to[E::at((i * NT + t) / (PER * VEC), t % (PER * VEC), ld)] = from[i / VEC][i % VEC];
     }
   };
   const std::integral_constant<int, PK> wide{};
@@ -363,9 +374,10 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
     fetch(narrow, nc, pc, ct, vd, r0);
   };
   auto stage_all = [&]() {
-    if constexpr (!STATE_ONLY) stage(wide, sa, na, LK);
-    stage(wide, sb, nb, LK);
-    stage(narrow, sc, nc, LV);
+    const int t = WHOLE ? 64 * w + lane_anew() : tid;
+    if constexpr (!STATE_ONLY) stage(wide, sa, na, LK, t);
+    stage(wide, sb, nb, LK, t);
+    stage(narrow, sc, nc, LV, t);
   };
   if (begin < last) {
     fetch_a(begin);
@@ -444,13 +456,20 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
           if (!past(f + 1)) E::mma(s1, x[f + 1], y[f + 1]);
         }
         s = (s + s1) * s_scale;
-        four z;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int ij = 16 * (it - jt) + l16 - 4 * g - r;
-          z[r] = static_cast<T>(ij >= 0 ? s[r] * pw[ij >= 0 ? ij : 0] : 0.0f);
+          s[r] = ij >= 0 ? s[r] * pw[ij >= 0 ? ij : 0] : 0.0f;
         }
-        *reinterpret_cast<four *>(sp + 16 * it * LP + 16 * jt + row_p) = z;
+        const four z = __builtin_convertvector(s, four);
+        T *to = sp + 16 * it * LP + 16 * jt + row_p;
+        *reinterpret_cast<four *>(to) = z;
+        if constexpr (E::HALVES == 2) {
+          // the lower halves in a matrix of their own, but those of a diagonal block
+          // that begins 32 steps in the block to its right, which is past the diagonal
+          to += it == jt && it % 2 == 0 ? 16 : C * LP;
+          *reinterpret_cast<four *>(to) = __builtin_convertvector(s - __builtin_convertvector(z, f32x4), four);
+        }
       }
     }
     // (of two workgroups of 8 waves the one in its products goes first: 2048 steps
@@ -464,7 +483,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
       for (int f = 0; f < CF; ++f) vf[f] = E::column(sc + 32 * f * LV + 16 * w + col_v, LV);
       if constexpr (!STATE_ONLY) {
         // a X, transposed: rows are columns of the result, the column its row
-        constexpr int XP = E::PARTS < 2 ? E::PARTS : 2;
+        constexpr int XP = E::HALVES;
 #pragma unroll
         for (int it = 0; it < CT; ++it) o[it] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -510,7 +529,7 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
           }
         }
         // (16 bits of X where it is only an operand)
-        constexpr int VP = EXACT || E::PARTS < 3 ? E::PARTS : 2;
+        constexpr int VP = EXACT ? E::PARTS : E::HALVES;
         Frag vs[VP];
         f32x4 lo, hi;
 #pragma unroll
@@ -572,15 +591,23 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
 #pragma unroll
       for (int f = 0; f < CF; ++f)
 #pragma unroll
-        for (int it = 2 * f; it < CT; ++it) E::mma(o[it], vf[f], E::row(sp + 16 * it * LP + 32 * f + row_p));
+        for (int it = 2 * f; it < CT; ++it) {
+          const T *z = sp + 16 * it * LP + 32 * f + row_p;
+          if constexpr (E::HALVES == 2) {
+            if (it == 2 * f) {
+              Frag twice = vf[f];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) twice[4 + x] = twice[x];
+              E::mma(o[it], twice, E::row(z));
+              continue;
+            }
+            E::mma(o[it], vf[f], E::row(z + C * LP));
+          }
+          E::mma(o[it], vf[f], E::row(z));
+        }
       // row i of the chunk, columns 16 w + 4 g .. + 3
       char *out = po + (reverse ? n - r0 - c : r0) * ot * (o_f32 ? 4 : sizeof(T));
-      // (16 w + 4 g, counted anew: kept over the loop it is spilled in the 8-wave
-      // kernels, and its load back waits for the rows that are on their way: 2048
-      // steps of 8 x 16 heads of 128, training, 372 us for 337)
-      uint32_t all = ~0u;
-      asm volatile("" : "+v"(all));
-      const int oc = 16 * w + 4 * static_cast<int>(__builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0)) >> 4);
+      const int oc = 16 * w + 4 * (lane_anew() >> 4);
 #pragma unroll
       for (int it = 0; it < CT; ++it) {
         const int i = 16 * it + l16;

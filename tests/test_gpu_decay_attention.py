@@ -540,3 +540,26 @@ def test_a_value_is_not_lost(T, Dk, Dv, dtype, which, bad):
         strange = ~w.isfinite()
         assert bool(strange.any()) == (name in reached), name
         assert not bool((a.detach().cpu().isfinite() & strange).any()), name
+
+
+@pytest.mark.parametrize("T,H,Hk,Dk,Dv", [(300, 2, 2, 128, 128), (517, 4, 2, 50, 75), (1400, 2, 1, 64, 96), (40, 2, 2, 128, 20)])
+def test_bf16_results_are_rounded_once(T, H, Hk, Dk, Dv):
+    """Half a unit of bf16's 8 bits is 2^-8.  What is multiplied again holds two bf16
+    parts, 2^-16 off, at most twice in a term (the values summed into a state, and the
+    state), and the sums are fp32's, 2^-16 of the terms' magnitudes A: in all below
+    2^-14 A, beside the result's own rounding, 2^-8 of it."""
+
+    _case(test="attention_rounded_once", T=T, Dk=Dk, Dv=Dv)
+    q, k, v, d, s, go, gs = _inputs(T, 2, H, Hk, Dk, Dv, "bf16")
+    for state, gstate in ((s, gs), (None, None)):
+        leaves = [t if t is None else t.detach().requires_grad_() for t in (q, k, v, state)]
+        final, out = myelin.decay_attention(*leaves[:3], d, leaves[3])
+        grads = (go,) if gstate is None else (go, gstate)
+        got = torch.autograd.grad((out, final)[: len(grads)], leaves[:3], grads)
+        args, scale = (q, k, v, d, state), Dk**-0.5
+        want = _reference(*args, None, scale, go, gstate)
+        ab = lambda t: None if t is None else t.abs()  # noqa: E731
+        size = _reference(*(ab(t) for t in args), None, scale, go.abs(), ab(gstate))
+        for name, a, w, z in zip(NAMES[1:], (out, *got), want[1:], size[1:]):
+            tol = 2.0**-8 * w.abs() + 2.0**-14 * z
+            assert bool(((a.detach().double().cpu() - w).abs() <= tol).all()), name

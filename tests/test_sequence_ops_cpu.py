@@ -113,8 +113,8 @@ def test_more_rows_than_a_launch_has_are_refused():
 
 def test_attention_is_cut_for_the_workgroups_that_fit():
     """Segments' states in the workspace: one less than the workgroups that the 256
-    CUs hold of a (b, h).  Two of 57,600 bytes of LDS share a CU (bf16, keys past 64,
-    values not), three of 41,216 and 47,360, two of 8 waves."""
+    CUs hold of a (b, h).  Two share the LDS of a CU in bf16 with keys past 64 and
+    values up to 64, three with both up to 64 and in fp32, two of 8 waves."""
 
     def segments(dtype, Dk, Dv, heads):
         kt, vt = (64 if Dk <= 64 else 128), (128 if dtype and Dk > 64 and Dv > 64 else 64)
