@@ -210,9 +210,10 @@ __device__ __forceinline__ float power(float d, int64_t n) {
 //
 // What bounds it: the waits between LDS reads, products and the two barriers of
 // a chunk, at 16 waves to a CU.  32768 steps of 16 heads of 128, bf16: the main
-// launch moves its 538 MB at about 3.5 TB/s (matrix cores a fifth of the time
-// busy, VALU two fifths, LDS two fifths), the one that forms the segments' states
-// k and v at 3.9; 501 steps of 16 x 8 heads of 50 and 75, fp32, backward 127 us.
+// launch moves its 538 MB at about 3.4 TB/s (matrix cores busy 0.29 of the time,
+// VALU 0.44, LDS 0.57, two fifths of that in conflicts), the one that forms the
+// segments' states k and v at 3.9; 501 steps of 16 x 8 heads of 50 and 75, fp32,
+// backward 126 us; 1024 of 4 x 16 heads of 128, fp32, training 317 us.
 //
 // WHOLE: all rows are whole 16-byte pieces.
 
@@ -223,7 +224,8 @@ constexpr int lds_bytes(int kt, int waves) {
 }
 
 // Registers bound how many waves a CU holds: with whole rows 8 waves to a
-// workgroup fit 128, so that two of them share it, and 4 fit 168, for three.
+// workgroup fit 128, so that two of them share it, and 4 fit 168, for three where
+// LDS holds them.
 constexpr int waves_per_simd(int waves, int lds, bool whole) {
   return !whole ? 2 : waves == 8 ? 4 : 160 * 1024 / lds < 3 ? 2 : 3;
 }
@@ -251,8 +253,8 @@ __attribute__((amdgpu_waves_per_eu(waves_per_simd(NW, lds_bytes<E>(KT, NW), WHOL
 
   // Workgroups go to the 8 XCDs in turn.  Those of one (b, h) and segment run on one
   // of them, whose L2 the problems and slices share; (b, h) and segments together
-  // are dealt out evenly (32768 steps of 128, bf16, 1 head 56 us, 12 heads 190; by
-  // (b, h) alone 124 and 247).
+  // are dealt out evenly (32768 steps of 128, bf16, 1 head 57 us, 12 heads 193; by
+  // (b, h) alone 127 and 267).
   const uint32_t id = blockIdx.x, rest = id >> 3;
   const int which = static_cast<int>(rest % args.problems);
   const Problem &p = args.p[which];
