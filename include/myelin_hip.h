@@ -696,6 +696,125 @@ int myelin_decay_attention_step(const void *q, const void *k, const void *v,
                                 int64_t H, int64_t Hk, int64_t Dk, int64_t Dv,
                                 float scale, myelin_stream_t stream);
 
+/*
+ * A linear recurrence with a gate for every step and channel:
+ *   a_t = sigmoid(gate_t),  h_t = a_t h_{t-1} + (1 - a_t) x_t
+ * x and gate [T, B, N], dtype 0 (fp32) or 2 (bf16), each with unit stride in its
+ * last dimension and element strides of t and b in `strides` (host memory: x's
+ * two, gate's, and for the backward pass grad_out's); states [B, N] contiguous
+ * fp32, state NULL for zeros; lengths [B] int32 or NULL: steps of each batch row
+ * (taken into [0, T]); later steps keep the state and give 0, and their inputs
+ * are not read.  out, grad_x and grad_gate are contiguous in x's type.
+ * kept (or NULL): myelin_gated_recurrence_kept_elems floats (host only) that the
+ * forward pass writes for the backward pass.  That takes grad_out and
+ * grad_state_out (either may be NULL) and writes grad_x, grad_gate and
+ * grad_state (each may be NULL).
+ * workspace: myelin_gated_recurrence_workspace_elems floats (host only), 16-byte
+ * aligned.
+ * _step is one step of it (x [B, N], ..., two strides); state_out may be state
+ * itself.
+ * No counterpart in myelin.
+ */
+int64_t myelin_gated_recurrence_kept_elems(int64_t T, int64_t B, int64_t N);
+int64_t myelin_gated_recurrence_workspace_elems(int dtype, int64_t T, int64_t B,
+                                                int64_t N, int backward);
+int myelin_gated_recurrence_fwd(const void *x, const void *gate, int dtype,
+                                const int64_t *strides, const float *state,
+                                const int32_t *lengths, void *out,
+                                float *state_out, float *kept, int64_t T,
+                                int64_t B, int64_t N, float *workspace,
+                                int64_t workspace_elems, myelin_stream_t stream);
+int myelin_gated_recurrence_bwd(const void *x, const void *gate,
+                                const void *grad_out, int dtype,
+                                const int64_t *strides, const int32_t *lengths,
+                                const float *kept, const float *grad_state_out,
+                                void *grad_x, void *grad_gate, float *grad_state,
+                                int64_t T, int64_t B, int64_t N,
+                                float *workspace, int64_t workspace_elems,
+                                myelin_stream_t stream);
+int myelin_gated_recurrence_step(const void *x, const void *gate, int dtype,
+                                 const int64_t *strides, const float *state,
+                                 void *out, float *state_out, int64_t B,
+                                 int64_t N, myelin_stream_t stream);
+
+/*
+ * The embeddings of tokens: out[i] = scale * weight[tokens[i]], tokens [M] int64,
+ * weight [V, D] with rows of unit stride and row stride ld elements, dtype 0
+ * (fp32) or 2 (bf16), out [M, D] contiguous in its type.  A token equal to
+ * padding (INT64_MIN: none is) gives zeros; any other outside [0, V) gives NaN.
+ * The backward pass writes the whole of grad_weight [V, D], contiguous, from
+ * grad_out [M, D], contiguous: fp32 sums over each token's positions in order,
+ * scaled and rounded once; padding and tokens outside the table give nothing.
+ * workspace: myelin_token_embedding_bwd_workspace_bytes (host only), 16-byte
+ * aligned.
+ * No counterpart in myelin.
+ */
+int myelin_token_embedding(const int64_t *tokens, const void *weight, int dtype,
+                           int64_t ld, void *out, int64_t M, int64_t V,
+                           int64_t D, float scale, int64_t padding,
+                           myelin_stream_t stream);
+int64_t myelin_token_embedding_bwd_workspace_bytes(int64_t M, int64_t V,
+                                                   int64_t D);
+int myelin_token_embedding_bwd(const int64_t *tokens, const void *grad_out,
+                               int dtype, void *grad_weight, int64_t M,
+                               int64_t V, int64_t D, float scale,
+                               int64_t padding, void *workspace,
+                               int64_t workspace_bytes, myelin_stream_t stream);
+
+/*
+ * Distillation from a teacher's top logits:
+ *   loss = sum_k p_k (log p_k - log q[token_k])
+ * with p = softmax(teacher_logits / temperature) over the K places of a row and q
+ * = softmax(logits / temperature) over V.  logits [R, V], rows of unit stride and
+ * row stride ld elements, dtype 0 (fp32) or 2 (bf16); teacher_logits [R, K] fp32
+ * and teacher_tokens [R, K] int64, contiguous, K at most 1024.  Outputs fp32: loss
+ * [R], probs [R, K] (p, or NULL) and stats [2, R], kept for the backward pass.
+ *   - a place of token -1 or value -inf is empty; a row of empty places is not
+ *     read and gives 0;
+ *   - any other token outside [0, V) gives loss NaN;
+ *   - a row of logits of nothing but -inf: loss +inf, gradient 0.
+ * workspace: myelin_distillation_loss_workspace_bytes (host only; 0 where a row
+ * is not split over workgroups), 16-byte aligned.
+ * The backward pass takes the gradient of loss and writes grad_logits [R, V],
+ * contiguous, in the logits' type.
+ * No counterpart in myelin.
+ */
+int64_t myelin_distillation_loss_workspace_bytes(int64_t R, int64_t V);
+int myelin_distillation_loss(const void *logits, int dtype, int64_t ld,
+                             const float *teacher_logits,
+                             const int64_t *teacher_tokens, float temperature,
+                             float *loss, float *probs, float *stats, int64_t R,
+                             int64_t V, int K, void *workspace,
+                             int64_t workspace_bytes, myelin_stream_t stream);
+int myelin_distillation_loss_bwd(const void *logits, int dtype, int64_t ld,
+                                 const int64_t *teacher_tokens,
+                                 const float *probs, const float *stats,
+                                 const float *grad_loss, float temperature,
+                                 void *grad_logits, int64_t R, int64_t V, int K,
+                                 myelin_stream_t stream);
+
+/*
+ * Verification of drafted tokens: target [n + 1, B, V] and draft [n, B, V] (or
+ * NULL: the tokens were chosen, not drawn) are probabilities, dtype 0 (fp32) or 2
+ * (bf16), with unit stride in the last dimension and element strides of the first
+ * two in `strides` (host memory: target's two, draft's); tokens [n, B] int64,
+ * uniforms [n + 1, B] fp32, lengths [B] int32 or NULL: drafted tokens of each
+ * sequence (taken into [0, n]).  Writes accepted [B] and out_tokens [n + 1, B].
+ * Token i is taken while uniforms[i] * draft[i, token] < target[i, token]; the
+ * first that is not is replaced by a draw from max(target - draft, 0), after all
+ * of them comes a draw from the target's next row, then -1.  A draw is the lowest
+ * token whose cumulative weight is above uniforms[n] times the sum.  In fp64.
+ * workspace: myelin_verify_draft_workspace_bytes (host only), 16-byte aligned.
+ * No counterpart in myelin.
+ */
+int64_t myelin_verify_draft_workspace_bytes(int64_t B, int64_t V);
+int myelin_verify_draft(const void *target, const void *draft, int dtype,
+                        const int64_t *strides, const int64_t *tokens,
+                        const float *uniforms, const int32_t *lengths,
+                        int64_t *accepted, int64_t *out_tokens, int64_t n,
+                        int64_t B, int64_t V, void *workspace,
+                        int64_t workspace_bytes, myelin_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

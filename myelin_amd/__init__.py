@@ -5,7 +5,9 @@ use on this path (kernels, packing, neuron types, surrogates, checkpoint
 policy, and the streamed-synapse / rate modules); every compute call runs a
 hand-written gfx950 HIP kernel from ``libmyelin_hip.so``.  Beside them are the
 operators of a spiking sequence model, which myelin does not have:
-``decay_attention`` and its step, ``counter_dropout`` and ``token_log_probs``.
+``decay_attention`` and its step, ``counter_dropout`` and ``token_log_probs``;
+and those of a small model that drafts for it: ``token_embedding``,
+``gated_recurrence`` and its step, ``distillation_loss`` and ``verify_draft``.
 """
 
 from myelin_amd.attention import DecayAttention, decay_attention, decay_attention_step
@@ -16,7 +18,10 @@ from myelin_amd.checkpointing import (
     recommended_checkpoint_size,
     resolve_checkpoint_size,
 )
+from myelin_amd.distillation import distillation_loss
 from myelin_amd.dropout import CounterDropout, counter_dropout
+from myelin_amd.embedding import TokenEmbedding, token_embedding
+from myelin_amd.gated import GatedRecurrence, gated_recurrence, gated_recurrence_step
 from myelin_amd.kernels import (
     Backend,
     alif_forward,
@@ -71,11 +76,13 @@ from myelin_amd.surrogates import (
     surrogate_name,
     triangular_surrogate,
 )
+from myelin_amd.verification import VerifiedTokens, verify_draft
 
 __all__ = [
     "ALIFCell",
     "CounterDropout",
     "DecayAttention",
+    "GatedRecurrence",
     "LIFCell",
     "LinearSurrogateLIF",
     "LinearSurrogateLIFPacked",
@@ -85,10 +92,15 @@ __all__ = [
     "SurrogateALIFCell",
     "SurrogateLIFCell",
     "TimeUnroll",
+    "TokenEmbedding",
     "TokenLogProbs",
+    "VerifiedTokens",
     "counter_dropout",
     "decay_attention",
     "decay_attention_step",
+    "distillation_loss",
+    "gated_recurrence",
+    "gated_recurrence_step",
     "linear_surrogate_lif_forward",
     "linear_surrogate_lif_packed_forward",
     "linear_surrogate_lif_rate_forward",
@@ -128,9 +140,11 @@ __all__ = [
     "surrogate_from_name",
     "surrogate_lif_forward",
     "surrogate_name",
+    "token_embedding",
     "token_log_probs",
     "triangular_surrogate",
     "two_layer_surrogate_lif_rate_packed_hidden_forward",
     "two_layer_surrogate_lif_rate_recompute_forward",
     "unpack_spikes",
+    "verify_draft",
 ]

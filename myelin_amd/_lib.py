@@ -90,6 +90,14 @@ SIGNATURES: dict[str, list] = {
     "myelin_decay_attention_bwd": [_P] * 4 + [_INT] + [_P] * 9 + [_I64] * 6 + [_F, _P, _I64, _P],
     "myelin_decay_attention_step": [_P] * 3 + [_INT] + [_P] * 5 + [_I64] * 5 + [_F, _P],
     "myelin_counter_dropout": [_P, _INT, _P, _P, _I64, _I64, _I64, _F, _I64, _I64, _P, _P],
+    "myelin_gated_recurrence_fwd": [_P, _P, _INT] + [_P] * 6 + [_I64] * 3 + [_P, _I64, _P],
+    "myelin_gated_recurrence_bwd": [_P] * 3 + [_INT] + [_P] * 7 + [_I64] * 3 + [_P, _I64, _P],
+    "myelin_gated_recurrence_step": [_P, _P, _INT] + [_P] * 4 + [_I64] * 2 + [_P],
+    "myelin_token_embedding": [_P, _P, _INT, _I64, _P] + [_I64] * 3 + [_F, _I64, _P],
+    "myelin_token_embedding_bwd": [_P, _P, _INT, _P] + [_I64] * 3 + [_F, _I64, _P, _I64, _P],
+    "myelin_distillation_loss": [_P, _INT, _I64, _P, _P, _F] + [_P] * 3 + [_I64] * 2 + [_INT, _P, _I64, _P],
+    "myelin_distillation_loss_bwd": [_P, _INT, _I64] + [_P] * 4 + [_F, _P] + [_I64] * 2 + [_INT, _P],
+    "myelin_verify_draft": [_P, _P, _INT] + [_P] * 6 + [_I64] * 3 + [_P, _I64, _P],
 }
 
 _lock = threading.Lock()
@@ -124,6 +132,13 @@ def load() -> ctypes.CDLL:
             lib.myelin_token_log_probs_workspace_bytes.restype = ctypes.c_int64
             lib.myelin_decay_attention_workspace_elems.argtypes = [_INT] + [_I64] * 6 + [_INT]
             lib.myelin_decay_attention_workspace_elems.restype = ctypes.c_int64
+            for name, argtypes in (("myelin_gated_recurrence_kept_elems", [_I64] * 3),
+                                   ("myelin_gated_recurrence_workspace_elems", [_INT] + [_I64] * 3 + [_INT]),
+                                   ("myelin_token_embedding_bwd_workspace_bytes", [_I64] * 3),
+                                   ("myelin_distillation_loss_workspace_bytes", [_I64] * 2),
+                                   ("myelin_verify_draft_workspace_bytes", [_I64] * 2)):
+                getattr(lib, name).argtypes = argtypes
+                getattr(lib, name).restype = ctypes.c_int64
             for name, argtypes in SIGNATURES.items():
                 fn = getattr(lib, name)
                 fn.argtypes = argtypes

@@ -54,7 +54,12 @@ def native():
         _autograd.bind_sequence({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
             "myelin_token_log_probs_workspace_bytes", "myelin_token_log_probs", "myelin_token_log_probs_bwd",
             "myelin_counter_dropout", "myelin_decay_attention_workspace_elems", "myelin_decay_attention_fwd",
-            "myelin_decay_attention_bwd", "myelin_decay_attention_step", "myelin_last_error")}, _lib.MyelinHipError)
+            "myelin_decay_attention_bwd", "myelin_decay_attention_step", "myelin_gated_recurrence_kept_elems",
+            "myelin_gated_recurrence_workspace_elems", "myelin_gated_recurrence_fwd", "myelin_gated_recurrence_bwd",
+            "myelin_gated_recurrence_step", "myelin_token_embedding", "myelin_token_embedding_bwd_workspace_bytes",
+            "myelin_token_embedding_bwd", "myelin_distillation_loss_workspace_bytes", "myelin_distillation_loss",
+            "myelin_distillation_loss_bwd", "myelin_verify_draft_workspace_bytes", "myelin_verify_draft",
+            "myelin_last_error")}, _lib.MyelinHipError)
         _native = _autograd
     return _native
 

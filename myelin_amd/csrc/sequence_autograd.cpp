@@ -1,6 +1,7 @@
 // The sequence-model operators' host code in C++: what the Functions of
-// attention.py, dropout.py and log_probs.py do (the same entry points, outputs
-// and saved tensors), without Python in either direction.  Their small calls
+// attention.py, dropout.py, log_probs.py, gated.py, embedding.py,
+// distillation.py and verification.py do (the same entry points, outputs and
+// saved tensors), without Python in either direction.  Their small calls
 // are host work: the training step of 12800 rows of 10 classes, 7 us of
 // kernels, took 134 us with the Python Function, half of it on the autograd
 // engine's device thread, which waits there for the interpreter lock that the
@@ -37,6 +38,19 @@ struct Library {
   decltype(&myelin_decay_attention_fwd) attention_fwd = nullptr;
   decltype(&myelin_decay_attention_bwd) attention_bwd = nullptr;
   decltype(&myelin_decay_attention_step) attention_step = nullptr;
+  decltype(&myelin_gated_recurrence_kept_elems) recurrence_kept = nullptr;
+  decltype(&myelin_gated_recurrence_workspace_elems) recurrence_workspace = nullptr;
+  decltype(&myelin_gated_recurrence_fwd) recurrence_fwd = nullptr;
+  decltype(&myelin_gated_recurrence_bwd) recurrence_bwd = nullptr;
+  decltype(&myelin_gated_recurrence_step) recurrence_step = nullptr;
+  decltype(&myelin_token_embedding) embedding = nullptr;
+  decltype(&myelin_token_embedding_bwd_workspace_bytes) embedding_workspace = nullptr;
+  decltype(&myelin_token_embedding_bwd) embedding_bwd = nullptr;
+  decltype(&myelin_distillation_loss_workspace_bytes) distillation_workspace = nullptr;
+  decltype(&myelin_distillation_loss) distillation = nullptr;
+  decltype(&myelin_distillation_loss_bwd) distillation_bwd = nullptr;
+  decltype(&myelin_verify_draft_workspace_bytes) verify_workspace = nullptr;
+  decltype(&myelin_verify_draft) verify = nullptr;
   decltype(&myelin_last_error) last_error = nullptr;
   PyObject *hip_error = nullptr;  // the class of failed launches; never released
 } lib;
@@ -305,6 +319,202 @@ variable_list decay_attention_step(const Tensor &q, const Tensor &k, const Tenso
   return {to, out};
 }
 
+// ---- gated recurrence ----------------------------------------------------
+Tensor recurrence_workspace(const Tensor &x, int backward, int64_t *elems) {
+  *elems = lib.recurrence_workspace(code_of(x), x.size(0), x.size(1), x.size(2), backward);
+  return *elems ? torch::empty({*elems}, x.options().dtype(torch::kFloat32)) : Tensor();
+}
+
+// {final state, out}, and the kept states where a gradient is wanted
+variable_list recurrence_forward(const Tensor &x, const Tensor &gate, const Tensor &state, const Tensor &lengths,
+                                 Tensor *kept) {
+  const int64_t T = x.size(0), B = x.size(1), N = x.size(2);
+  const auto f32s = x.options().dtype(torch::kFloat32);
+  Tensor out = torch::empty({T, B, N}, x.options()), last = torch::empty({B, N}, f32s);
+  if (kept) *kept = torch::empty({lib.recurrence_kept(T, B, N)}, f32s);
+  int64_t elems;
+  const Tensor ws = recurrence_workspace(x, 0, &elems);
+  check(lib.recurrence_fwd(at(x), at(gate), code_of(x), strides_of({x, gate}).data(), f32(state), i32(lengths), at(out),
+                           f32(last), kept ? f32(*kept) : nullptr, T, B, N, f32(ws), elems, stream_of(x)),
+        "myelin_gated_recurrence_fwd");
+  return {last, out};
+}
+
+struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &gate, const OptTensor &state,
+                               const OptTensor &lengths) {
+    ctx->set_materialize_grads(false);
+    Tensor kept;
+    variable_list out = recurrence_forward(x, gate, plain(state), plain(lengths), &kept);
+    ctx->save_for_backward({x, gate, plain(lengths), kept});
+    ctx->saved_data["state"] = state.has_value();
+    return out;
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list out(4);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &gate = saved[1];
+    const int64_t T = x.size(0), B = x.size(1), N = x.size(2);
+    const c10::DeviceGuard guard(x.device());
+    const Tensor g_out = grads[1].defined() ? unit_stride(grads[1]) : Tensor(), g_last = contiguous(grads[0]);
+    if (ctx->needs_input_grad(0)) out[0] = torch::empty({T, B, N}, x.options());
+    if (ctx->needs_input_grad(1)) out[1] = torch::empty({T, B, N}, x.options());
+    // (inputs are counted without those that were not given)
+    if (ctx->saved_data["state"].toBool() && ctx->needs_input_grad(2))
+      out[2] = torch::empty({B, N}, x.options().dtype(torch::kFloat32));
+    int64_t elems;
+    const Tensor ws = recurrence_workspace(x, 1, &elems);
+    check(lib.recurrence_bwd(at(x), at(gate), at(g_out), code_of(x),
+                             strides_of({x, gate, g_out.defined() ? g_out : x}).data(), i32(saved[2]), f32(saved[3]),
+                             f32(g_last), at(out[0]), at(out[1]), f32(out[2]), T, B, N, f32(ws), elems, stream_of(x)),
+          "myelin_gated_recurrence_bwd");
+    return once(std::move(out));
+  }
+};
+
+// x and gate with unit stride in their last dimension, the others contiguous
+variable_list gated_recurrence(const Tensor &x, const Tensor &gate, const OptTensor &state, const OptTensor &lengths) {
+  const c10::DeviceGuard guard(x.device());
+  if (needs({x, gate, plain(state)})) return RecurrenceFunction::apply(x, gate, state, lengths);
+  return recurrence_forward(x, gate, plain(state), plain(lengths), nullptr);
+}
+
+// {new state, out}; the new state goes to out_state, if given
+variable_list gated_recurrence_step(const Tensor &x, const Tensor &gate, const Tensor &state,
+                                    const OptTensor &out_state) {
+  const c10::DeviceGuard guard(x.device());
+  const int64_t B = x.size(0), N = x.size(1);
+  Tensor out = torch::empty({B, N}, x.options());
+  Tensor to = out_state.has_value() ? *out_state : torch::empty({B, N}, state.options());
+  check(lib.recurrence_step(at(x), at(gate), code_of(x), strides_of({x, gate}).data(), f32(state), at(out), f32(to), B,
+                            N, stream_of(x)),
+        "myelin_gated_recurrence_step");
+  // autograd notices where it keeps out_state for a backward pass
+  if (out_state.has_value() && !to.is_inference()) to.unsafeGetTensorImpl()->bump_version();
+  return {to, out};
+}
+
+// ---- embedding -----------------------------------------------------------
+Tensor embedded(const Tensor &weight, const Tensor &tokens, double scale, int64_t padding) {
+  const int64_t M = tokens.numel(), V = weight.size(0), D = weight.size(1);
+  Tensor out = torch::empty({M, D}, weight.options());
+  check(lib.embedding(i64(tokens), at(weight), code_of(weight), weight.stride(0), at(out), M, V, D,
+                      static_cast<float>(scale), padding, stream_of(weight)),
+        "myelin_token_embedding");
+  return out;
+}
+
+struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &weight, const Tensor &tokens, double scale,
+                        int64_t padding) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["sizes"] = std::vector<int64_t>{padding, weight.size(0), weight.size(1)};
+    return embedded(weight, tokens, scale, padding);
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    const Tensor tokens = ctx->get_saved_variables()[0], g = grads[0].contiguous();
+    const std::vector<int64_t> z = ctx->saved_data["sizes"].toIntVector();
+    const int64_t M = tokens.numel(), V = z[1], D = z[2];
+    const c10::DeviceGuard guard(g.device());
+    out[0] = torch::empty({V, D}, g.options());
+    const int64_t need = lib.embedding_workspace(M, V, D);
+    Tensor ws;
+    if (need) ws = torch::empty({need}, g.options().dtype(torch::kUInt8));
+    check(lib.embedding_bwd(i64(tokens), at(g), code_of(g), at(out[0]), M, V, D,
+                            static_cast<float>(ctx->saved_data["scale"].toDouble()), z[0], at(ws), need, stream_of(g)),
+          "myelin_token_embedding_bwd");
+    return once(std::move(out));
+  }
+};
+
+// weight with rows of unit stride, tokens [M] int64 contiguous
+Tensor token_embedding(const Tensor &weight, const Tensor &tokens, double scale, int64_t padding) {
+  const c10::DeviceGuard guard(weight.device());
+  if (needs({weight})) return EmbeddingFunction::apply(weight, tokens, scale, padding);
+  return embedded(weight, tokens, scale, padding);
+}
+
+// ---- distillation --------------------------------------------------------
+struct Distilled {
+  Tensor loss, probs, stats;
+};
+
+Distilled distillation_forward(const Tensor &x, const Tensor &values, const Tensor &tokens, double temperature,
+                               bool keep) {
+  const int64_t R = x.size(0), V = x.size(1), K = tokens.size(1);
+  const auto f32s = x.options().dtype(torch::kFloat32);
+  Distilled d{torch::empty({R}, f32s), Tensor(), torch::empty({2, R}, f32s)};
+  if (keep) d.probs = torch::empty({R, K}, f32s);
+  const int64_t need = lib.distillation_workspace(R, V);
+  Tensor ws;
+  if (need) ws = torch::empty({need}, x.options().dtype(torch::kUInt8));
+  check(lib.distillation(at(x), code_of(x), x.stride(0), f32(values), i64(tokens), static_cast<float>(temperature),
+                         f32(d.loss), f32(d.probs), f32(d.stats), R, V, static_cast<int>(K), at(ws), need,
+                         stream_of(x)),
+        "myelin_distillation_loss");
+  return d;
+}
+
+struct DistillationFunction : torch::autograd::Function<DistillationFunction> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &values, const Tensor &tokens,
+                        double temperature) {
+    const Distilled d = distillation_forward(x, values, tokens, temperature, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, tokens, d.probs, d.stats});
+    ctx->saved_data["temperature"] = temperature;
+    return d.loss;
+  }
+
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    variable_list out(4);
+    if (!grads[0].defined()) return out;
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], g = grads[0].contiguous();
+    const int64_t R = x.size(0), V = x.size(1);
+    const c10::DeviceGuard guard(x.device());
+    out[0] = torch::empty({R, V}, x.options());
+    check(lib.distillation_bwd(at(x), code_of(x), x.stride(0), i64(saved[1]), f32(saved[2]), f32(saved[3]), f32(g),
+                               static_cast<float>(ctx->saved_data["temperature"].toDouble()), at(out[0]), R, V,
+                               static_cast<int>(saved[1].size(1)), stream_of(x)),
+          "myelin_distillation_loss_bwd");
+    return once(std::move(out));
+  }
+};
+
+// x with rows of unit stride, values [R, K] fp32 and tokens [R, K] int64 contiguous
+Tensor distillation_loss(const Tensor &x, const Tensor &values, const Tensor &tokens, double temperature) {
+  const c10::DeviceGuard guard(x.device());
+  if (needs({x})) return DistillationFunction::apply(x, values, tokens, temperature);
+  return distillation_forward(x, values, tokens, temperature, false).loss;
+}
+
+// ---- verification --------------------------------------------------------
+// {accepted, tokens}; probabilities with unit stride in their last dimension, the
+// others contiguous
+variable_list verify_draft(const Tensor &target, const OptTensor &draft, const Tensor &tokens, const Tensor &uniforms,
+                           const OptTensor &lengths) {
+  const c10::DeviceGuard guard(target.device());
+  const int64_t n = target.size(0) - 1, B = target.size(1), V = target.size(2);
+  const auto whole = target.options().dtype(torch::kInt64);
+  Tensor accepted = torch::empty({B}, whole), out = torch::empty({n + 1, B}, whole);
+  const Tensor q = plain(draft);
+  const int64_t need = lib.verify_workspace(B, V);
+  Tensor ws;
+  if (need) ws = torch::empty({need}, target.options().dtype(torch::kUInt8));
+  check(lib.verify(at(target), at(q), code_of(target), strides_of({target, q.defined() ? q : target}).data(),
+                   i64(tokens), f32(uniforms), i32(plain(lengths)), i64(accepted), i64(out), n, B, V, at(ws), need,
+                   stream_of(target)),
+        "myelin_verify_draft");
+  return {accepted, out};
+}
+
 template <class F>
 void take(F &to, const pybind11::dict &from, const char *name) {
   to = reinterpret_cast<F>(from[name].cast<uintptr_t>());
@@ -322,6 +532,19 @@ void register_sequence_operators(pybind11::module_ &m) {
     take(lib.attention_fwd, addresses, "myelin_decay_attention_fwd");
     take(lib.attention_bwd, addresses, "myelin_decay_attention_bwd");
     take(lib.attention_step, addresses, "myelin_decay_attention_step");
+    take(lib.recurrence_kept, addresses, "myelin_gated_recurrence_kept_elems");
+    take(lib.recurrence_workspace, addresses, "myelin_gated_recurrence_workspace_elems");
+    take(lib.recurrence_fwd, addresses, "myelin_gated_recurrence_fwd");
+    take(lib.recurrence_bwd, addresses, "myelin_gated_recurrence_bwd");
+    take(lib.recurrence_step, addresses, "myelin_gated_recurrence_step");
+    take(lib.embedding, addresses, "myelin_token_embedding");
+    take(lib.embedding_workspace, addresses, "myelin_token_embedding_bwd_workspace_bytes");
+    take(lib.embedding_bwd, addresses, "myelin_token_embedding_bwd");
+    take(lib.distillation_workspace, addresses, "myelin_distillation_loss_workspace_bytes");
+    take(lib.distillation, addresses, "myelin_distillation_loss");
+    take(lib.distillation_bwd, addresses, "myelin_distillation_loss_bwd");
+    take(lib.verify_workspace, addresses, "myelin_verify_draft_workspace_bytes");
+    take(lib.verify, addresses, "myelin_verify_draft");
     take(lib.last_error, addresses, "myelin_last_error");
     lib.hip_error = pybind11::object(hip_error).release().ptr();
   });
@@ -331,4 +554,9 @@ void register_sequence_operators(pybind11::module_ &m) {
   m.def("counter_dropout", &counter_dropout, nogil);
   m.def("decay_attention", &decay_attention, nogil);
   m.def("decay_attention_step", &decay_attention_step, nogil);
+  m.def("gated_recurrence", &gated_recurrence, nogil);
+  m.def("gated_recurrence_step", &gated_recurrence_step, nogil);
+  m.def("token_embedding", &token_embedding, nogil);
+  m.def("distillation_loss", &distillation_loss, nogil);
+  m.def("verify_draft", &verify_draft, nogil);
 }
