@@ -325,6 +325,13 @@ Tensor recurrence_workspace(const Tensor &x, int backward, int64_t *elems) {
   return *elems ? torch::empty({*elems}, x.options().dtype(torch::kFloat32)) : Tensor();
 }
 
+// unit stride in the last dimension, and batch rows near enough for the kernels
+Tensor recurrence_rows(const Tensor &t) {
+  const int64_t B = t.size(-2), N = t.size(-1);
+  const bool near = B <= 1 || N == 0 || (64 / N + 1) * t.stride(-2) + N < int64_t{1} << 30;
+  return near ? unit_stride(t) : t.contiguous();
+}
+
 // {final state, out}, and the kept states where a gradient is wanted
 variable_list recurrence_forward(const Tensor &x, const Tensor &gate, const Tensor &state, const Tensor &lengths,
                                  Tensor *kept) {
@@ -358,7 +365,7 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
     const Tensor &x = saved[0], &gate = saved[1];
     const int64_t T = x.size(0), B = x.size(1), N = x.size(2);
     const c10::DeviceGuard guard(x.device());
-    const Tensor g_out = grads[1].defined() ? unit_stride(grads[1]) : Tensor(), g_last = contiguous(grads[0]);
+    const Tensor g_out = grads[1].defined() ? recurrence_rows(grads[1]) : Tensor(), g_last = contiguous(grads[0]);
     if (ctx->needs_input_grad(0)) out[0] = torch::empty({T, B, N}, x.options());
     if (ctx->needs_input_grad(1)) out[1] = torch::empty({T, B, N}, x.options());
     // (inputs are counted without those that were not given)
@@ -374,7 +381,7 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
   }
 };
 
-// x and gate with unit stride in their last dimension, the others contiguous
+// x and gate as recurrence_rows gives them, the others contiguous
 variable_list gated_recurrence(const Tensor &x, const Tensor &gate, const OptTensor &state, const OptTensor &lengths) {
   const c10::DeviceGuard guard(x.device());
   if (needs({x, gate, plain(state)})) return RecurrenceFunction::apply(x, gate, state, lengths);

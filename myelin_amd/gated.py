@@ -33,9 +33,12 @@ def _strides(*tensors):
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with unit stride in its last dimension."""
+    """``t`` with unit stride in its last dimension, and batch rows near enough for
+    a workgroup's 32-bit offsets."""
 
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    B, N = t.shape[-2:]
+    near = B <= 1 or N == 0 or (64 // N + 1) * t.stride(-2) + N < 2**30
+    return t if near and (t.stride(-1) == 1 or N == 1) else t.contiguous()
 
 
 def _workspace(x, backward):
@@ -62,7 +65,7 @@ def _forward(x, gate, state, lengths, keep):
 
 
 class HipGatedRecurrenceFunction(torch.autograd.Function):
-    """Saves its inputs, by reference, and the states before every 16th step:
+    """Saves its inputs, by reference, and the states before every 8th step:
     the backward pass runs the steps between them again, and the adjoint."""
 
     @staticmethod

@@ -42,7 +42,7 @@ def test_recurrence_entry_points_validate():
     with pytest.raises(ValueError, match="null pointer"):
         _lib.call("myelin_gated_recurrence_step", 16, 16, 0, 16, None, 16, 16, 2, 3, None)
     kept = _lib.load().myelin_gated_recurrence_kept_elems
-    assert kept(1, 2, 3) == 6 and kept(16, 2, 3) == 6 and kept(17, 2, 3) == 12
+    assert kept(1, 2, 3) == 6 and kept(8, 2, 3) == 6 and kept(9, 2, 3) == 12
 
 
 def test_recurrence_workspace_is_checked():
