@@ -12,6 +12,10 @@
 //
 // One pass: a lane keeps the running maximum m of its elements and s = sum
 // e^((x - m) / temperature); all of it is fp32, whatever the logits' type.
+//
+// The forward pass writes p for the backward pass with tokens that are named twice
+// put together at the first of their places (0 at the others): each token then has
+// one place, and the backward pass can put p where its element looks for it.
 
 #include "elements.h"
 
@@ -25,6 +29,7 @@ using myelin::kWave;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kInf = __builtin_huge_valf();
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kNarrow = 1024;  // widest row of a single wave
 
 // e^((x - m) rate), rate = 1 / temperature
 struct Stats {
@@ -55,6 +60,14 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// The rounding of d rate log2(e), |d| rate 2^-24 of an exponential, is left: it is
+// small where the exponential is large and of random sign over the sum.
+struct Rate {
+  float rate, log2;  // 1 / temperature, and times log2(e)
+  __device__ explicit Rate(float r) : rate(r), log2(r * kLog2e) {}
+  __device__ float exp(float d) const { return __builtin_amdgcn_exp2f(d * log2); }
+};
+
 struct Args {
   const void *x;
   int64_t ld;
@@ -65,9 +78,19 @@ struct Args {
   float *stats;         // [2, R]: m, then log s (-inf: no gradient)
   int64_t R, V;
   int K;
+  int parts;
+  int64_t part;  // elements of a part
+  int64_t rows;  // of a launch in x
+  Stats *part_stats;
 };
 
-__device__ __forceinline__ bool empty(const Args &a, int64_t at) { return a.tokens[at] == -1 || a.values[at] == -kInf; }
+__device__ __forceinline__ bool empty(int64_t token, float value) { return token == -1 || value == -kInf; }
+
+__device__ __forceinline__ bool nothing(const Args &a, int64_t row, int lane) {
+  bool some = false;
+  for (int k = lane; k < a.K; k += kWave) some |= !empty(a.tokens[row * a.K + k], a.values[row * a.K + k]);
+  return !__any(some);
+}
 
 // a row with nothing to learn from
 __device__ __forceinline__ void store_nothing(const Args &a, int64_t row, int lane) {
@@ -80,37 +103,63 @@ __device__ __forceinline__ void store_nothing(const Args &a, int64_t row, int la
   }
 }
 
+// Bits of the tokens seen, by their number modulo BITS: a wave's, cleared.  Only
+// where two meet is it looked at which are the same.
+constexpr int kSeen = 1 << 15;
+
+template <int BITS>
+__device__ __forceinline__ void clear(uint32_t *seen, int lane) {
+  for (int o = lane; o < BITS / 32; o += kWave) seen[o] = 0;
+}
+
 // The row's loss from its logits' statistics, by one wave.
-template <class E>
-__device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int lane) {
+template <class E, int BITS>
+__device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int lane, uint32_t *seen) {
   const int64_t first = row * a.K;
   const typename E::T *x = static_cast<const typename E::T *>(a.x) + row * a.ld;
   float peak = kLowest;
-  bool bad = false;
-  for (int k = lane; k < a.K; k += kWave)
-    if (!empty(a, first + k)) {
-      peak = fmaxf(peak, a.values[first + k]);
-      bad |= a.tokens[first + k] < 0 || a.tokens[first + k] >= a.V;
-    }
+  bool bad = false, twice = false;
+  for (int k = lane; k < a.K; k += kWave) {
+    const int64_t token = a.tokens[first + k];
+    const float v = a.values[first + k];
+    if (empty(token, v)) continue;
+    peak = fmaxf(peak, v);
+    bad |= token < 0 || token >= a.V;
+    const uint32_t at = static_cast<uint32_t>(token) % BITS, bit = 1u << (at % 32);
+    if (a.probs) twice |= (atomicOr(&seen[at / 32], bit) & bit) != 0;
+  }
   for (int o = kWave >> 1; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
   float total = 0.0f;
   for (int k = lane; k < a.K; k += kWave)
-    if (!empty(a, first + k)) total += myelin::exp_f32((a.values[first + k] - peak) * a.rate);
+    if (!empty(a.tokens[first + k], a.values[first + k]))
+      total += myelin::exp_f32((a.values[first + k] - peak) * a.rate);
   total = wave_sum(total);
   bad = __any(bad);
+  twice = __any(twice);
   const float log_total = logf(total), log_s = t.s == 0.0f ? -kInf : logf(t.s);
   float loss = 0.0f;
   for (int k = lane; k < a.K; k += kWave) {
+    const int64_t token = a.tokens[first + k];
     float p = 0.0f;
-    if (!empty(a, first + k)) {
+    if (!empty(token, a.values[first + k])) {
       const float d = (a.values[first + k] - peak) * a.rate;
       p = myelin::exp_f32(d) / total;
-      const int64_t token = a.tokens[first + k];
       if (p != 0.0f && !bad) {
         // nothing allowed: log q is -inf for every token
         const float log_q = t.s == 0.0f ? -kInf : (E::get(x[token]) - t.m) * a.rate - log_s;
         loss += p * ((d - log_total) - log_q);
       }
+    }
+    if (a.probs && twice && p != 0.0f) {
+      // put together, in the places' order, at the first
+      float sum = 0.0f;
+      bool mine = true;
+      for (int o = 0; o < a.K; ++o)
+        if (a.tokens[first + o] == token && a.values[first + o] != -kInf) {
+          mine &= o >= k;
+          sum += myelin::exp_f32((a.values[first + o] - peak) * a.rate) / total;
+        }
+      p = mine ? sum : 0.0f;
     }
     if (a.probs) a.probs[first + k] = p;
   }
@@ -122,38 +171,110 @@ __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int 
   }
 }
 
-__device__ __forceinline__ bool nothing(const Args &a, int64_t row) {
-  bool some = false;
-  for (int k = threadIdx.x & (kWave - 1); k < a.K; k += kWave) some |= !empty(a, row * a.K + k);
-  return !__any(some);
-}
-
-// a workgroup to a row
+// ---- few classes: a wave to a row ---------------------------------------
 template <class E>
-__global__ __launch_bounds__(kThreads) void rows(Args a) {
-  __shared__ Stats red[kWaves];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid >> 6;
-  const int64_t row = myelin::block_id();
-  if (row >= a.R) return;
-  if (nothing(a, row)) {
-    if (w == 0) store_nothing(a, row, lane);
+__global__ __launch_bounds__(kThreads) void narrow_rows(Args a) {
+  __shared__ uint32_t seen[kWaves][kNarrow / 32];
+  const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x >> 6;
+  const int64_t row = myelin::block_id() * kWaves + w;
+  if (row >= a.R) return;  // whole waves
+  const typename E::T *x = static_cast<const typename E::T *>(a.x) + row * a.ld;
+  // (in LDS a wave's own writes and atomics are done in its order)
+  if (a.probs) clear<kNarrow>(seen[w], lane);
+  if (nothing(a, row, lane)) {
+    store_nothing(a, row, lane);
     return;
   }
-  const typename E::T *x = static_cast<const typename E::T *>(a.x) + row * a.ld;
+  const Rate r(a.rate);
   Stats t = Stats::none();
-  for (int64_t i = tid; i < a.V; i += kThreads) {
-    const float v = E::get(x[i]);
-    if (v > t.m) t.rescale(v, a.rate);
-    t.s += myelin::exp_f32((v - t.m) * a.rate);
+  constexpr int kEach = kNarrow / kWave;
+  float v[kEach];
+#pragma unroll
+  for (int o = 0; o < kEach; ++o) v[o] = o * kWave + lane < a.V ? E::get(x[o * kWave + lane]) : -kInf;
+#pragma unroll
+  for (int o = 0; o < kEach; ++o) t.m = fmaxf(t.m, v[o]);
+#pragma unroll
+  for (int o = 0; o < kEach; ++o) t.s += r.exp(v[o] - t.m);
+  t = across(t, a.rate);
+  finish<E, kNarrow>(a, row, t, lane, seen[w]);
+}
+
+// ---- wide rows: a workgroup to a row, or to one of its parts -------------
+constexpr int kPerThread = 16;                // elements of a tile a thread holds
+constexpr int kTile = kThreads * kPerThread;  // 4096
+
+template <class E>
+__global__ __launch_bounds__(kThreads) void wide_rows(Args a) {
+  using T = typename E::T;
+  constexpr int VEC = E::VEC, NV = kPerThread / VEC;
+  __shared__ Stats red[kWaves];
+  __shared__ uint32_t seen[kSeen / 32];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid >> 6;
+  const int64_t row = blockIdx.x / a.parts + blockIdx.y * a.rows;
+  if (row >= a.R) return;  // the whole workgroup
+  const int part = static_cast<int>(blockIdx.x % a.parts);
+  const int64_t begin = part * a.part;
+  const int64_t end = begin + a.part < a.V ? begin + a.part : a.V;
+  if (nothing(a, row, lane)) {
+    if (part == 0 && w == 0) store_nothing(a, row, lane);
+    return;
+  }
+  if (a.probs && w == 0) clear<kSeen>(seen, lane);
+  const Rate r(a.rate);
+  const T *x = static_cast<const T *>(a.x) + row * a.ld;
+  // whole vectors start where the address is a multiple of 16: `lead` elements
+  // before `begin` belong to the first one
+  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(x + begin) % 16) / sizeof(T));
+  typedef T vec __attribute__((ext_vector_type(VEC)));
+  Stats t = Stats::none();
+  for (int64_t at = begin - lead; at < end; at += kTile) {
+    float v[kPerThread];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int64_t i = at + (static_cast<int64_t>(j) * kThreads + tid) * VEC;
+      if (i >= begin && i + VEC <= end) {
+        const vec p = __builtin_nontemporal_load(reinterpret_cast<const vec *>(x + i));
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) v[j * VEC + q] = E::get(p[q]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) v[j * VEC + q] = i + q >= begin && i + q < end ? E::get(x[i + q]) : -kInf;
+      }
+    }
+    float top = t.m;
+#pragma unroll
+    for (int q = 0; q < kPerThread; ++q) top = fmaxf(top, v[q]);
+    if (top > t.m) t.rescale(top, a.rate);
+#pragma unroll
+    for (int q = 0; q < kPerThread; ++q) t.s += r.exp(v[q] - t.m);
   }
   t = across(t, a.rate);
   if (lane == 0) red[w] = t;
   __syncthreads();
+  if (w != 0) return;
   t = red[0];
   for (int o = 1; o < kWaves; ++o) t.merge(red[o], a.rate);
-  if (w == 0) finish<E>(a, row, t, lane);
+  if (a.parts > 1) {
+    if (lane == 0) a.part_stats[row * a.parts + part] = t;
+    return;
+  }
+  finish<E, kSeen>(a, row, t, lane, seen);
 }
 
+// joins a row's parts: a wave a row
+template <class E>
+__global__ __launch_bounds__(kWave) void join_parts(Args a) {
+  __shared__ uint32_t seen[kSeen / 32];
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  if (a.probs) clear<kSeen>(seen, lane);
+  if (nothing(a, row, lane)) return;
+  Stats t = Stats::none();
+  for (int p = lane; p < a.parts; p += kWave) t.merge(a.part_stats[row * a.parts + p], a.rate);
+  finish<E, kSeen>(a, row, across(t, a.rate), lane, seen);
+}
+
+// ---- gradient ------------------------------------------------------------
 struct BwdArgs {
   const void *x;
   int64_t ld;
@@ -163,23 +284,133 @@ struct BwdArgs {
   void *dx;  // [R, V] contiguous
   int64_t R, V;
   int K;
+  int64_t per_row;  // groups of a row
 };
 
-template <class E>
+// GROUP threads have a tile of a row, 16 elements each.  The tile's tokens put
+// their p into LDS, at their element's place, and a bit that says that it is there.
+template <class E, int GROUP, bool VECTOR, bool STREAM>
 __global__ __launch_bounds__(kThreads) void gradient(BwdArgs a) {
-  const int64_t at = myelin::block_id() * kThreads + threadIdx.x;
-  if (at >= a.R * a.V) return;
-  const int64_t row = at / a.V, i = at - row * a.V;
-  const float m = a.stats[row], log_s = a.stats[a.R + row];
-  float d = 0.0f;
-  if (log_s != -kInf) {
-    const float x = E::get(static_cast<const typename E::T *>(a.x)[row * a.ld + i]);
-    d = myelin::exp_f32((x - m) * a.rate - log_s);
-    for (int k = 0; k < a.K; ++k)
-      if (a.tokens[row * a.K + k] == i) d -= a.probs[row * a.K + k];
-    d *= a.g[row] * a.rate;
+  using T = typename E::T;
+  constexpr int VEC = VECTOR ? E::VEC : 1, NV = kPerThread / VEC, TILE = GROUP * kPerThread;
+  typedef T vec __attribute__((ext_vector_type(VEC)));
+  __shared__ float put[kThreads / GROUP][TILE];
+  __shared__ uint32_t bits[kThreads / GROUP][TILE / 32];
+  const int tid = threadIdx.x % GROUP, group = threadIdx.x / GROUP;
+  const int64_t unit = myelin::block_id() * (kThreads / GROUP) + group, row = unit / a.per_row;
+  const int64_t at = (unit - row * a.per_row) * TILE;
+  const bool in = row < a.R;
+  const float m = in ? a.stats[row] : 0.0f, log_s = in ? a.stats[a.R + row] : -kInf;
+  const bool zero = log_s == -kInf;
+  const T *x = static_cast<const T *>(a.x) + (in ? row : 0) * a.ld;
+  T *dx = static_cast<T *>(a.dx) + row * a.V;
+  float v[kPerThread];
+  if (!zero) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int64_t i = at + (static_cast<int64_t>(j) * GROUP + tid) * VEC;
+      if (i >= a.V) continue;
+      if constexpr (VECTOR) {  // V is a multiple of VEC
+        const vec p = __builtin_nontemporal_load(reinterpret_cast<const vec *>(x + i));
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) v[j * VEC + q] = E::get(p[q]);
+      } else {
+        v[j] = E::get(x[i]);
+      }
+    }
   }
-  static_cast<typename E::T *>(a.dx)[at] = E::put(d);
+  if (tid < TILE / 32) bits[group][tid] = 0;
+  __syncthreads();
+  if (!zero)
+    for (int k = tid; k < a.K; k += GROUP) {
+      const int64_t o = a.tokens[row * a.K + k] - at;
+      const float p = a.probs[row * a.K + k];
+      if (p != 0.0f && o >= 0 && o < TILE) {
+        put[group][o] = p;
+        atomicOr(&bits[group][o / 32], 1u << (o % 32));
+      }
+    }
+  __syncthreads();
+  if (!in) return;
+  const float rate = a.rate * kLog2e, less = log_s * kLog2e, g = zero ? 0.0f : a.g[row] * a.rate;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int o = (j * GROUP + tid) * VEC;
+    const int64_t i = at + o;
+    if (i >= a.V) continue;
+    T out[VEC];
+    if (zero) {
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) out[q] = E::put(0.0f);
+    } else {
+      const uint32_t here = bits[group][o / 32] >> (o % 32);
+      float d[VEC];
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) d[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[j * VEC + q] - m, rate, -less));
+      if (here & ((1u << VEC) - 1)) {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q)
+          if (here >> q & 1) d[q] -= put[group][o + q];
+      }
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) out[q] = E::put(g * d[q]);
+    }
+    if constexpr (VECTOR) {
+      vec w;
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) w[q] = out[q];
+      myelin::store<STREAM>(w, reinterpret_cast<vec *>(dx + i));
+    } else {
+      dx[i] = out[0];
+    }
+  }
+}
+
+// Parts of a row: enough workgroups to fill the chip where rows are few, of
+// whole tiles.
+void split(int64_t R, int64_t V, int64_t *parts, int64_t *part) {
+  const int64_t tiles = (V + kTile - 1) / kTile;
+  int64_t n = R > 0 ? 512 / R : 1;
+  if (n < 1) n = 1;
+  if (n > tiles) n = tiles;
+  const int64_t per = (tiles + n - 1) / n;
+  *part = per * kTile;
+  *parts = (tiles + per - 1) / per;
+}
+
+template <class E>
+void launch_fwd(Args &a, hipStream_t s) {
+  if (a.V <= kNarrow) {
+    narrow_rows<E><<<myelin::grid_of((a.R + kWaves - 1) / kWaves), kThreads, 0, s>>>(a);
+    return;
+  }
+  a.rows = a.R < myelin::kGridX / a.parts ? a.R : myelin::kGridX / a.parts;
+  const dim3 grid(static_cast<unsigned>(a.rows * a.parts), static_cast<unsigned>((a.R + a.rows - 1) / a.rows));
+  wide_rows<E><<<grid, kThreads, 0, s>>>(a);
+  if (a.parts > 1) join_parts<E><<<static_cast<unsigned>(a.R), kWave, 0, s>>>(a);
+}
+
+template <class E, int GROUP>
+void launch_gradient(BwdArgs &a, hipStream_t s) {
+  a.per_row = (a.V + GROUP * kPerThread - 1) / (GROUP * kPerThread);
+  const int64_t units = a.R * a.per_row, each = kThreads / GROUP;
+  const dim3 grid = myelin::grid_of((units + each - 1) / each);
+  const bool vector = a.V % E::VEC == 0 && (a.ld * sizeof(typename E::T)) % 16 == 0 && myelin::aligned(a.x, 16) &&
+                      myelin::aligned(a.dx, 16);
+  if (!vector)
+    gradient<E, GROUP, false, false><<<grid, kThreads, 0, s>>>(a);
+  else if (a.R * a.V * static_cast<int64_t>(sizeof(typename E::T)) >= myelin::kStreamBytes)
+    gradient<E, GROUP, true, true><<<grid, kThreads, 0, s>>>(a);
+  else
+    gradient<E, GROUP, true, false><<<grid, kThreads, 0, s>>>(a);
+}
+
+template <class E>
+void launch_bwd(BwdArgs &a, hipStream_t s) {
+  if (a.V <= kNarrow)
+    launch_gradient<E, kWave>(a, s);
+  else
+    launch_gradient<E, kThreads>(a, s);
 }
 
 constexpr int kMaxTop = 1024;
@@ -198,7 +429,12 @@ int check(const char *what, const void *x, int dtype, int64_t ld, int64_t R, int
 
 }  // namespace
 
-extern "C" int64_t myelin_distillation_loss_workspace_bytes(int64_t R, int64_t V) { return 0; }
+extern "C" int64_t myelin_distillation_loss_workspace_bytes(int64_t R, int64_t V) {
+  if (R < 1 || V <= kNarrow) return 0;
+  int64_t parts, part;
+  split(R, V, &parts, &part);
+  return parts == 1 ? 0 : R * parts * static_cast<int64_t>(sizeof(Stats));
+}
 
 extern "C" int myelin_distillation_loss(const void *logits, int dtype, int64_t ld, const float *teacher_logits,
                                         const int64_t *teacher_tokens, float temperature, float *loss, float *probs,
@@ -208,12 +444,20 @@ extern "C" int myelin_distillation_loss(const void *logits, int dtype, int64_t l
   if (int rc = check(what, logits, dtype, ld, R, V, K, temperature)) return rc;
   if (R == 0) return MYELIN_OK;
   if (!teacher_logits || !teacher_tokens || !loss || !stats) return myelin::invalid("%s: null pointer", what);
-  Args a{logits, ld, teacher_logits, teacher_tokens, 1.0f / temperature, loss, probs, stats, R, V, K};
-  const dim3 grid = myelin::grid_of(R);
+  Args a{logits, ld, teacher_logits, teacher_tokens, 1.0f / temperature, loss, probs, stats, R, V, K, 1, V, R, nullptr};
+  if (const int64_t need = myelin_distillation_loss_workspace_bytes(R, V)) {
+    if (!workspace || workspace_bytes < need)
+      return myelin::invalid("%s: workspace of %lld bytes needed", what, static_cast<long long>(need));
+    if (!myelin::aligned(workspace, 16)) return myelin::invalid("%s: workspace must be 16-byte aligned", what);
+    int64_t parts;
+    split(R, V, &parts, &a.part);
+    a.parts = static_cast<int>(parts);
+    a.part_stats = static_cast<Stats *>(workspace);
+  }
   if (dtype == 0)
-    rows<F32><<<grid, kThreads, 0, myelin::as_hip(stream)>>>(a);
+    launch_fwd<F32>(a, myelin::as_hip(stream));
   else
-    rows<BF16><<<grid, kThreads, 0, myelin::as_hip(stream)>>>(a);
+    launch_fwd<BF16>(a, myelin::as_hip(stream));
   return myelin::launched(what);
 }
 
@@ -226,11 +470,10 @@ extern "C" int myelin_distillation_loss_bwd(const void *logits, int dtype, int64
   if (R == 0) return MYELIN_OK;
   if (!teacher_tokens || !probs || !stats || !grad_loss || !grad_logits)
     return myelin::invalid("%s: null pointer", what);
-  BwdArgs a{logits, ld, teacher_tokens, probs, stats, grad_loss, 1.0f / temperature, grad_logits, R, V, K};
-  const dim3 grid = myelin::grid_of((R * V + kThreads - 1) / kThreads);
+  BwdArgs a{logits, ld, teacher_tokens, probs, stats, grad_loss, 1.0f / temperature, grad_logits, R, V, K, 1};
   if (dtype == 0)
-    gradient<F32><<<grid, kThreads, 0, myelin::as_hip(stream)>>>(a);
+    launch_bwd<F32>(a, myelin::as_hip(stream));
   else
-    gradient<BF16><<<grid, kThreads, 0, myelin::as_hip(stream)>>>(a);
+    launch_bwd<BF16>(a, myelin::as_hip(stream));
   return myelin::launched(what);
 }
