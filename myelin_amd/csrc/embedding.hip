@@ -4,7 +4,13 @@
 //
 // A padding token's row is 0 and has no gradient; a token outside [0, V) gives a
 // row of NaN and has none either: nothing is read out of range.  The sums are
-// fp32, over the positions in order: the same bits on every run.
+// fp32, in an order that the positions alone decide: the same bits on every run.
+//
+// The gradient takes the positions in the order of their tokens (a stable sort), so
+// that each row of the table is written once, by the threads that sum it, and
+// nothing is atomic.  A token may have a tenth of all positions: a run of equal
+// tokens is cut at multiples of 64 sorted positions, whole pieces are summed by
+// workgroups of their own, and the row's threads add up what is left.
 
 #include "elements.h"
 
@@ -12,6 +18,9 @@ namespace {
 
 using myelin::BF16;
 using myelin::F32;
+using myelin::kWave;
+
+constexpr int kThreads = 256;
 
 struct Args {
   const int64_t *tokens;
@@ -19,39 +28,602 @@ struct Args {
   void *to;          // y [M, D]; backward: dw [V, D]
   int64_t ld, M, V, D, padding;
   float scale;
+  int64_t units;        // vectors of a row
+  int64_t slices;       // pieces of a row that a group of threads takes at a time
+  const int32_t *keys, *places, *starts;
+  float *pieces, *pieces2;
 };
 
-template <class E>
-__global__ __launch_bounds__(256) void lookup(Args a) {
-  using T = typename E::T;
-  const int64_t at = myelin::block_id() * 256 + threadIdx.x;
-  if (at >= a.M * a.D) return;
-  const int64_t i = at / a.D, d = at - i * a.D, token = a.tokens[i];
-  float v = 0.0f;
-  if (token != a.padding)
-    v = token < 0 || token >= a.V ? __builtin_nanf("")
-                                  : E::get(static_cast<const T *>(a.from)[token * a.ld + d]) * a.scale;
-  static_cast<T *>(a.to)[at] = E::put(v);
+// A row's threads: a power of two of them, each with a vector of VEC elements.
+int threads_of(int64_t units, int most) {
+  int t = 1;
+  while (t < most && t < units) t *= 2;
+  return t;
 }
 
-// a thread to an element of the table, over all positions
-template <class E>
-__global__ __launch_bounds__(256) void gradient(Args a) {
+template <class E, int VEC>
+struct Vector {
   using T = typename E::T;
-  const int64_t at = myelin::block_id() * 256 + threadIdx.x;
-  if (at >= a.V * a.D) return;
-  const int64_t v = at / a.D, d = at - v * a.D;
-  float sum = 0.0f;
-  if (v != a.padding)
-    for (int64_t i = 0; i < a.M; ++i)
-      if (a.tokens[i] == v) sum += E::get(static_cast<const T *>(a.from)[i * a.D + d]);
-  static_cast<T *>(a.to)[at] = E::put(sum * a.scale);
+  typedef T vec __attribute__((ext_vector_type(VEC)));
+  float v[VEC];
+  __device__ void zero() {
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) v[q] = 0.0f;
+  }
+  // (whole vectors only: D is a multiple of VEC)
+  __device__ void load(const T *p) {
+    if constexpr (VEC == 1) {
+      v[0] = E::get(*p);
+    } else {
+      const vec r = *reinterpret_cast<const vec *>(p);
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) v[q] = E::get(r[q]);
+    }
+  }
+  __device__ void add(const Vector &o) {
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) v[q] += o.v[q];
+  }
+  template <bool STREAM>
+  __device__ void store(T *p, float scale) const {
+    if constexpr (VEC == 1) {
+      *p = E::put(v[0] * scale);
+    } else {
+      vec r;
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) r[q] = E::put(v[q] * scale);
+      myelin::store<STREAM>(r, reinterpret_cast<vec *>(p));
+    }
+  }
+};
+
+// ---- lookup ----------------------------------------------------------------
+constexpr int kRows = 4;  // rows of a thread, loaded together
+
+// PER threads to a row (or a slice of it).
+template <class E, int VEC, bool STREAM>
+__global__ __launch_bounds__(kThreads) void lookup(Args a, int per) {
+  using T = typename E::T;
+  const int groups = kThreads / per, group = threadIdx.x / per;
+  const int64_t block = myelin::block_id(), rows = block / a.slices, slice = block - rows * a.slices;
+  const int64_t u = slice * per + threadIdx.x % per;
+  if (u >= a.units) return;
+  Vector<E, VEC> r[kRows];
+  int64_t i[kRows];
+#pragma unroll
+  for (int o = 0; o < kRows; ++o) {
+    i[o] = (rows * kRows + o) * groups + group;
+    if (i[o] >= a.M) continue;
+    const int64_t token = a.tokens[i[o]];
+    if (token == a.padding)
+      r[o].zero();
+    else if (token < 0 || token >= a.V)
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) r[o].v[q] = __builtin_nanf("");
+    else
+      r[o].load(static_cast<const T *>(a.from) + token * a.ld + u * VEC);
+  }
+#pragma unroll
+  for (int o = 0; o < kRows; ++o)
+    if (i[o] < a.M) r[o].template store<STREAM>(static_cast<T *>(a.to) + i[o] * a.D + u * VEC, a.scale);
+}
+
+// ---- gradient: the positions in the order of their tokens -------------------
+// A stable sort by digits of the key, the lowest first.  Padding and tokens outside
+// the table have the key V, behind all others.
+constexpr int kDigit = 9, kBins = 1 << kDigit;
+
+__device__ __forceinline__ int32_t key_of(const Args &a, int64_t i) {
+  const int64_t t = a.tokens[i];
+  return static_cast<int32_t>(t < 0 || t >= a.V || t == a.padding ? a.V : t);
+}
+
+// The lanes whose digit is this lane's, of those that have one.
+__device__ __forceinline__ uint64_t alike(int digit, bool in) {
+  uint64_t m = __ballot(in);
+#pragma unroll
+  for (int b = 0; b < kDigit; ++b) {
+    const uint64_t set = __ballot(digit >> b & 1);
+    m &= digit >> b & 1 ? set : ~set;
+  }
+  return m;
+}
+
+__device__ __forceinline__ int lower(uint64_t m) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), 0));
+}
+
+// Takes each wave's counts of the bins to where its items of them go, with `base`
+// for each bin the count of all smaller ones.  WAVES * 64 threads; scratch of kBins.
+template <int WAVES>
+__device__ __forceinline__ void offsets(int32_t (*count)[kBins], int32_t *scratch) {
+  const int tid = threadIdx.x;
+  for (int b = tid; b < kBins; b += WAVES * kWave) {
+    int32_t sum = 0;
+    for (int w = 0; w < WAVES; ++w) {
+      const int32_t c = count[w][b];
+      count[w][b] = sum;
+      sum += c;
+    }
+    scratch[b] = sum;
+  }
+  __syncthreads();
+  if (tid < kWave) {  // a wave adds the bins up: 8 each, then the lanes
+    constexpr int EACH = kBins / kWave;
+    int32_t v[EACH], sum = 0;
+    for (int o = 0; o < EACH; ++o) {
+      v[o] = scratch[tid * EACH + o];
+      sum += v[o];
+    }
+    int32_t run = sum;
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int32_t up = __shfl_up(run, o);
+      if (tid >= o) run += up;
+    }
+    run -= sum;
+    for (int o = 0; o < EACH; ++o) {
+      scratch[tid * EACH + o] = run;
+      run += v[o];
+    }
+  }
+  __syncthreads();
+  for (int b = tid; b < kBins; b += WAVES * kWave)
+    for (int w = 0; w < WAVES; ++w) count[w][b] += scratch[b];
+  __syncthreads();
+}
+
+// Up to 16384 positions: one workgroup, in LDS.  Each of 16 waves has a stretch of
+// the positions, 64 at a time.  (More are sorted by several workgroups, below.)
+constexpr int kOneWaves = 16, kOneRounds = 16, kOne = kOneWaves * kOneRounds * kWave;
+
+__global__ __launch_bounds__(kOneWaves * kWave) void sort_one(Args a, int rounds, int passes, int32_t *keys,
+                                                              int32_t *places) {
+  __shared__ int32_t key[kOne];
+  __shared__ uint16_t place[kOne];
+  __shared__ int32_t count[kOneWaves][kBins], scratch[kBins];
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, M = static_cast<int>(a.M);
+  const int first = wave * rounds * kWave;
+  int32_t k[kOneRounds], p[kOneRounds];
+#pragma unroll
+  for (int r = 0; r < kOneRounds; ++r) {
+    const int i = first + r * kWave + lane;
+    p[r] = i;
+    k[r] = r < rounds && i < M ? key_of(a, i) : 0;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * kDigit;
+    for (int b = lane; b < kBins; b += kWave) count[wave][b] = 0;
+#pragma unroll
+    for (int r = 0; r < kOneRounds; ++r)
+      if (r < rounds && first + r * kWave + lane < M) atomicAdd(&count[wave][k[r] >> shift & (kBins - 1)], 1);
+    __syncthreads();
+    offsets<kOneWaves>(count, scratch);
+#pragma unroll
+    for (int r = 0; r < kOneRounds; ++r) {
+      if (r >= rounds) continue;
+      const bool in = first + r * kWave + lane < M;
+      const int digit = k[r] >> shift & (kBins - 1);
+      const uint64_t m = alike(digit, in);
+      if (!in) continue;
+      const int rank = lower(m), to = count[wave][digit] + rank;
+      // (LDS of one wave is in order: the others have read it)
+      if (rank == 0) count[wave][digit] = to + __popcll(m);
+      if (pass + 1 < passes) {
+        key[to] = k[r];
+        place[to] = static_cast<uint16_t>(p[r]);
+      } else {
+        keys[to] = k[r];
+        places[to] = p[r];
+      }
+    }
+    __syncthreads();
+    if (pass + 1 < passes)
+#pragma unroll
+      for (int r = 0; r < kOneRounds; ++r) {
+        const int i = first + r * kWave + lane;
+        if (r < rounds && i < M) {
+          k[r] = key[i];
+          p[r] = place[i];
+        }
+      }
+  }
+}
+
+// More positions: each workgroup has a stretch, in turns of kTurn.  Its counts of
+// the bins, the offsets of all counts, and each position to its place.
+constexpr int kSortWaves = 4, kSortRounds = 16, kTurn = kSortWaves * kSortRounds * kWave;
+
+struct Sort {
+  Args a;
+  const int32_t *from_keys, *from_places;  // null: the tokens
+  int32_t *to_keys, *to_places, *counts;   // counts [kBins, blocks]
+  int blocks, shift;
+  int64_t stretch;  // a multiple of kTurn
+  __device__ int32_t key(int64_t i) const { return from_keys ? from_keys[i] : key_of(a, i); }
+  __device__ int32_t place(int64_t i) const { return from_keys ? from_places[i] : static_cast<int32_t>(i); }
+};
+
+__global__ __launch_bounds__(kThreads) void sort_count(Sort s) {
+  __shared__ int32_t count[kBins];
+  for (int b = threadIdx.x; b < kBins; b += kThreads) count[b] = 0;
+  __syncthreads();
+  const int64_t begin = blockIdx.x * s.stretch, end = begin + s.stretch < s.a.M ? begin + s.stretch : s.a.M;
+  for (int64_t i = begin + threadIdx.x; i < end; i += kThreads)
+    atomicAdd(&count[s.key(i) >> s.shift & (kBins - 1)], 1);
+  __syncthreads();
+  for (int b = threadIdx.x; b < kBins; b += kThreads) s.counts[static_cast<int64_t>(b) * s.blocks + blockIdx.x] = count[b];
+}
+
+// one workgroup: the sums of all counts before each
+__global__ __launch_bounds__(1024) void sort_offsets(int32_t *counts, int64_t n) {
+  __shared__ int32_t sums[16];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  constexpr int EACH = 8;
+  int32_t base = 0;
+  for (int64_t at = 0; at < n; at += 1024 * EACH) {
+    int32_t v[EACH], sum = 0;
+    const int64_t mine = at + tid * EACH;
+    for (int o = 0; o < EACH; ++o) {
+      v[o] = mine + o < n ? counts[mine + o] : 0;
+      sum += v[o];
+    }
+    int32_t run = sum;
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int32_t up = __shfl_up(run, o);
+      if (lane >= o) run += up;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) sums[wave] = run;
+    __syncthreads();
+    int32_t total = 0;
+    run += base - sum;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) run += sums[w];
+      total += sums[w];
+    }
+    for (int o = 0; o < EACH; ++o) {
+      if (mine + o < n) counts[mine + o] = run;
+      run += v[o];
+    }
+    base += total;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void sort_place(Sort s) {
+  __shared__ int32_t count[kSortWaves][kBins], next[kBins];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  for (int b = tid; b < kBins; b += kThreads) next[b] = s.counts[static_cast<int64_t>(b) * s.blocks + blockIdx.x];
+  const int64_t begin = blockIdx.x * s.stretch, end = begin + s.stretch < s.a.M ? begin + s.stretch : s.a.M;
+  for (int64_t turn = begin; turn < end; turn += kTurn) {
+    const int64_t first = turn + wave * kSortRounds * kWave + lane;
+    int32_t k[kSortRounds];
+    for (int b = lane; b < kBins; b += kWave) count[wave][b] = 0;
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      const int64_t i = first + r * kWave;
+      k[r] = i < end ? s.key(i) : 0;
+      if (i < end) atomicAdd(&count[wave][k[r] >> s.shift & (kBins - 1)], 1);
+    }
+    __syncthreads();
+    for (int b = tid; b < kBins; b += kThreads) {
+      int32_t run = next[b];
+      for (int w = 0; w < kSortWaves; ++w) {
+        const int32_t c = count[w][b];
+        count[w][b] = run;
+        run += c;
+      }
+      next[b] = run;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      const int64_t i = first + r * kWave;
+      const bool in = i < end;
+      const int digit = k[r] >> s.shift & (kBins - 1);
+      const uint64_t m = alike(digit, in);
+      if (!in) continue;
+      const int rank = lower(m), to = count[wave][digit] + rank;
+      if (rank == 0) count[wave][digit] = to + __popcll(m);
+      s.to_keys[to] = k[r];
+      s.to_places[to] = s.place(i);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- gradient: sums ---------------------------------------------------------
+constexpr int kPiece = 64;  // sorted positions of a piece, pieces of a larger one
+
+// Sums n rows (of the list places[0, n)) into r, in order, some loads at a time.
+template <class E, int VEC>
+__device__ __forceinline__ void sum_rows(const Args &a, const int32_t *places, int n, int64_t u, Vector<E, VEC> &r) {
+  using T = typename E::T;
+  const T *from = static_cast<const T *>(a.from) + u * VEC;
+  constexpr int MANY = 8;
+  int i = 0;
+  for (; i + MANY <= n; i += MANY) {
+    Vector<E, VEC> v[MANY];
+#pragma unroll
+    for (int o = 0; o < MANY; ++o) v[o].load(from + places[i + o] * a.D);
+#pragma unroll
+    for (int o = 0; o < MANY; ++o) r.add(v[o]);
+  }
+  for (; i < n; ++i) {
+    Vector<E, VEC> v;
+    v.load(from + places[i] * a.D);
+    r.add(v);
+  }
+}
+
+// fp32 rows [n, D] in a row
+template <class E, int VEC>
+__device__ __forceinline__ void sum_pieces(const float *from, int64_t n, int64_t D, Vector<E, VEC> &r) {
+  constexpr int MANY = 4;
+  int64_t i = 0;
+  for (; i + MANY <= n; i += MANY) {
+    float v[MANY][VEC];
+#pragma unroll
+    for (int o = 0; o < MANY; ++o)
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) v[o][q] = from[(i + o) * D + q];
+#pragma unroll
+    for (int o = 0; o < MANY; ++o)
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) r.v[q] += v[o][q];
+  }
+  for (; i < n; ++i)
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) r.v[q] += from[i * D + q];
+}
+
+// Adds up the groups' vectors, in their order, into the first group's.
+template <class E, int VEC>
+__device__ __forceinline__ void join(float *red, int groups, int group, int per, int at, Vector<E, VEC> &r) {
+#pragma unroll
+  for (int q = 0; q < VEC; ++q) red[(group * per + at) * VEC + q] = r.v[q];
+  __syncthreads();
+  if (group == 0)
+    for (int o = 1; o < groups; ++o)
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) r.v[q] += red[(o * per + at) * VEC + q];
+}
+
+// The pieces of the sorted positions that one token has, a workgroup each (and
+// slice); the workgroups after them find where each token's positions start.
+template <class E, int VEC>
+__global__ __launch_bounds__(kThreads) void sum_whole_pieces(Args a, int per, int64_t blocks, int32_t *starts) {
+  __shared__ float red[kThreads * VEC];
+  const int64_t block = myelin::block_id();
+  if (block >= blocks) {
+    const int64_t v = (block - blocks) * kThreads + threadIdx.x;
+    if (v > a.V) return;
+    int64_t lo = 0, hi = a.M;  // the first whose key is at least v
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (a.keys[mid] < v)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    starts[v] = static_cast<int32_t>(lo);
+    return;
+  }
+  const int64_t piece = block / a.slices, slice = block - piece * a.slices, at = piece * kPiece;
+  if (a.keys[at] != a.keys[at + kPiece - 1] || a.keys[at] == a.V) return;  // the whole workgroup
+  const int groups = kThreads / per, group = threadIdx.x / per, lane = threadIdx.x % per;
+  const int64_t u = slice * per + lane;
+  Vector<E, VEC> r;
+  r.zero();
+  const int each = kPiece / groups > 0 ? kPiece / groups : 1, used = kPiece / each;
+  if (u < a.units && group < used) sum_rows<E, VEC>(a, a.places + at + group * each, each, u, r);
+  join<E, VEC>(red, used < groups ? used : groups, group, per, lane, r);
+  if (group == 0 && u < a.units)
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) a.pieces[piece * a.D + u * VEC + q] = r.v[q];
+}
+
+// and 64 of those that one token has
+template <class E, int VEC>
+__global__ __launch_bounds__(kThreads) void sum_larger_pieces(Args a, int per) {
+  __shared__ float red[kThreads * VEC];
+  const int64_t block = myelin::block_id();
+  const int64_t piece = block / a.slices, slice = block - piece * a.slices, at = piece * kPiece * kPiece;
+  if (at + kPiece * kPiece > a.M || a.keys[at] != a.keys[at + kPiece * kPiece - 1] || a.keys[at] == a.V) return;
+  const int groups = kThreads / per, group = threadIdx.x / per, lane = threadIdx.x % per;
+  const int64_t u = slice * per + lane;
+  Vector<E, VEC> r;
+  r.zero();
+  const int each = kPiece / groups > 0 ? kPiece / groups : 1, used = kPiece / each;
+  if (u < a.units && group < used)
+    sum_pieces<E, VEC>(a.pieces + (piece * kPiece + group * each) * a.D + u * VEC, each, a.D, r);
+  join<E, VEC>(red, used < groups ? used : groups, group, per, lane, r);
+  if (group == 0 && u < a.units)
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) a.pieces2[piece * a.D + u * VEC + q] = r.v[q];
+}
+
+// Each row of the table: what of its run is before the first whole piece, the whole
+// pieces (the larger ones among them), what is behind them.
+template <class E, int VEC, bool STREAM>
+__global__ __launch_bounds__(kThreads) void sum_runs(Args a, int per) {
+  using T = typename E::T;
+  const int groups = kThreads / per, group = threadIdx.x / per;
+  const int64_t block = myelin::block_id(), rows = block / a.slices, slice = block - rows * a.slices;
+  const int64_t v = rows * groups + group, u = slice * per + threadIdx.x % per;
+  if (v >= a.V || u >= a.units) return;
+  const int64_t lo = a.starts[v], hi = a.starts[v + 1];
+  Vector<E, VEC> r;
+  r.zero();
+  const int64_t p0 = (lo + kPiece - 1) / kPiece, p1 = hi / kPiece;
+  if (p0 >= p1) {
+    sum_rows<E, VEC>(a, a.places + lo, static_cast<int>(hi - lo), u, r);
+  } else {
+    sum_rows<E, VEC>(a, a.places + lo, static_cast<int>(p0 * kPiece - lo), u, r);
+    const float *pieces = a.pieces + u * VEC;
+    const int64_t l0 = (p0 + kPiece - 1) / kPiece, l1 = p1 / kPiece;
+    if (!a.pieces2 || l0 >= l1) {
+      sum_pieces<E, VEC>(pieces + p0 * a.D, p1 - p0, a.D, r);
+    } else {
+      sum_pieces<E, VEC>(pieces + p0 * a.D, l0 * kPiece - p0, a.D, r);
+      sum_pieces<E, VEC>(a.pieces2 + u * VEC + l0 * a.D, l1 - l0, a.D, r);
+      sum_pieces<E, VEC>(pieces + l1 * kPiece * a.D, p1 - l1 * kPiece, a.D, r);
+    }
+    sum_rows<E, VEC>(a, a.places + p1 * kPiece, static_cast<int>(hi - p1 * kPiece), u, r);
+  }
+  r.template store<STREAM>(static_cast<T *>(a.to) + v * a.D + u * VEC, a.scale);
+}
+
+// ---- gradient: few tokens, small tables -------------------------------------
+// A workgroup to a row (and slice): it goes through all tokens itself, keeps the
+// positions of its own in order, and sums their rows.  No sort, one launch.
+constexpr int kFewThreads = 512, kFew = 4096;
+
+template <class E, int VEC>
+__global__ __launch_bounds__(kFewThreads) void sum_few(Args a, int per) {
+  using T = typename E::T;
+  __shared__ int32_t list[kFew];
+  __shared__ int found[kFew / kFewThreads][kFewThreads / kWave];
+  __shared__ float red[kFewThreads * VEC];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const int64_t block = myelin::block_id(), v = block / a.slices, slice = block - v * a.slices;
+  constexpr int ROUNDS = kFew / kFewThreads, WAVES = kFewThreads / kWave;
+  uint64_t hit[ROUNDS];
+#pragma unroll
+  for (int o = 0; o < ROUNDS; ++o) {
+    const int i = o * kFewThreads + tid;
+    hit[o] = __ballot(i < a.M && key_of(a, i) == v);
+    if (lane == 0) found[o][wave] = __popcll(hit[o]);
+  }
+  __syncthreads();
+  int before = 0, n = 0;
+#pragma unroll
+  for (int o = 0; o < ROUNDS; ++o) {
+    for (int w = 0; w < WAVES; ++w) {
+      if (w == wave) before = n;
+      n += found[o][w];
+    }
+    if (hit[o] >> lane & 1) list[before + lower(hit[o])] = o * kFewThreads + tid;
+  }
+  __syncthreads();
+  const int groups = kFewThreads / per, group = tid / per, at = tid % per;
+  const int64_t u = slice * per + at;
+  const int each = (n + groups - 1) / groups, from = group * each < n ? group * each : n,
+            to = from + each < n ? from + each : n;
+  Vector<E, VEC> r;
+  r.zero();
+  if (u < a.units) sum_rows<E, VEC>(a, list + from, to - from, u, r);
+  join<E, VEC>(red, groups, group, per, at, r);
+  if (group == 0 && u < a.units)
+    r.template store<false>(static_cast<T *>(a.to) + v * a.D + u * VEC, a.scale);
+}
+
+// ---- launches ---------------------------------------------------------------
+struct Layout {  // of the workspace, in bytes
+  bool few, one;
+  int passes, blocks;
+  int64_t stretch, keys[2], places[2], counts, starts, pieces, pieces2, size;
+};
+
+// Rows of the table times slices that sum_few is taken for: each goes through all
+// tokens.
+constexpr int64_t kFewRows = 2048;
+
+Layout layout_of(int64_t M, int64_t V, int64_t D) {
+  Layout l{};
+  l.few = M <= kFew && V * ((D + 63) / 64) <= kFewRows;
+  if (l.few || M == 0) return l;
+  l.one = M <= kOne;
+  int bits = 1;
+  while (V >> bits) ++bits;
+  l.passes = (bits + kDigit - 1) / kDigit;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += (bytes + 15) / 16 * 16;
+    return here;
+  };
+  for (int o = 0; o < (l.one ? 1 : 2); ++o) {
+    l.keys[o] = take(4 * M);
+    l.places[o] = take(4 * M);
+  }
+  if (!l.one) {
+    // up to 1024 workgroups, of whole turns
+    const int64_t turns = (M + kTurn - 1) / kTurn, each = (turns + 1023) / 1024;
+    l.stretch = each * kTurn;
+    l.blocks = static_cast<int>((M + l.stretch - 1) / l.stretch);
+    l.counts = take(4 * static_cast<int64_t>(kBins) * l.blocks);
+  }
+  l.starts = take(4 * (V + 1));
+  l.pieces = take(4 * (M / kPiece) * D);
+  // (a run of 16384 has 256 pieces: few enough to add up at once)
+  l.pieces2 = l.one ? -1 : take(4 * (M / (kPiece * kPiece)) * D);
+  l.size = at;
+  return l;
+}
+
+template <class E, int VEC>
+void launch_lookup(Args &a, hipStream_t s) {
+  a.units = a.D / VEC;
+  const int per = threads_of(a.units, kThreads);
+  a.slices = (a.units + per - 1) / per;
+  const int64_t rows = static_cast<int64_t>(kThreads / per) * kRows;
+  const dim3 grid = myelin::grid_of((a.M + rows - 1) / rows * a.slices);
+  if (a.M * a.D * static_cast<int64_t>(sizeof(typename E::T)) >= myelin::kStreamBytes)
+    lookup<E, VEC, true><<<grid, kThreads, 0, s>>>(a, per);
+  else
+    lookup<E, VEC, false><<<grid, kThreads, 0, s>>>(a, per);
+}
+
+template <class E, int VEC>
+void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
+  a.units = a.D / VEC;
+  if (l.few) {
+    const int per = threads_of(a.units, kWave);
+    a.slices = (a.units + per - 1) / per;
+    sum_few<E, VEC><<<myelin::grid_of(a.V * a.slices), kFewThreads, 0, s>>>(a, per);
+    return;
+  }
+  a.starts = reinterpret_cast<int32_t *>(ws + l.starts);
+  a.pieces = reinterpret_cast<float *>(ws + l.pieces);
+  a.pieces2 = l.pieces2 < 0 ? nullptr : reinterpret_cast<float *>(ws + l.pieces2);
+  const auto words = [&](int64_t at) { return reinterpret_cast<int32_t *>(ws + at); };
+  if (l.one) {
+    const int rounds = static_cast<int>((a.M + kOneWaves * kWave - 1) / (kOneWaves * kWave));
+    sort_one<<<1, kOneWaves * kWave, 0, s>>>(a, rounds, l.passes, words(l.keys[0]), words(l.places[0]));
+    a.keys = words(l.keys[0]);
+    a.places = words(l.places[0]);
+  } else {
+    for (int pass = 0; pass < l.passes; ++pass) {
+      Sort t{a, pass ? a.keys : nullptr, pass ? a.places : nullptr, words(l.keys[pass & 1]), words(l.places[pass & 1]),
+             words(l.counts), l.blocks, pass * kDigit, l.stretch};
+      sort_count<<<l.blocks, kThreads, 0, s>>>(t);
+      sort_offsets<<<1, 1024, 0, s>>>(t.counts, static_cast<int64_t>(kBins) * l.blocks);
+      sort_place<<<l.blocks, kThreads, 0, s>>>(t);
+      a.keys = t.to_keys;
+      a.places = t.to_places;
+    }
+  }
+  int per = threads_of(a.units, kWave);
+  a.slices = (a.units + per - 1) / per;
+  const int64_t blocks = a.M / kPiece * a.slices;
+  sum_whole_pieces<E, VEC><<<myelin::grid_of(blocks + a.V / kThreads + 1), kThreads, 0, s>>>(a, per, blocks,
+                                                                                        words(l.starts));
+  if (a.pieces2 && a.M >= kPiece * kPiece)
+    sum_larger_pieces<E, VEC><<<myelin::grid_of(a.M / (kPiece * kPiece) * a.slices), kThreads, 0, s>>>(a, per);
+  per = threads_of(a.units, kThreads);
+  a.slices = (a.units + per - 1) / per;
+  const int64_t rows = kThreads / per;
+  const dim3 grid = myelin::grid_of((a.V + rows - 1) / rows * a.slices);
+  if (a.V * a.D * static_cast<int64_t>(sizeof(typename E::T)) >= myelin::kStreamBytes)
+    sum_runs<E, VEC, true><<<grid, kThreads, 0, s>>>(a, per);
+  else
+    sum_runs<E, VEC, false><<<grid, kThreads, 0, s>>>(a, per);
 }
 
 int check(const char *what, int dtype, int64_t M, int64_t V, int64_t D, float scale) {
   if (dtype != 0 && dtype != 2) return myelin::invalid("%s: unsupported dtype %d", what, dtype);
   if (M < 0 || V < 1 || D < 1) return myelin::invalid("%s: V and D must be positive, M not negative", what);
-  if (M >= int64_t{1} << 31 || V >= int64_t{1} << 31 || D >= int64_t{1} << 31 || M * D >= int64_t{1} << 40 ||
+  if (M >= int64_t{1} << 30 || V >= int64_t{1} << 31 || D >= int64_t{1} << 31 || M * D >= int64_t{1} << 40 ||
       V * D >= int64_t{1} << 40)
     return myelin::invalid("%s: too many tokens or elements", what);
   if (!(__builtin_fabsf(scale) <= 3.402823466e38f)) return myelin::invalid("%s: scale must be finite", what);
@@ -68,16 +640,23 @@ extern "C" int myelin_token_embedding(const int64_t *tokens, const void *weight,
   if (V > 1 && ld < D) return myelin::invalid("%s: row stride below D", what);
   if (M == 0) return MYELIN_OK;
   if (!tokens || !weight || !out) return myelin::invalid("%s: null pointer", what);
-  Args a{tokens, weight, out, ld, M, V, D, padding, scale};
-  const dim3 grid = myelin::grid_of((M * D + 255) / 256);
+  Args a{};
+  a.tokens = tokens, a.from = weight, a.to = out, a.ld = ld, a.M = M, a.V = V, a.D = D;
+  a.padding = padding, a.scale = scale;
+  const int64_t size = dtype == 0 ? 4 : 2;
+  const bool vector = (D * size) % 16 == 0 && (V == 1 || (ld * size) % 16 == 0) && myelin::aligned(weight, 16) &&
+                      myelin::aligned(out, 16);
+  hipStream_t s = myelin::as_hip(stream);
   if (dtype == 0)
-    lookup<F32><<<grid, 256, 0, myelin::as_hip(stream)>>>(a);
+    vector ? launch_lookup<F32, F32::VEC>(a, s) : launch_lookup<F32, 1>(a, s);
   else
-    lookup<BF16><<<grid, 256, 0, myelin::as_hip(stream)>>>(a);
+    vector ? launch_lookup<BF16, BF16::VEC>(a, s) : launch_lookup<BF16, 1>(a, s);
   return myelin::launched(what);
 }
 
-extern "C" int64_t myelin_token_embedding_bwd_workspace_bytes(int64_t M, int64_t V, int64_t D) { return 0; }
+extern "C" int64_t myelin_token_embedding_bwd_workspace_bytes(int64_t M, int64_t V, int64_t D) {
+  return M < 1 || V < 1 || D < 1 ? 0 : layout_of(M, V, D).size;
+}
 
 extern "C" int myelin_token_embedding_bwd(const int64_t *tokens, const void *grad_out, int dtype, void *grad_weight,
                                           int64_t M, int64_t V, int64_t D, float scale, int64_t padding,
@@ -85,11 +664,23 @@ extern "C" int myelin_token_embedding_bwd(const int64_t *tokens, const void *gra
   const char *what = "token_embedding_bwd";
   if (int rc = check(what, dtype, M, V, D, scale)) return rc;
   if (!grad_weight || (M > 0 && (!tokens || !grad_out))) return myelin::invalid("%s: null pointer", what);
-  Args a{tokens, grad_out, grad_weight, D, M, V, D, padding, scale};
-  const dim3 grid = myelin::grid_of((V * D + 255) / 256);
+  Layout l = layout_of(M, V, D);
+  if (l.size) {
+    if (!workspace || workspace_bytes < l.size)
+      return myelin::invalid("%s: workspace of %lld bytes needed", what, static_cast<long long>(l.size));
+    if (!myelin::aligned(workspace, 16)) return myelin::invalid("%s: workspace must be 16-byte aligned", what);
+  }
+  Args a{};
+  a.tokens = tokens, a.from = grad_out, a.to = grad_weight, a.ld = D, a.M = M, a.V = V, a.D = D;
+  a.padding = padding, a.scale = scale;
+  if (M == 0) l.few = true;  // zeros
+  const int64_t size = dtype == 0 ? 4 : 2;
+  const bool vector = (D * size) % 16 == 0 && myelin::aligned(grad_out, 16) && myelin::aligned(grad_weight, 16);
+  hipStream_t s = myelin::as_hip(stream);
+  char *ws = static_cast<char *>(workspace);
   if (dtype == 0)
-    gradient<F32><<<grid, 256, 0, myelin::as_hip(stream)>>>(a);
+    vector ? launch_gradient<F32, F32::VEC>(a, l, ws, s) : launch_gradient<F32, 1>(a, l, ws, s);
   else
-    gradient<BF16><<<grid, 256, 0, myelin::as_hip(stream)>>>(a);
+    vector ? launch_gradient<BF16, BF16::VEC>(a, l, ws, s) : launch_gradient<BF16, 1>(a, l, ws, s);
   return myelin::launched(what);
 }
