@@ -88,24 +88,28 @@ __global__ __launch_bounds__(kThreads) void lookup(Args a, int per) {
   const int64_t block = myelin::block_id(), rows = block / a.slices, slice = block - rows * a.slices;
   const int64_t u = slice * per + threadIdx.x % per;
   if (u >= a.units) return;
+  // (what is not there is loaded from the last position and the first row: loads
+  // under conditions wait for each other)
   Vector<E, VEC> r[kRows];
-  int64_t i[kRows];
+  int64_t i[kRows], token[kRows];
 #pragma unroll
   for (int o = 0; o < kRows; ++o) {
     i[o] = (rows * kRows + o) * groups + group;
-    if (i[o] >= a.M) continue;
-    const int64_t token = a.tokens[i[o]];
-    if (token == a.padding)
-      r[o].zero();
-    else if (token < 0 || token >= a.V)
-#pragma unroll
-      for (int q = 0; q < VEC; ++q) r[o].v[q] = __builtin_nanf("");
-    else
-      r[o].load(static_cast<const T *>(a.from) + token * a.ld + u * VEC);
+    token[o] = a.tokens[i[o] < a.M ? i[o] : a.M - 1];
   }
 #pragma unroll
-  for (int o = 0; o < kRows; ++o)
-    if (i[o] < a.M) r[o].template store<STREAM>(static_cast<T *>(a.to) + i[o] * a.D + u * VEC, a.scale);
+  for (int o = 0; o < kRows; ++o) {
+    const bool inside = token[o] >= 0 && token[o] < a.V;
+    r[o].load(static_cast<const T *>(a.from) + (inside ? token[o] : 0) * a.ld + u * VEC);
+  }
+#pragma unroll
+  for (int o = 0; o < kRows; ++o) {
+    if (i[o] >= a.M) continue;
+    const bool hole = token[o] == a.padding, outside = token[o] < 0 || token[o] >= a.V;
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) r[o].v[q] = hole ? 0.0f : outside ? __builtin_nanf("") : r[o].v[q];
+    r[o].template store<STREAM>(static_cast<T *>(a.to) + i[o] * a.D + u * VEC, a.scale);
+  }
 }
 
 // ---- gradient: the positions in the order of their tokens -------------------
@@ -114,23 +118,40 @@ __global__ __launch_bounds__(kThreads) void lookup(Args a, int per) {
 constexpr int kDigit = 9, kBins = 1 << kDigit;
 
 __device__ __forceinline__ int32_t key_of(const Args &a, int64_t i) {
-  const int64_t t = a.tokens[i];
+  const int64_t t = a.tokens[i < a.M ? i : a.M - 1];
   return static_cast<int32_t>(t < 0 || t >= a.V || t == a.padding ? a.V : t);
 }
 
-// The lanes whose digit is this lane's, of those that have one.
+// The lanes whose digit is this lane's, of those that have one.  (BITS: 2 passes
+// of 8 bits rather than 9 where they will do: these ballots are what a sort takes.)
+template <int BITS>
 __device__ __forceinline__ uint64_t alike(int digit, bool in) {
-  uint64_t m = __ballot(in);
+  const uint64_t m = __ballot(in);
+  uint32_t lo = static_cast<uint32_t>(m), hi = static_cast<uint32_t>(m >> 32);
 #pragma unroll
-  for (int b = 0; b < kDigit; ++b) {
-    const uint64_t set = __ballot(digit >> b & 1);
-    m &= digit >> b & 1 ? set : ~set;
+  for (int b = 0; b < BITS; ++b) {
+    const int one = digit << (31 - b) >> 31;  // all ones where the bit is set
+    const uint64_t set = __ballot(one != 0);
+    lo &= ~(static_cast<uint32_t>(set) ^ one);
+    hi &= ~(static_cast<uint32_t>(set >> 32) ^ one);
   }
-  return m;
+  return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
 __device__ __forceinline__ int lower(uint64_t m) {
   return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(m >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(m), 0));
+}
+
+// An item's place among those of its digit that its wave has had, in `count`, which
+// it goes into.  (One lane of those alike writes it: as atomics, equal digits would
+// wait for each other.  In LDS a wave's accesses are done in its order.)
+template <int BITS>
+__device__ __forceinline__ int32_t place_in_wave(int32_t *count, int digit, bool in) {
+  const uint64_t m = alike<BITS>(digit, in);
+  const int rank = lower(m);
+  const int32_t had = in ? count[digit] : 0;
+  if (in && rank == 0) count[digit] = had + __popcll(m);
+  return had + rank;
 }
 
 // Takes each wave's counts of the bins to where its items of them go, with `base`
@@ -139,11 +160,13 @@ template <int WAVES>
 __device__ __forceinline__ void offsets(int32_t (*count)[kBins], int32_t *scratch) {
   const int tid = threadIdx.x;
   for (int b = tid; b < kBins; b += WAVES * kWave) {
-    int32_t sum = 0;
+    int32_t c[WAVES], sum = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) c[w] = count[w][b];
+#pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      const int32_t c = count[w][b];
       count[w][b] = sum;
-      sum += c;
+      sum += c[w];
     }
     scratch[b] = sum;
   }
@@ -167,8 +190,14 @@ __device__ __forceinline__ void offsets(int32_t (*count)[kBins], int32_t *scratc
     }
   }
   __syncthreads();
-  for (int b = tid; b < kBins; b += WAVES * kWave)
-    for (int w = 0; w < WAVES; ++w) count[w][b] += scratch[b];
+  for (int b = tid; b < kBins; b += WAVES * kWave) {
+    const int32_t base = scratch[b];
+    int32_t c[WAVES];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) c[w] = count[w][b];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) count[w][b] = c[w] + base;
+  }
   __syncthreads();
 }
 
@@ -176,56 +205,70 @@ __device__ __forceinline__ void offsets(int32_t (*count)[kBins], int32_t *scratc
 // the positions, 64 at a time.  (More are sorted by several workgroups, below.)
 constexpr int kOneWaves = 16, kOneRounds = 16, kOne = kOneWaves * kOneRounds * kWave;
 
+//
+// One CU sorts and the others have nothing to do: where most rows of the table stay
+// 0 (more rows than positions), the other workgroups write all of it as zeros
+// meanwhile, and only rows with tokens are written after that.  16384 positions take
+// 26 us, of which two passes' ballots are 15; 134 MB of zeros take as long.
+template <int BITS>
 __global__ __launch_bounds__(kOneWaves * kWave) void sort_one(Args a, int rounds, int passes, int32_t *keys,
-                                                              int32_t *places) {
+                                                              int32_t *places, int64_t zeros) {
   __shared__ int32_t key[kOne];
   __shared__ uint16_t place[kOne];
   __shared__ int32_t count[kOneWaves][kBins], scratch[kBins];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, M = static_cast<int>(a.M);
+  if (blockIdx.x > 0) {  // `zeros` whole vectors of 16 bytes of the table
+    typedef float vec __attribute__((ext_vector_type(4)));
+    const int64_t step = static_cast<int64_t>(gridDim.x - 1) * (kOneWaves * kWave);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x - 1) * (kOneWaves * kWave) + threadIdx.x; i < zeros; i += step)
+      __builtin_nontemporal_store(vec{0.0f, 0.0f, 0.0f, 0.0f}, static_cast<vec *>(a.to) + i);
+    return;
+  }
   const int first = wave * rounds * kWave;
   int32_t k[kOneRounds], p[kOneRounds];
 #pragma unroll
   for (int r = 0; r < kOneRounds; ++r) {
     const int i = first + r * kWave + lane;
     p[r] = i;
-    k[r] = r < rounds && i < M ? key_of(a, i) : 0;
+    k[r] = key_of(a, i);
   }
   for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * kDigit;
+    const int shift = pass * BITS;
     for (int b = lane; b < kBins; b += kWave) count[wave][b] = 0;
+    // each item's place among the wave's of its digit
+    int32_t local[kOneRounds];
 #pragma unroll
-    for (int r = 0; r < kOneRounds; ++r)
-      if (r < rounds && first + r * kWave + lane < M) atomicAdd(&count[wave][k[r] >> shift & (kBins - 1)], 1);
+    for (int r = 0; r < kOneRounds; ++r) {
+      local[r] = 0;
+      if (r < rounds)
+        local[r] = place_in_wave<BITS>(count[wave], k[r] >> shift & ((1 << BITS) - 1), first + r * kWave + lane < M);
+    }
     __syncthreads();
     offsets<kOneWaves>(count, scratch);
 #pragma unroll
     for (int r = 0; r < kOneRounds; ++r) {
-      if (r >= rounds) continue;
-      const bool in = first + r * kWave + lane < M;
-      const int digit = k[r] >> shift & (kBins - 1);
-      const uint64_t m = alike(digit, in);
-      if (!in) continue;
-      const int rank = lower(m), to = count[wave][digit] + rank;
-      // (LDS of one wave is in order: the others have read it)
-      if (rank == 0) count[wave][digit] = to + __popcll(m);
-      if (pass + 1 < passes) {
+      if (r < rounds && first + r * kWave + lane < M) {
+        const int to = count[wave][k[r] >> shift & ((1 << BITS) - 1)] + local[r];
         key[to] = k[r];
         place[to] = static_cast<uint16_t>(p[r]);
-      } else {
-        keys[to] = k[r];
-        places[to] = p[r];
       }
     }
     __syncthreads();
-    if (pass + 1 < passes)
 #pragma unroll
-      for (int r = 0; r < kOneRounds; ++r) {
-        const int i = first + r * kWave + lane;
-        if (r < rounds && i < M) {
-          k[r] = key[i];
-          p[r] = place[i];
-        }
-      }
+    for (int r = 0; r < kOneRounds; ++r) {
+      const int i = first + r * kWave + lane;  // (what is not there is not looked at)
+      k[r] = key[i];
+      p[r] = place[i];
+    }
+  }
+  // (64 places of 64 lines would take a store 64 turns)
+#pragma unroll
+  for (int r = 0; r < kOneRounds; ++r) {
+    const int i = first + r * kWave + lane;
+    if (r < rounds && i < M) {
+      keys[i] = k[r];
+      places[i] = p[r];
+    }
   }
 }
 
@@ -239,7 +282,7 @@ struct Sort {
   int32_t *to_keys, *to_places, *counts;   // counts [kBins, blocks]
   int blocks, shift;
   int64_t stretch;  // a multiple of kTurn
-  __device__ int32_t key(int64_t i) const { return from_keys ? from_keys[i] : key_of(a, i); }
+  __device__ int32_t key(int64_t i) const { return from_keys ? from_keys[i < a.M ? i : a.M - 1] : key_of(a, i); }
   __device__ int32_t place(int64_t i) const { return from_keys ? from_places[i] : static_cast<int32_t>(i); }
 };
 
@@ -301,9 +344,12 @@ __global__ __launch_bounds__(kThreads) void sort_place(Sort s) {
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
       const int64_t i = first + r * kWave;
-      k[r] = i < end ? s.key(i) : 0;
-      if (i < end) atomicAdd(&count[wave][k[r] >> s.shift & (kBins - 1)], 1);
+      k[r] = s.key(i);
     }
+    int32_t local[kSortRounds];
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r)
+      local[r] = place_in_wave<kDigit>(count[wave], k[r] >> s.shift & (kBins - 1), first + r * kWave < end);
     __syncthreads();
     for (int b = tid; b < kBins; b += kThreads) {
       int32_t run = next[b];
@@ -318,14 +364,11 @@ __global__ __launch_bounds__(kThreads) void sort_place(Sort s) {
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
       const int64_t i = first + r * kWave;
-      const bool in = i < end;
-      const int digit = k[r] >> s.shift & (kBins - 1);
-      const uint64_t m = alike(digit, in);
-      if (!in) continue;
-      const int rank = lower(m), to = count[wave][digit] + rank;
-      if (rank == 0) count[wave][digit] = to + __popcll(m);
-      s.to_keys[to] = k[r];
-      s.to_places[to] = s.place(i);
+      if (i < end) {
+        const int32_t to = count[wave][k[r] >> s.shift & (kBins - 1)] + local[r];
+        s.to_keys[to] = k[r];
+        s.to_places[to] = s.place(i);
+      }
     }
     __syncthreads();
   }
@@ -443,34 +486,45 @@ __global__ __launch_bounds__(kThreads) void sum_larger_pieces(Args a, int per) {
 }
 
 // Each row of the table: what of its run is before the first whole piece, the whole
-// pieces (the larger ones among them), what is behind them.
-template <class E, int VEC, bool STREAM>
+// pieces (the larger ones among them), what is behind them.  ZEROED: rows without
+// positions are there already.
+constexpr int kTableRows = 4;  // of a group of threads
+
+template <class E, int VEC, bool STREAM, bool ZEROED>
 __global__ __launch_bounds__(kThreads) void sum_runs(Args a, int per) {
   using T = typename E::T;
   const int groups = kThreads / per, group = threadIdx.x / per;
   const int64_t block = myelin::block_id(), rows = block / a.slices, slice = block - rows * a.slices;
-  const int64_t v = rows * groups + group, u = slice * per + threadIdx.x % per;
-  if (v >= a.V || u >= a.units) return;
-  const int64_t lo = a.starts[v], hi = a.starts[v + 1];
-  Vector<E, VEC> r;
-  r.zero();
-  const int64_t p0 = (lo + kPiece - 1) / kPiece, p1 = hi / kPiece;
-  if (p0 >= p1) {
-    sum_rows<E, VEC>(a, a.places + lo, static_cast<int>(hi - lo), u, r);
-  } else {
-    sum_rows<E, VEC>(a, a.places + lo, static_cast<int>(p0 * kPiece - lo), u, r);
-    const float *pieces = a.pieces + u * VEC;
-    const int64_t l0 = (p0 + kPiece - 1) / kPiece, l1 = p1 / kPiece;
-    if (!a.pieces2 || l0 >= l1) {
-      sum_pieces<E, VEC>(pieces + p0 * a.D, p1 - p0, a.D, r);
+  const int64_t first = (rows * groups + group) * kTableRows, u = slice * per + threadIdx.x % per;
+  if (first >= a.V || u >= a.units) return;
+  int32_t start[kTableRows + 1];
+#pragma unroll
+  for (int o = 0; o <= kTableRows; ++o) start[o] = a.starts[first + o < a.V ? first + o : a.V];
+#pragma unroll
+  for (int o = 0; o < kTableRows; ++o) {
+    const int64_t v = first + o, lo = start[o], hi = start[o + 1];
+    if (v >= a.V) return;
+    if (ZEROED && lo == hi) continue;
+    Vector<E, VEC> r;
+    r.zero();
+    const int64_t p0 = (lo + kPiece - 1) / kPiece, p1 = hi / kPiece;
+    if (p0 >= p1) {
+      sum_rows<E, VEC>(a, a.places + lo, static_cast<int>(hi - lo), u, r);
     } else {
-      sum_pieces<E, VEC>(pieces + p0 * a.D, l0 * kPiece - p0, a.D, r);
-      sum_pieces<E, VEC>(a.pieces2 + u * VEC + l0 * a.D, l1 - l0, a.D, r);
-      sum_pieces<E, VEC>(pieces + l1 * kPiece * a.D, p1 - l1 * kPiece, a.D, r);
+      sum_rows<E, VEC>(a, a.places + lo, static_cast<int>(p0 * kPiece - lo), u, r);
+      const float *pieces = a.pieces + u * VEC;
+      const int64_t l0 = (p0 + kPiece - 1) / kPiece, l1 = p1 / kPiece;
+      if (!a.pieces2 || l0 >= l1) {
+        sum_pieces<E, VEC>(pieces + p0 * a.D, p1 - p0, a.D, r);
+      } else {
+        sum_pieces<E, VEC>(pieces + p0 * a.D, l0 * kPiece - p0, a.D, r);
+        sum_pieces<E, VEC>(a.pieces2 + u * VEC + l0 * a.D, l1 - l0, a.D, r);
+        sum_pieces<E, VEC>(pieces + l1 * kPiece * a.D, p1 - l1 * kPiece, a.D, r);
+      }
+      sum_rows<E, VEC>(a, a.places + p1 * kPiece, static_cast<int>(hi - p1 * kPiece), u, r);
     }
-    sum_rows<E, VEC>(a, a.places + p1 * kPiece, static_cast<int>(hi - p1 * kPiece), u, r);
+    r.template store<STREAM>(static_cast<T *>(a.to) + v * a.D + u * VEC, a.scale);
   }
-  r.template store<STREAM>(static_cast<T *>(a.to) + v * a.D + u * VEC, a.scale);
 }
 
 // ---- gradient: few tokens, small tables -------------------------------------
@@ -520,7 +574,7 @@ __global__ __launch_bounds__(kFewThreads) void sum_few(Args a, int per) {
 // ---- launches ---------------------------------------------------------------
 struct Layout {  // of the workspace, in bytes
   bool few, one;
-  int passes, blocks;
+  int passes, bits, blocks;
   int64_t stretch, keys[2], places[2], counts, starts, pieces, pieces2, size;
 };
 
@@ -536,6 +590,7 @@ Layout layout_of(int64_t M, int64_t V, int64_t D) {
   int bits = 1;
   while (V >> bits) ++bits;
   l.passes = (bits + kDigit - 1) / kDigit;
+  l.bits = (bits + l.passes - 1) / l.passes;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -587,9 +642,17 @@ void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
   a.pieces = reinterpret_cast<float *>(ws + l.pieces);
   a.pieces2 = l.pieces2 < 0 ? nullptr : reinterpret_cast<float *>(ws + l.pieces2);
   const auto words = [&](int64_t at) { return reinterpret_cast<int32_t *>(ws + at); };
+  const int64_t bytes = a.V * a.D * static_cast<int64_t>(sizeof(typename E::T));
+  const bool zeroed = l.one && a.V > a.M && bytes % 16 == 0 && myelin::aligned(a.to, 16);
   if (l.one) {
+    // (workgroups of 256 KB: a CU has one at a time)
+    const int64_t zeros = zeroed ? bytes / 16 : 0, fill = (zeros + 16383) / 16384;
+    const unsigned grid = static_cast<unsigned>(1 + (fill < 4096 ? fill : 4096));
     const int rounds = static_cast<int>((a.M + kOneWaves * kWave - 1) / (kOneWaves * kWave));
-    sort_one<<<1, kOneWaves * kWave, 0, s>>>(a, rounds, l.passes, words(l.keys[0]), words(l.places[0]));
+    if (l.bits <= 8)
+      sort_one<8><<<grid, kOneWaves * kWave, 0, s>>>(a, rounds, l.passes, words(l.keys[0]), words(l.places[0]), zeros);
+    else
+      sort_one<9><<<grid, kOneWaves * kWave, 0, s>>>(a, rounds, l.passes, words(l.keys[0]), words(l.places[0]), zeros);
     a.keys = words(l.keys[0]);
     a.places = words(l.places[0]);
   } else {
@@ -612,12 +675,15 @@ void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
     sum_larger_pieces<E, VEC><<<myelin::grid_of(a.M / (kPiece * kPiece) * a.slices), kThreads, 0, s>>>(a, per);
   per = threads_of(a.units, kThreads);
   a.slices = (a.units + per - 1) / per;
-  const int64_t rows = kThreads / per;
+  const int64_t rows = kThreads / per * kTableRows;
   const dim3 grid = myelin::grid_of((a.V + rows - 1) / rows * a.slices);
-  if (a.V * a.D * static_cast<int64_t>(sizeof(typename E::T)) >= myelin::kStreamBytes)
-    sum_runs<E, VEC, true><<<grid, kThreads, 0, s>>>(a, per);
+  const bool stream = bytes >= myelin::kStreamBytes;
+  if (zeroed)
+    stream ? sum_runs<E, VEC, true, true><<<grid, kThreads, 0, s>>>(a, per)
+           : sum_runs<E, VEC, false, true><<<grid, kThreads, 0, s>>>(a, per);
   else
-    sum_runs<E, VEC, false><<<grid, kThreads, 0, s>>>(a, per);
+    stream ? sum_runs<E, VEC, true, false><<<grid, kThreads, 0, s>>>(a, per)
+           : sum_runs<E, VEC, false, false><<<grid, kThreads, 0, s>>>(a, per);
 }
 
 int check(const char *what, int dtype, int64_t M, int64_t V, int64_t D, float scale) {

@@ -406,7 +406,9 @@ variable_list gated_recurrence_step(const Tensor &x, const Tensor &gate, const T
 // ---- embedding -----------------------------------------------------------
 Tensor embedded(const Tensor &weight, const Tensor &tokens, double scale, int64_t padding) {
   const int64_t M = tokens.numel(), V = weight.size(0), D = weight.size(1);
-  Tensor out = torch::empty({M, D}, weight.options());
+  std::vector<int64_t> shape = tokens.sizes().vec();
+  shape.push_back(D);
+  Tensor out = torch::empty(shape, weight.options());
   check(lib.embedding(i64(tokens), at(weight), code_of(weight), weight.stride(0), at(out), M, V, D,
                       static_cast<float>(scale), padding, stream_of(weight)),
         "myelin_token_embedding");
@@ -441,9 +443,10 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
   }
 };
 
-// weight with rows of unit stride, tokens [M] int64 contiguous
-Tensor token_embedding(const Tensor &weight, const Tensor &tokens, double scale, int64_t padding) {
+// weight with rows of unit stride
+Tensor token_embedding(const Tensor &weight, const Tensor &given, double scale, int64_t padding) {
   const c10::DeviceGuard guard(weight.device());
+  const Tensor tokens = given.to(torch::kInt64).contiguous();
   if (needs({weight})) return EmbeddingFunction::apply(weight, tokens, scale, padding);
   return embedded(weight, tokens, scale, padding);
 }

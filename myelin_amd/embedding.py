@@ -19,7 +19,7 @@ NO_PADDING = -(2**63)  # no token has this number
 def _forward(tokens, weight, scale, padding):
     V, D = weight.shape
     M = tokens.numel()
-    out = torch.empty((M, D), dtype=weight.dtype, device=weight.device)
+    out = torch.empty((*tokens.shape, D), dtype=weight.dtype, device=weight.device)
     with _device_of(weight):
         _lib.call("myelin_token_embedding", tokens.data_ptr(), weight.data_ptr(), _lib.DT[weight.dtype],
                   weight.stride(0), out.data_ptr(), M, V, D, scale, padding, _lib.stream(weight.device))
@@ -88,15 +88,12 @@ def token_embedding(
     if padding_index is not None and not -(2**63) < padding_index < 2**63:
         raise ValueError(f"padding_index must fit 64 bits; got {padding_index}")
     padding = NO_PADDING if padding_index is None else padding_index
-    flat = tokens.reshape(-1).to(torch.int64).contiguous()
     if (weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]) or (
             weight.stride(1) != 1 and weight.shape[1] > 1):
         weight = weight.contiguous()
     if autograd.plain(weight):
-        out = autograd.native().token_embedding(weight, flat, scale, padding)
-    else:
-        out = HipTokenEmbeddingFunction.apply(weight, flat, scale, padding)
-    return out.view(*tokens.shape, weight.shape[1])
+        return autograd.native().token_embedding(weight, tokens, scale, padding)
+    return HipTokenEmbeddingFunction.apply(weight, tokens.to(torch.int64).contiguous(), scale, padding)
 
 
 class TokenEmbedding(nn.Module):
