@@ -23,6 +23,7 @@ using myelin::F32;
 constexpr int kSteps = 16;     // steps of a wave at a time
 constexpr int kBackSteps = 8;  // and in the backward pass; and steps between two kept states
 constexpr int kMaxWaves = 16;
+constexpr int kWave = myelin::kWave;
 
 struct Affine;
 
@@ -39,12 +40,16 @@ struct Args {
   Affine *joins;                             // [segments, B, N]
 };
 
-// sigmoid and 1 - sigmoid, each to its own accuracy
+// sigmoid and 1 - sigmoid, each to its own accuracy.  fp32 puts the rounding of the
+// exponential's argument back, |g| 2^-24 of the smaller of the two.  A bf16 gate is
+// itself only known to |g| 2^-9.
+template <class E>
 struct Gate {
   float a, b;
   __device__ explicit Gate(float g) {
-    const float e = myelin::exp_f32(-__builtin_fabsf(g));
-    const float r = myelin::recip_rn(1.0f + e), s = e * r;
+    const float d = -__builtin_fabsf(g);
+    const float e = sizeof(typename E::T) == 4 ? myelin::exp_f32(d) : __builtin_amdgcn_exp2f(d * myelin::kLog2e);
+    const float r = __builtin_amdgcn_rcpf(1.0f + e), s = e * r;
     a = g >= 0.0f ? r : s;
     b = g >= 0.0f ? s : r;
   }
@@ -52,66 +57,76 @@ struct Gate {
 
 constexpr float kInf = __builtin_huge_valf();
 
-// A workgroup has 64 channels, a lane each, and walks over time in tiles: each of
-// its waves takes the next kSteps steps, into registers.  A run of steps maps the
-// state before it to the one after it as h -> A h + H; the waves exchange A and H
-// in LDS, join those before them to their own first state and only then run their
-// steps again.  x and gate are read once.
+// A run of steps maps the state before it to the one after it as h -> A h + H.
 struct Affine {
   float A, H;
 };
 
-// A lane's channel.  Rows are addressed from bases that the workgroup shares, with
-// 32-bit byte offsets of the lanes: a load takes no address registers of its own.
+// A workgroup has 64 channels, a lane each, and walks over time in tiles: each of its
+// waves takes the next STEPS steps, into registers; the waves exchange A and H of
+// their steps in LDS, join those before them to their own first state and only then
+// run their steps again.  x and gate are read once.  (Two groups of 32 channels to a
+// wave, for twice the workgroups, read rows in pieces of 64 bytes: [2048, 8, 2048]
+// bf16 48 -> 62 us forward, 88 -> 105 us backward.)
+//
+// Rows are addressed from bases that the wave shares, with 32-bit byte offsets of
+// the lanes: a load takes no address registers of its own.
+template <int STEPS>
 struct Place {
   int64_t first;  // the workgroup's first channel, of B * N
   int lane, wave, waves;
+  int64_t live;                    // the channel's steps
   bool in;
-  int64_t live;                   // its steps
-  const char *x, *gate, *out;     // of the first channel's batch row
+  const char *x, *gate, *out;      // of the first channel's batch row
   uint32_t at_x, at_gate, at_out;  // bytes from there
   __device__ int64_t c() const { return first + lane; }
+  __device__ int64_t tile_steps() const { return waves * STEPS; }
+  // the wave's first step of a tile, and how many the lane has from there
+  __device__ int64_t step(int64_t tile) const { return tile + wave * STEPS; }
+  __device__ int steps(int64_t tile) const {
+    const int64_t n = live - step(tile);
+    return n < 0 ? 0 : n < STEPS ? static_cast<int>(n) : STEPS;
+  }
+
+  template <class T>
+  __device__ void set(const Args &a, int64_t block) {
+    lane = threadIdx.x % kWave;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    waves = blockDim.x / kWave;
+    first = block * kWave;
+    in = c() < a.B * a.N;
+    const int64_t mine = in ? c() : first;
+    const int64_t b0 = first / a.N, b = mine / a.N, n = mine - b * a.N;
+    x = reinterpret_cast<const char *>(static_cast<const T *>(a.x) + b0 * a.xb);
+    gate = reinterpret_cast<const char *>(static_cast<const T *>(a.gate) + b0 * a.gb);
+    out = reinterpret_cast<const char *>(static_cast<const T *>(a.g_out) + b0 * a.ob);
+    at_x = static_cast<uint32_t>(((b - b0) * a.xb + n) * sizeof(T));
+    at_gate = static_cast<uint32_t>(((b - b0) * a.gb + n) * sizeof(T));
+    at_out = static_cast<uint32_t>(((b - b0) * a.ob + n) * sizeof(T));
+    live = a.T;
+    if (a.lengths) {
+      live = a.lengths[b];
+      live = live < 0 ? 0 : live < a.T ? live : a.T;
+    }
+    if (!in) live = 0;
+  }
+
+  // The lane's STEPS values of a tile.  Rows past the last are the last; what a lane
+  // has no step for is masked afterwards (loads under conditions wait for each other).
+  template <class T>
+  __device__ void load(T *v, const char *from, uint32_t at, int64_t stride, int64_t tile, int64_t steps) const {
+    const int64_t t0 = step(tile), row = stride * static_cast<int64_t>(sizeof(T));
+    const char *p = from + t0 * row;
+    if (t0 + STEPS <= steps) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) v[i] = *reinterpret_cast<const T *>(p + i * row + at);
+    } else {
+      const int last = static_cast<int>(steps - 1 - t0);
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) v[i] = *reinterpret_cast<const T *>(p + (i < last ? i : last) * row + at);
+    }
+  }
 };
-
-template <class T>
-__device__ __forceinline__ Place place_of(const Args &a, int64_t block) {
-  Place p;
-  p.lane = threadIdx.x & (myelin::kWave - 1);
-  p.wave = __builtin_amdgcn_readfirstlane(threadIdx.x / myelin::kWave);
-  p.waves = blockDim.x / myelin::kWave;
-  p.first = block * myelin::kWave;
-  p.in = p.c() < a.B * a.N;
-  const int64_t b0 = p.first / a.N, b = (p.in ? p.c() : p.first) / a.N, n = (p.in ? p.c() : p.first) - b * a.N;
-  p.x = reinterpret_cast<const char *>(static_cast<const T *>(a.x) + b0 * a.xb);
-  p.gate = reinterpret_cast<const char *>(static_cast<const T *>(a.gate) + b0 * a.gb);
-  p.out = reinterpret_cast<const char *>(static_cast<const T *>(a.g_out) + b0 * a.ob);
-  p.at_x = static_cast<uint32_t>(((b - b0) * a.xb + n) * sizeof(T));
-  p.at_gate = static_cast<uint32_t>(((b - b0) * a.gb + n) * sizeof(T));
-  p.at_out = static_cast<uint32_t>(((b - b0) * a.ob + n) * sizeof(T));
-  int64_t live = a.T;
-  if (a.lengths) {
-    live = a.lengths[b];
-    live = live < 0 ? 0 : live < a.T ? live : a.T;
-  }
-  p.live = p.in ? live : 0;
-  return p;
-}
-
-// STEPS values from step t0 on.  Rows past the last are the last; what a lane has
-// no step for is masked below.
-template <int STEPS, class T>
-__device__ __forceinline__ void load(T *v, const char *from, uint32_t at, int64_t stride, int64_t t0, int64_t steps) {
-  const char *p = from + t0 * stride * static_cast<int64_t>(sizeof(T));
-  const int64_t row = stride * static_cast<int64_t>(sizeof(T));
-  if (t0 + STEPS <= steps) {
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) v[i] = *reinterpret_cast<const T *>(p + i * row + at);
-  } else {
-    const int last = static_cast<int>(steps - 1 - t0);
-#pragma unroll
-    for (int i = 0; i < STEPS; ++i) v[i] = *reinterpret_cast<const T *>(p + (i < last ? i : last) * row + at);
-  }
-}
 
 template <int STEPS, class T>
 __device__ __forceinline__ void mask(T *v, int n, T past) {
@@ -119,57 +134,57 @@ __device__ __forceinline__ void mask(T *v, int n, T past) {
   for (int i = 0; i < STEPS; ++i) v[i] = i < n ? v[i] : past;
 }
 
-template <int STEPS>
-__device__ __forceinline__ int steps_from(const Place &p, int64_t t0) {
-  const int64_t n = p.live - t0;
-  return n < 0 ? 0 : n < STEPS ? static_cast<int>(n) : STEPS;
-}
-
-// The state before segment `seg` of a sequence, from the one before the first.
-__device__ __forceinline__ float join_before(const Args &a, const Place &p, float s) {
+// The state before segment a.seg, from the one before the first.
+__device__ __forceinline__ float join_before(const Args &a, int64_t c, float s) {
   for (int64_t o = 0; o < a.seg; ++o) {
-    const Affine m = a.joins[o * a.B * a.N + p.c()];
+    const Affine m = a.joins[o * a.B * a.N + c];
     s = __builtin_fmaf(m.A, s, m.H);
   }
   return s;
 }
-__device__ __forceinline__ float join_after(const Args &a, const Place &p, float s) {
+__device__ __forceinline__ float join_after(const Args &a, int64_t c, float s) {
   for (int64_t o = a.segments - 1; o > a.seg; --o) {
-    const Affine m = a.joins[o * a.B * a.N + p.c()];
+    const Affine m = a.joins[o * a.B * a.N + c];
     s = __builtin_fmaf(m.A, s, m.H);
   }
   return s;
 }
 
-// A block's channels and segment.
-__device__ __forceinline__ int64_t locate(Args &a) {
-  const int64_t block = myelin::block_id();
-  a.seg = block / a.blocks;
-  return block - a.seg * a.blocks;
+// A workgroup's segment and block of channels, or -1.  Consecutive workgroups run on
+// XCDs in turn; each XCD takes a stretch of the (segment, channels), so that blocks
+// that share lines of 128 bytes share an L2.
+__device__ __forceinline__ int64_t locate(Args &a, int64_t segments) {
+  constexpr int kXcds = 8;
+  const int64_t id = myelin::block_id(), units = a.blocks * segments, each = (units + kXcds - 1) / kXcds;
+  const int64_t unit = id % kXcds * each + id / kXcds;
+  if (id >= each * kXcds || unit >= units) return -1;
+  a.seg = unit / a.blocks;
+  return unit - a.seg * a.blocks;
 }
 
 template <class E>
-__global__ __launch_bounds__(kMaxWaves * myelin::kWave) void forward(Args a) {
+__global__ __launch_bounds__(kMaxWaves * kWave) void forward(Args a) {
   using T = typename E::T;
-  __shared__ Affine maps[2][kMaxWaves][myelin::kWave];
-  const int64_t block = locate(a);
-  if (a.seg >= a.segments) return;  // the whole workgroup
-  const Place p = place_of<T>(a, block);
-  const int lane = p.lane, wave = p.wave, waves = p.waves;
+  using P = Place<kSteps>;
+  __shared__ Affine maps[2][kMaxWaves][kWave];
+  const int64_t block = locate(a, a.segments);
+  if (block < 0) return;  // the whole workgroup
+  P p;
+  p.template set<T>(a, block);
   const int64_t BN = a.B * a.N, first = a.seg * a.seg_steps;
   const int64_t end = first + a.seg_steps < a.T ? first + a.seg_steps : a.T;
   float s = p.in && a.state ? a.state[p.c()] : 0.0f;
-  if (p.in) s = join_before(a, p, s);
+  if (p.in) s = join_before(a, p.c(), s);
   T x[kSteps], gate[kSteps];
-  int64_t t0 = first + wave * kSteps;
-  int n = steps_from<kSteps>(p, t0);
-  const auto fetch = [&]() {
+  int n = 0;
+  const auto fetch = [&](int64_t tile) {
+    n = p.steps(tile);
     if (!__any(n > 0)) return;
-    load<kSteps>(x, p.x, p.at_x, a.xt, t0, a.T);
-    load<kSteps>(gate, p.gate, p.at_gate, a.gt, t0, a.T);
+    p.load(x, p.x, p.at_x, a.xt, tile, a.T);
+    p.load(gate, p.gate, p.at_gate, a.gt, tile, a.T);
   };
-  fetch();
-  for (int64_t tile = first, turn = 0; tile < end; tile += waves * kSteps, ++turn) {
+  fetch(first);
+  for (int64_t tile = first, turn = 0; tile < end; tile += p.tile_steps(), ++turn) {
     const bool all = __all(n == kSteps);
     if (!all) {
       mask<kSteps>(x, n, E::put(0.0f));
@@ -179,75 +194,73 @@ __global__ __launch_bounds__(kMaxWaves * myelin::kWave) void forward(Args a) {
     Affine m{1.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      const Gate g(E::get(gate[i]));
+      const Gate<E> g(E::get(gate[i]));
       ra[i] = g.a;
       ru[i] = g.b * E::get(x[i]);
       m = {m.A * g.a, __builtin_fmaf(g.a, m.H, ru[i])};
     }
-    maps[turn & 1][wave][lane] = m;
-    const int64_t here = t0;
+    maps[turn & 1][p.wave][p.lane] = m;
     const int mine = n;
-    t0 += waves * kSteps;
-    if (tile + waves * kSteps < end) {
-      n = steps_from<kSteps>(p, t0);
-      fetch();
-    }
+    if (tile + p.tile_steps() < end) fetch(tile + p.tile_steps());
     __syncthreads();
     float h = s;
 #pragma unroll 4
-    for (int o = 0; o < waves; ++o) {
-      if (o == wave) h = s;
-      const Affine q = maps[turn & 1][o][lane];
+    for (int o = 0; o < p.waves; ++o) {
+      if (o == p.wave) h = s;
+      const Affine q = maps[turn & 1][o][p.lane];
       s = __builtin_fmaf(q.A, s, q.H);
     }
-    float *kept = a.kept && p.in ? a.kept + here / kBackSteps * BN + p.first : nullptr;
+    const int64_t here = p.step(tile);
+    const int left = p.in ? static_cast<int>(end - p.step(tile) < kSteps ? end - p.step(tile) : kSteps) : 0;
     T *out = static_cast<T *>(a.out) + here * BN + p.first;
+    float *kept = a.kept ? a.kept + here / kBackSteps * BN + p.first : nullptr;
     if (all) {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        if (kept && i % kBackSteps == 0) (kept + i / kBackSteps * BN)[lane] = h;
+        if (kept && i % kBackSteps == 0) (kept + i / kBackSteps * BN)[p.lane] = h;
         h = __builtin_fmaf(ra[i], h, ru[i]);
-        (out + i * BN)[lane] = E::put(h);
+        (out + i * BN)[p.lane] = E::put(h);
       }
-    } else if (p.in) {
+    } else {
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        if (kept && i % kBackSteps == 0 && here + i < end) (kept + i / kBackSteps * BN)[lane] = h;
+        if (kept && i % kBackSteps == 0 && i < left) (kept + i / kBackSteps * BN)[p.lane] = h;
         h = __builtin_fmaf(ra[i], h, ru[i]);
-        if (here + i < end) (out + i * BN)[lane] = E::put(i < mine ? h : 0.0f);
+        if (i < left) (out + i * BN)[p.lane] = E::put(i < mine ? h : 0.0f);
       }
     }
   }
-  if (p.in && wave == 0 && a.seg == a.segments - 1) a.state_out[p.c()] = s;
+  if (p.in && p.wave == 0 && a.seg == a.segments - 1) a.state_out[p.c()] = s;
 }
 
 template <class E>
-__global__ __launch_bounds__(kMaxWaves * myelin::kWave) void backward(Args a) {
+__global__ __launch_bounds__(kMaxWaves * kWave) void backward(Args a) {
   using T = typename E::T;
-  __shared__ Affine maps[2][kMaxWaves][myelin::kWave];
-  const int64_t block = locate(a);
-  if (a.seg >= a.segments) return;  // the whole workgroup
-  const Place p = place_of<T>(a, block);
-  const int lane = p.lane, wave = p.wave, waves = p.waves;
-  const int64_t BN = a.B * a.N, first = a.seg * a.seg_steps, tile_steps = waves * kBackSteps;
+  using P = Place<kBackSteps>;
+  __shared__ Affine maps[2][kMaxWaves][kWave];
+  const int64_t block = locate(a, a.segments);
+  if (block < 0) return;  // the whole workgroup
+  P p;
+  p.template set<T>(a, block);
+  const int64_t BN = a.B * a.N, first = a.seg * a.seg_steps;
   const int64_t end = first + a.seg_steps < a.T ? first + a.seg_steps : a.T;
   float s = p.in && a.state ? a.state[p.c()] : 0.0f;
-  if (p.in) s = join_after(a, p, s);
+  if (p.in) s = join_after(a, p.c(), s);
   T x[kBackSteps], gate[kBackSteps], go[kBackSteps];
   float start = 0.0f;
-  int64_t tile = first + (end - first - 1) / tile_steps * tile_steps;
-  int64_t t0 = tile + wave * kBackSteps;
-  int n = steps_from<kBackSteps>(p, t0);
-  const auto fetch = [&]() {
+  int n = 0;
+  const auto fetch = [&](int64_t tile) {
+    n = p.steps(tile);
     start = 0.0f;
     if (!__any(n > 0)) return;
-    load<kBackSteps>(x, p.x, p.at_x, a.xt, t0, a.T);
-    load<kBackSteps>(gate, p.gate, p.at_gate, a.gt, t0, a.T);
-    if (a.g_out) load<kBackSteps>(go, p.out, p.at_out, a.ot, t0, a.T);
-    if (p.in) start = (a.kept + t0 / kBackSteps * BN + p.first)[lane];
+    p.load(x, p.x, p.at_x, a.xt, tile, a.T);
+    p.load(gate, p.gate, p.at_gate, a.gt, tile, a.T);
+    if (a.g_out) p.load(go, p.out, p.at_out, a.ot, tile, a.T);
+    if (n > 0) start = (a.kept + p.step(tile) / kBackSteps * BN + p.first)[p.lane];
   };
-  fetch();
-  for (int64_t turn = 0; tile >= first; tile -= tile_steps, ++turn) {
+  int64_t tile = first + (end - first - 1) / p.tile_steps() * p.tile_steps();
+  fetch(tile);
+  for (int64_t turn = 0; tile >= first; tile -= p.tile_steps(), ++turn) {
     const bool all = __all(n == kBackSteps);
     if (!all) {
       mask<kBackSteps>(x, n, E::put(0.0f));
@@ -259,7 +272,7 @@ __global__ __launch_bounds__(kMaxWaves * myelin::kWave) void backward(Args a) {
     float h = start;
 #pragma unroll
     for (int i = 0; i < kBackSteps; ++i) {
-      const Gate g(E::get(gate[i]));
+      const Gate<E> g(E::get(gate[i]));
       ra[i] = g.a;
       rb[i] = g.b;
       const float v = E::get(x[i]);
@@ -269,89 +282,108 @@ __global__ __launch_bounds__(kMaxWaves * myelin::kWave) void backward(Args a) {
     }
 #pragma unroll
     for (int i = kBackSteps - 1; i >= 0; --i) m = {m.A * ra[i], ra[i] * (rg[i] + m.H)};
-    maps[turn & 1][wave][lane] = m;
-    const int64_t here = t0;
+    maps[turn & 1][p.wave][p.lane] = m;
     const int mine = n;
-    t0 -= tile_steps;
-    if (tile > first) {
-      n = steps_from<kBackSteps>(p, t0);
-      fetch();
-    }
+    if (tile > first) fetch(tile - p.tile_steps());
     __syncthreads();
     float c = s;
 #pragma unroll 4
-    for (int o = waves - 1; o >= 0; --o) {
-      if (o == wave) c = s;
-      const Affine q = maps[turn & 1][o][lane];
+    for (int o = p.waves - 1; o >= 0; --o) {
+      if (o == p.wave) c = s;
+      const Affine q = maps[turn & 1][o][p.lane];
       s = __builtin_fmaf(q.A, s, q.H);
     }
+    const int64_t here = p.step(tile);
+    const int left = p.in ? static_cast<int>(end - p.step(tile) < kBackSteps ? end - p.step(tile) : kBackSteps) : 0;
     T *gx = static_cast<T *>(a.gx) + here * BN + p.first, *gg = static_cast<T *>(a.gg) + here * BN + p.first;
 #pragma unroll
     for (int i = kBackSteps - 1; i >= 0; --i) {
       const float g = rg[i] + c, dx = rb[i] * g, dg = dx * rd[i] * ra[i];
       c = ra[i] * g;
       if (all) {
-        if (a.gx) (gx + i * BN)[lane] = E::put(dx);
-        if (a.gg) (gg + i * BN)[lane] = E::put(dg);
-      } else if (p.in && here + i < end) {
-        if (a.gx) (gx + i * BN)[lane] = E::put(i < mine ? dx : 0.0f);
-        if (a.gg) (gg + i * BN)[lane] = E::put(i < mine ? dg : 0.0f);
+        if (a.gx) (gx + i * BN)[p.lane] = E::put(dx);
+        if (a.gg) (gg + i * BN)[p.lane] = E::put(dg);
+      } else if (i < left) {
+        if (a.gx) (gx + i * BN)[p.lane] = E::put(i < mine ? dx : 0.0f);
+        if (a.gg) (gg + i * BN)[p.lane] = E::put(i < mine ? dg : 0.0f);
       }
     }
   }
-  if (p.in && wave == 0 && a.seg == 0 && a.state_out) a.state_out[p.c()] = s;
+  if (p.in && p.wave == 0 && a.seg == 0 && a.state_out) a.state_out[p.c()] = s;
 }
 
 // What a segment does to the state before it (BACK: to the gradient of the state
-// after it): each wave runs over a stretch of its own, then they are joined.
+// after it).  The waves take their steps of a tile as in the main pass and leave
+// what these do in LDS, for kTiles tiles at once.
+constexpr int kTiles = 4;
+
 template <class E, bool BACK>
-__global__ __launch_bounds__(kMaxWaves * myelin::kWave) void summarise(Args a) {
+__global__ __launch_bounds__(kMaxWaves * kWave) void summarise(Args a) {
   using T = typename E::T;
-  __shared__ Affine maps[kMaxWaves][myelin::kWave];
-  const int64_t block = locate(a);
-  if (BACK) ++a.seg;  // the first needs none, as the last forward
-  if (a.seg >= a.segments - !BACK) return;
-  const Place p = place_of<T>(a, block);
-  const int lane = p.lane, wave = p.wave, waves = p.waves;
+  constexpr int STEPS = BACK ? kBackSteps : kSteps;  // (16 do not fit the registers)
+  using P = Place<STEPS>;
+  __shared__ Affine maps[kTiles][kMaxWaves][kWave];
+  __shared__ Affine whole[kTiles][kWave];
+  const int64_t block = locate(a, a.segments - 1);
+  if (block < 0) return;  // the whole workgroup
+  if (BACK) ++a.seg;      // the first needs none, as the last forward
+  P p;
+  p.template set<T>(a, block);
   const int64_t first = a.seg * a.seg_steps;
   const int64_t end = first + a.seg_steps < a.T ? first + a.seg_steps : a.T;
-  // (whole chunks: a segment is a multiple of waves * kSteps steps)
-  const int64_t each = a.seg_steps / waves, from = first + wave * each;
-  const int64_t to = from + each < end ? from + each : end;
-  Affine m{1.0f, 0.0f};
-  const int chunks = to > from ? static_cast<int>((to - from + kSteps - 1) / kSteps) : 0;
-  for (int k = 0; k < chunks; ++k) {
-    const int64_t t0 = from + (BACK ? chunks - 1 - k : k) * kSteps;
-    const int n = steps_from<kSteps>(p, t0);
-    if (!__any(n > 0)) continue;
-    T v[kSteps], gate[kSteps];
-    load<kSteps>(gate, p.gate, p.at_gate, a.gt, t0, a.T);
+  const int tiles = static_cast<int>((end - first + p.tile_steps() - 1) / p.tile_steps());
+  T v[STEPS], gate[STEPS];
+  int n = 0;
+  const auto fetch = [&](int o) {
+    const int64_t tile = first + (BACK ? tiles - 1 - o : o) * p.tile_steps();
+    n = p.steps(tile);
+    if (!__any(n > 0)) return;
+    p.load(gate, p.gate, p.at_gate, a.gt, tile, a.T);
     if (!BACK)
-      load<kSteps>(v, p.x, p.at_x, a.xt, t0, a.T);
+      p.load(v, p.x, p.at_x, a.xt, tile, a.T);
     else if (a.g_out)
-      load<kSteps>(v, p.out, p.at_out, a.ot, t0, a.T);
-    if (!__all(n == kSteps)) mask<kSteps>(gate, n, E::put(kInf));
-    if (!__all(n == kSteps) || (BACK && !a.g_out)) mask<kSteps>(v, BACK && !a.g_out ? 0 : n, E::put(0.0f));
+      p.load(v, p.out, p.at_out, a.ot, tile, a.T);
+  };
+  fetch(0);
+  Affine all{1.0f, 0.0f};
+  for (int o = 0; o < tiles; ++o) {
+    if (!__all(n == STEPS)) mask<STEPS>(gate, n, E::put(kInf));
+    if (!__all(n == STEPS) || (BACK && !a.g_out)) mask<STEPS>(v, BACK && !a.g_out ? 0 : n, E::put(0.0f));
+    float ra[STEPS], ru[STEPS];
 #pragma unroll
-    for (int o = 0; o < kSteps; ++o) {
-      const int i = BACK ? kSteps - 1 - o : o;
-      const Gate g(E::get(gate[i]));
-      if (BACK)
-        m = {m.A * g.a, g.a * (E::get(v[i]) + m.H)};
-      else
-        m = {m.A * g.a, __builtin_fmaf(g.a, m.H, g.b * E::get(v[i]))};
+    for (int i = 0; i < STEPS; ++i) {
+      const Gate<E> g(E::get(gate[i]));
+      ra[i] = g.a;
+      ru[i] = BACK ? E::get(v[i]) : g.b * E::get(v[i]);
     }
-  }
-  maps[wave][lane] = m;
-  __syncthreads();
-  if (wave == 0 && p.in) {
-    m = {1.0f, 0.0f};
-    for (int o = 0; o < waves; ++o) {
-      const Affine q = maps[BACK ? waves - 1 - o : o][lane];
-      m = {m.A * q.A, __builtin_fmaf(q.A, m.H, q.H)};
+    if (o + 1 < tiles) fetch(o + 1);
+    Affine m{1.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+      const int i = BACK ? STEPS - 1 - k : k;
+      m = {m.A * ra[i], BACK ? ra[i] * (ru[i] + m.H) : __builtin_fmaf(ra[i], m.H, ru[i])};
     }
-    a.joins[a.seg * a.B * a.N + p.c()] = m;
+    const int slot = o % kTiles;
+    maps[slot][p.wave][p.lane] = m;
+    if (slot + 1 < kTiles && o + 1 < tiles) continue;
+    __syncthreads();
+    // a wave to a tile, then the first one over the tiles
+    for (int t = p.wave; t <= slot; t += p.waves) {
+      m = {1.0f, 0.0f};
+      for (int g = 0; g < p.waves; ++g) {
+        const Affine q = maps[t][BACK ? p.waves - 1 - g : g][p.lane];
+        m = {m.A * q.A, __builtin_fmaf(q.A, m.H, q.H)};
+      }
+      whole[t][p.lane] = m;
+    }
+    __syncthreads();
+    if (p.wave == 0)
+      for (int t = 0; t <= slot; ++t) {
+        const Affine q = whole[t][p.lane];
+        all = {all.A * q.A, __builtin_fmaf(q.A, all.H, q.H)};
+      }
   }
+  if (p.wave == 0 && p.in) a.joins[a.seg * a.B * a.N + p.c()] = all;
 }
 
 template <class E>
@@ -360,7 +392,7 @@ __global__ __launch_bounds__(256) void step(Args a) {
   const int64_t c = myelin::block_id() * 256 + threadIdx.x;
   if (c >= a.B * a.N) return;
   const int64_t b = c / a.N, n = c - b * a.N;
-  const Gate g(E::get(static_cast<const T *>(a.gate)[b * a.gb + n]));
+  const Gate<E> g(E::get(static_cast<const T *>(a.gate)[b * a.gb + n]));
   const float h = __builtin_fmaf(g.a, a.state[c], g.b * E::get(static_cast<const T *>(a.x)[b * a.xb + n]));
   a.state_out[c] = h;
   static_cast<T *>(a.out)[c] = E::put(h);
@@ -368,13 +400,13 @@ __global__ __launch_bounds__(256) void step(Args a) {
 
 // A workgroup's lanes reach over this many batch rows; their offsets have 32 bits.
 bool reachable(int64_t stride, int64_t B, int64_t N) {
-  return B == 1 || (stride < int64_t{1} << 30 && (64 / N + 1) * stride + N < int64_t{1} << 30);
+  return B == 1 || (stride < int64_t{1} << 29 && (64 / N + 1) * stride + N < int64_t{1} << 29);
 }
 
 int check(const char *what, int dtype, int64_t T, int64_t B, int64_t N) {
   if (dtype != 0 && dtype != 2) return myelin::invalid("%s: unsupported dtype %d", what, dtype);
   if (T < 1 || B < 0 || N < 0) return myelin::invalid("%s: T must be positive, B and N not negative", what);
-  if (T >= int64_t{1} << 31 || B >= int64_t{1} << 31 || N >= int64_t{1} << 29 || B * N >= int64_t{1} << 36)
+  if (T >= int64_t{1} << 31 || B >= int64_t{1} << 31 || N >= int64_t{1} << 28 || B * N >= int64_t{1} << 36)
     return myelin::invalid("%s: too many steps or channels", what);
   return MYELIN_OK;
 }
@@ -384,37 +416,33 @@ struct Plan {
   int waves;
 };
 
-// Time is split where the channels leave CUs without a workgroup.
-Plan plan_of(int64_t T, int64_t B, int64_t N, bool back) {
+// Time is split where the channels leave half of the CUs without a workgroup.
+Plan plan_of(int64_t T, int64_t B, int64_t N) {
   Plan p;
-  p.blocks = (B * N + myelin::kWave - 1) / myelin::kWave;
-  // (segments are whole chunks of kSteps to each wave for summarise)
-  const int64_t chunks = (T + kSteps - 1) / kSteps;
-  p.waves = static_cast<int>(chunks < kMaxWaves ? chunks : kMaxWaves);
+  p.blocks = (B * N + kWave - 1) / kWave;
+  const int64_t needed = (T + kSteps - 1) / kSteps;
+  p.waves = static_cast<int>(needed < kMaxWaves ? needed : kMaxWaves);
   const int64_t tile = p.waves * kSteps, tiles = (T + tile - 1) / tile;
-  (void)back;
   int64_t n = p.blocks >= 128 ? 1 : 256 / p.blocks;
   if (n > tiles) n = tiles;
-  const int64_t each = (tiles + n - 1) / n;
-  p.seg_steps = each * tile;
-  p.segments = (tiles + each - 1) / each;
+  const int64_t some = (tiles + n - 1) / n;
+  p.seg_steps = some * tile;
+  p.segments = (tiles + some - 1) / some;
   return p;
 }
 
 // Workgroups of up to 1024 threads, fewer than 2^32 in x.
 dim3 grid_for(int64_t blocks) {
+  blocks = (blocks + 7) / 8 * 8;  // as many to each XCD
   const int64_t x = int64_t{1} << 21, y = (blocks + x - 1) / x;
   return dim3(static_cast<unsigned>(y > 1 ? x : blocks), static_cast<unsigned>(y));
 }
 
-int64_t workspace_of(int64_t T, int64_t B, int64_t N, bool back) {
-  const Plan p = plan_of(T, B, N, back);
-  return p.segments == 1 ? 0 : 2 * p.segments * B * N;
-}
+int64_t workspace_of(const Plan &p, int64_t B, int64_t N) { return p.segments == 1 ? 0 : 2 * p.segments * B * N; }
 
-int prepare(const char *what, Args &a, Plan &p, float *workspace, int64_t elems, bool back) {
-  p = plan_of(a.T, a.B, a.N, back);
-  const int64_t need = workspace_of(a.T, a.B, a.N, back);
+int prepare(const char *what, Args &a, Plan &p, float *workspace, int64_t elems) {
+  p = plan_of(a.T, a.B, a.N);
+  const int64_t need = workspace_of(p, a.B, a.N);
   if (need) {
     if (!workspace || elems < need)
       return myelin::invalid("%s: workspace of %lld floats needed", what, static_cast<long long>(need));
@@ -429,7 +457,7 @@ int prepare(const char *what, Args &a, Plan &p, float *workspace, int64_t elems,
 
 template <class E, bool BACK>
 void launch(const Args &a, const Plan &p, hipStream_t s) {
-  const int threads = p.waves * myelin::kWave;
+  const int threads = p.waves * kWave;
   if (p.segments > 1) summarise<E, BACK><<<grid_for(p.blocks * (p.segments - 1)), threads, 0, s>>>(a);
   if (BACK)
     backward<E><<<grid_for(p.blocks * p.segments), threads, 0, s>>>(a);
@@ -445,7 +473,9 @@ extern "C" int64_t myelin_gated_recurrence_kept_elems(int64_t T, int64_t B, int6
 
 extern "C" int64_t myelin_gated_recurrence_workspace_elems(int dtype, int64_t T, int64_t B, int64_t N, int backward) {
   (void)dtype;
-  return T < 1 || B < 1 || N < 1 ? 0 : workspace_of(T, B, N, backward);
+  (void)backward;
+  if (T < 1 || B < 1 || N < 1) return 0;
+  return workspace_of(plan_of(T, B, N), B, N);
 }
 
 extern "C" int myelin_gated_recurrence_fwd(const void *x, const void *gate, int dtype, const int64_t *strides,
@@ -461,7 +491,7 @@ extern "C" int myelin_gated_recurrence_fwd(const void *x, const void *gate, int 
   Args a{};
   a.T = T, a.B = B, a.N = N;
   Plan p;
-  if (int rc = prepare(what, a, p, workspace, workspace_elems, false)) return rc;
+  if (int rc = prepare(what, a, p, workspace, workspace_elems)) return rc;
   a.x = x, a.gate = gate, a.lengths = lengths, a.state = state;
   a.xt = strides[0], a.xb = strides[1], a.gt = strides[2], a.gb = strides[3];
   a.out = out, a.state_out = state_out, a.kept = kept;
@@ -486,7 +516,7 @@ extern "C" int myelin_gated_recurrence_bwd(const void *x, const void *gate, cons
   Args a{};
   a.T = T, a.B = B, a.N = N;
   Plan p;
-  if (int rc = prepare(what, a, p, workspace, workspace_elems, true)) return rc;
+  if (int rc = prepare(what, a, p, workspace, workspace_elems)) return rc;
   a.x = x, a.gate = gate, a.g_out = grad_out, a.lengths = lengths, a.state = grad_state_out;
   a.xt = strides[0], a.xb = strides[1], a.gt = strides[2], a.gb = strides[3], a.ot = strides[4], a.ob = strides[5];
   a.gx = grad_x, a.gg = grad_gate, a.state_out = grad_state, a.kept = const_cast<float *>(kept);

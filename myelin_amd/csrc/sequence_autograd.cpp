@@ -328,7 +328,7 @@ Tensor recurrence_workspace(const Tensor &x, int backward, int64_t *elems) {
 // unit stride in the last dimension, and batch rows near enough for the kernels
 Tensor recurrence_rows(const Tensor &t) {
   const int64_t B = t.size(-2), N = t.size(-1);
-  const bool near = B <= 1 || N == 0 || (64 / N + 1) * t.stride(-2) + N < int64_t{1} << 30;
+  const bool near = B <= 1 || N == 0 || (64 / N + 1) * t.stride(-2) + N < int64_t{1} << 29;
   return near ? unit_stride(t) : t.contiguous();
 }
 

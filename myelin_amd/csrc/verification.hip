@@ -29,7 +29,7 @@ struct Args {
   const float *uniforms;  // [n + 1, B]
   const int32_t *lengths;
   int64_t *accepted, *out;
-  int64_t n, B, V;
+  int64_t n, B, V, pieces;
 };
 
 // How many tokens of a sequence are taken, by one wave.
@@ -90,55 +90,52 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-// What each part of a row holds: the sum of w, and that of p alone.
+// A row in pieces of 1024 tokens, a wave each: what a piece's weights add up to, and
+// what p alone does.
+constexpr int kEach = 16, kPiece = kEach * kWave;
+
 struct Sums {
   double rest, all;
 };
 
-// Tiles of a part: enough workgroups to fill the chip where sequences are few.
-constexpr int kPer = 16, kTile = kThreads * kPer, kMaxParts = 512;
-
-void split(int64_t B, int64_t V, int64_t *parts, int64_t *part) {
-  const int64_t tiles = (V + kTile - 1) / kTile;
-  int64_t n = B > 0 ? 1024 / B : 1;
-  n = n < 1 ? 1 : n > kMaxParts ? kMaxParts : n;
-  if (n > tiles) n = tiles;
-  const int64_t per = (tiles + n - 1) / n;
-  *part = per * kTile;
-  *parts = (tiles + per - 1) / per;
-}
-
-// A workgroup to a part of a sequence's row: each finds out by itself how many
-// tokens are taken, so that none waits for another.
+// Each wave finds out by itself how many tokens are taken, so that none waits for
+// another.
 template <class E>
-__global__ __launch_bounds__(kThreads) void sum_parts(Args a, int parts, int64_t part, Sums *sums) {
-  __shared__ Sums red[kWaves];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid >> 6;
-  const int64_t b = blockIdx.x / parts, at = blockIdx.x % parts;
+__global__ __launch_bounds__(kThreads) void sum_pieces(Args a, Sums *sums) {
+  using T = typename E::T;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int64_t unit = myelin::block_id() * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t b = unit / a.pieces, piece = unit - b * a.pieces;
+  if (b >= a.B) return;  // the whole wave
   const int64_t drafted = drafted_of(a, b), accepted = taken<E>(a, b, drafted, lane);
-  const bool refused = accepted < drafted;
-  const Weights<E> w = weights_of<E>(a, b, accepted, refused);
-  const int64_t begin = at * part, end = begin + part < a.V ? begin + part : a.V;
+  const Weights<E> w = weights_of<E>(a, b, accepted, accepted < drafted);
+  if (piece == 0) {
+    for (int64_t i = lane; i <= a.n; i += kWave)
+      if (i != accepted) a.out[i * a.B + b] = i < accepted ? a.tokens[i * a.B + b] : -1;
+    if (lane == 0) a.accepted[b] = accepted;
+  }
+  // (loads under conditions wait for each other: past the end it is the last token's)
+  const int64_t at = piece * kPiece + lane;
+  T p[kEach], q[kEach];
+#pragma unroll
+  for (int o = 0; o < kEach; ++o) p[o] = w.p[at + o * kWave < a.V ? at + o * kWave : a.V - 1];
+  if (w.q) {
+#pragma unroll
+    for (int o = 0; o < kEach; ++o) q[o] = w.q[at + o * kWave < a.V ? at + o * kWave : a.V - 1];
+  }
   Sums s{0.0, 0.0};
-  for (int64_t i = begin + tid; i < end; i += kThreads) {
-    s.rest += w(i);
-    s.all += w.of_p(i);
+#pragma unroll
+  for (int o = 0; o < kEach; ++o) {
+    const bool in = at + o * kWave < a.V;
+    const double v = E::get(p[o]);
+    s.all += in ? positive(v) : 0.0;
+    if (w.q)
+      s.rest += in ? positive(v - static_cast<double>(E::get(q[o]))) : 0.0;
+    else
+      s.rest += in && at + o * kWave != w.without ? positive(v) : 0.0;
   }
   s = {wave_sum(s.rest), wave_sum(s.all)};
-  if (lane == 0) red[wave] = s;
-  if (at == 0) {
-    for (int64_t i = tid; i <= a.n; i += kThreads)
-      if (i != accepted) a.out[i * a.B + b] = i < accepted ? a.tokens[i * a.B + b] : -1;
-    if (tid == 0) a.accepted[b] = accepted;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    for (int o = 1; o < kWaves; ++o) {
-      s.rest += red[o].rest;
-      s.all += red[o].all;
-    }
-    sums[blockIdx.x] = s;
-  }
+  if (lane == 0) sums[unit] = s;
 }
 
 // The sum of v over the threads before this one, and over all.
@@ -162,93 +159,121 @@ __device__ __forceinline__ double before(double v, double *red, double *total) {
   return base + (lane ? up : 0.0);
 }
 
-// A workgroup to a sequence: the part of its row that the draw falls into, then
-// the token.  Sums in another order than the parts' may differ in their last bits:
-// a draw that is not found in its part is looked for in the next ones, and the last
+// Of values that grow from thread to thread: the smallest and the largest of the
+// workgroup's, by one atomic of each wave.
+__device__ __forceinline__ void take_first(unsigned long long *to, unsigned long long v, bool have) {
+  const uint64_t m = __ballot(have);
+  if (m && (threadIdx.x & (kWave - 1)) == __builtin_ctzll(m)) atomicMin(to, v);
+}
+__device__ __forceinline__ void take_last(long long *to, long long v, bool have) {
+  const uint64_t m = __ballot(have);
+  if (m && (threadIdx.x & (kWave - 1)) == 63 - __builtin_clzll(m)) atomicMax(to, v);
+}
+
+// A workgroup to a sequence: the piece of its row that the draw falls into, then the
+// token.  Sums in another order than the pieces' may differ in their last bits: a
+// draw that is not found in its piece is looked for in the next ones, and the last
 // token with a weight takes what is left.
 template <class E>
-__global__ __launch_bounds__(kThreads) void locate(Args a, int parts, int64_t part, const Sums *sums) {
+__global__ __launch_bounds__(kThreads) void locate(Args a, const Sums *sums) {
+  constexpr int FEW = kPiece / kThreads;
   __shared__ double red[kWaves];
-  __shared__ int first, last;
+  __shared__ unsigned long long first, found;
+  __shared__ long long last, some;
   __shared__ double run_at;
-  __shared__ int64_t found, some;
   const int tid = threadIdx.x;
   const int64_t b = blockIdx.x, accepted = a.accepted[b];
-  const bool refused = accepted < drafted_of(a, b);
-  Weights<E> w = weights_of<E>(a, b, accepted, refused);
-  sums += b * parts;
-  // each thread two parts
-  double s[2], total, ignored;
-  for (int o = 0; o < 2; ++o) s[o] = 2 * tid + o < parts ? sums[2 * tid + o].rest : 0.0;
-  double base = before(s[0] + s[1], red, &total);
-  if (!(total > 0.0)) {
+  Weights<E> w = weights_of<E>(a, b, accepted, accepted < drafted_of(a, b));
+  sums += b * a.pieces;
+  // each thread has some pieces in a row
+  const int64_t each = (a.pieces + kThreads - 1) / kThreads, from = tid * each;
+  const int64_t to = from + each < a.pieces ? from + each : a.pieces;
+  const double u = a.uniforms[a.n * a.B + b];
+  const Sums own = from < to ? sums[from] : Sums{0.0, 0.0};  // (all there are below 2^18 tokens)
+  double rest = own.rest, all = own.all, total, ignored;
+  for (int64_t o = from + 1; o < to; ++o) {
+    rest += sums[o].rest;
+    all += sums[o].all;
+  }
+  double base = before(rest, red, &total);
+  const bool refilled = !(total > 0.0);
+  if (refilled) {
     w.q = nullptr;
     w.without = -1;
-    for (int o = 0; o < 2; ++o) s[o] = 2 * tid + o < parts ? sums[2 * tid + o].all : 0.0;
-    base = before(s[0] + s[1], red, &total);
+    base = before(all, red, &total);
   }
   if (!(total > 0.0)) {
     if (tid == 0) a.out[accepted * a.B + b] = -1;
-    return;
+    return;  // the whole workgroup
   }
-  const double bound = static_cast<double>(a.uniforms[a.n * a.B + b]) * total;
+  const double bound = u * total;
   if (tid == 0) {
-    first = kMaxParts;
-    last = 0;
-    found = a.V;
-    some = -1;
+    first = found = ~0ull;
+    last = some = -1;
   }
   __syncthreads();
-  const double from_here[2] = {base, base + s[0]};
-  for (int o = 0; o < 2; ++o)
-    if (s[o] > 0.0) {
-      atomicMax(&last, 2 * tid + o);
-      if (from_here[o] + s[o] > bound) atomicMin(&first, 2 * tid + o);
-    }
-  __syncthreads();
-  const int from = first < kMaxParts ? first : last;
-  for (int o = 0; o < 2; ++o)
-    if (2 * tid + o == from) run_at = from_here[o];
-  __syncthreads();
-  double run = run_at;
-  for (int64_t at = from * part; at < a.V; at += kTile) {
-    const int64_t mine = at + tid * kPer;
-    double v[kPer], sum = 0.0;
-    for (int o = 0; o < kPer; ++o) {
-      v[o] = mine + o < a.V ? w(mine + o) : 0.0;
-      sum += v[o];
-    }
-    double here = run + before(sum, red, &ignored);
-    int64_t hit = a.V, kept = -1;
-    for (int o = 0; o < kPer; ++o) {
-      here += v[o];
-      if (v[o] > 0.0) {
-        kept = mine + o;
-        if (hit == a.V && here > bound) hit = mine + o;
+  long long mine = -1;
+  unsigned long long hit = ~0ull;
+  double run = base, at_hit = 0.0, at_last = 0.0;
+  for (int64_t o = from; o < to; ++o) {
+    const Sums here = o == from ? own : sums[o];
+    const double v = refilled ? here.all : here.rest;
+    if (v > 0.0) {
+      mine = o;
+      at_last = run;
+      if (hit == ~0ull && run + v > bound) {
+        hit = static_cast<unsigned long long>(o);
+        at_hit = run;
       }
     }
-    if (hit < a.V) atomicMin(reinterpret_cast<unsigned long long *>(&found), static_cast<unsigned long long>(hit));
-    if (kept >= 0) atomicMax(reinterpret_cast<long long *>(&some), static_cast<long long>(kept));
+    run += v;
+  }
+  take_first(&first, hit, hit != ~0ull);
+  take_last(&last, mine, mine >= 0);
+  __syncthreads();
+  const int64_t start = first != ~0ull ? static_cast<int64_t>(first) : last;
+  if (start >= from && start < to) run_at = first != ~0ull ? at_hit : at_last;
+  __syncthreads();
+  run = run_at;
+  for (int64_t at = start * kPiece; at < a.V; at += kPiece) {
+    double v[FEW], sum = 0.0;
+    const int64_t here = at + tid * FEW;
+#pragma unroll
+    for (int o = 0; o < FEW; ++o) {
+      const double weight = w(here + o < a.V ? here + o : a.V - 1);
+      v[o] = here + o < a.V ? weight : 0.0;
+      sum += v[o];
+    }
+    double upto = run + before(sum, red, &ignored);
+    unsigned long long at_bound = ~0ull;
+    long long kept = -1;
+#pragma unroll
+    for (int o = 0; o < FEW; ++o) {
+      upto += v[o];
+      if (v[o] > 0.0) {
+        kept = here + o;
+        if (at_bound == ~0ull && upto > bound) at_bound = static_cast<unsigned long long>(here + o);
+      }
+    }
+    take_first(&found, at_bound, at_bound != ~0ull);
+    take_last(&some, kept, kept >= 0);
     __syncthreads();
-    if (found < a.V) break;  // (the same for all threads)
+    if (found != ~0ull) break;  // (the same for all threads)
     run += ignored;
   }
-  if (tid == 0) a.out[accepted * a.B + b] = found < a.V ? found : some;
+  if (tid == 0) a.out[accepted * a.B + b] = found != ~0ull ? static_cast<int64_t>(found) : some;
 }
 
 template <class E>
-void launch(const Args &a, int64_t parts, int64_t part, Sums *sums, hipStream_t s) {
-  sum_parts<E><<<static_cast<unsigned>(a.B * parts), kThreads, 0, s>>>(a, static_cast<int>(parts), part, sums);
-  locate<E><<<static_cast<unsigned>(a.B), kThreads, 0, s>>>(a, static_cast<int>(parts), part, sums);
+void launch(const Args &a, Sums *sums, hipStream_t s) {
+  sum_pieces<E><<<myelin::grid_of((a.B * a.pieces + kWaves - 1) / kWaves), kThreads, 0, s>>>(a, sums);
+  locate<E><<<static_cast<unsigned>(a.B), kThreads, 0, s>>>(a, sums);
 }
 
 }  // namespace
 
 extern "C" int64_t myelin_verify_draft_workspace_bytes(int64_t B, int64_t V) {
-  if (B < 1 || V < 1) return 0;
-  int64_t parts, part;
-  split(B, V, &parts, &part);
-  return B * parts * static_cast<int64_t>(sizeof(Sums));
+  return B < 1 || V < 1 ? 0 : B * ((V + kPiece - 1) / kPiece) * static_cast<int64_t>(sizeof(Sums));
 }
 
 extern "C" int myelin_verify_draft(const void *target, const void *draft, int dtype, const int64_t *strides,
@@ -263,17 +288,15 @@ extern "C" int myelin_verify_draft(const void *target, const void *draft, int dt
   if (B == 0) return MYELIN_OK;
   if (!target || !strides || !uniforms || !accepted || !out_tokens || (n > 0 && !tokens))
     return myelin::invalid("%s: null pointer", what);
-  int64_t parts, part;
-  split(B, V, &parts, &part);
   const int64_t need = myelin_verify_draft_workspace_bytes(B, V);
   if (!workspace || workspace_bytes < need)
     return myelin::invalid("%s: workspace of %lld bytes needed", what, static_cast<long long>(need));
   if (!myelin::aligned(workspace, 16)) return myelin::invalid("%s: workspace must be 16-byte aligned", what);
   Args a{target, draft, strides[0], strides[1], draft ? strides[2] : 0, draft ? strides[3] : 0, tokens, uniforms,
-         lengths, accepted, out_tokens, n, B, V};
+         lengths, accepted, out_tokens, n, B, V, (V + kPiece - 1) / kPiece};
   if (dtype == 0)
-    launch<F32>(a, parts, part, static_cast<Sums *>(workspace), myelin::as_hip(stream));
+    launch<F32>(a, static_cast<Sums *>(workspace), myelin::as_hip(stream));
   else
-    launch<BF16>(a, parts, part, static_cast<Sums *>(workspace), myelin::as_hip(stream));
+    launch<BF16>(a, static_cast<Sums *>(workspace), myelin::as_hip(stream));
   return myelin::launched(what);
 }

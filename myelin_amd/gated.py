@@ -37,7 +37,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     a workgroup's 32-bit offsets."""
 
     B, N = t.shape[-2:]
-    near = B <= 1 or N == 0 or (64 // N + 1) * t.stride(-2) + N < 2**30
+    near = B <= 1 or N == 0 or (64 // N + 1) * t.stride(-2) + N < 2**29
     return t if near and (t.stride(-1) == 1 or N == 1) else t.contiguous()
 
 
