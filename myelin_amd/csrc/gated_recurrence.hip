@@ -42,16 +42,23 @@ struct Args {
 
 // sigmoid and 1 - sigmoid, each to its own accuracy.  fp32 puts the rounding of the
 // exponential's argument back, |g| 2^-24 of the smaller of the two.  A bf16 gate is
-// itself only known to |g| 2^-9.
+// itself only known to |g| 2^-9: it does without that, and bounds the exponential of
+// -g, keeping NaN (below -86.6 a stays at 2^-125), in place of a choice by its sign;
+// [2048, 8, 1500] bf16: backward 80 -> 75 us.
 template <class E>
 struct Gate {
   float a, b;
   __device__ explicit Gate(float g) {
-    const float d = -__builtin_fabsf(g);
-    const float e = sizeof(typename E::T) == 4 ? myelin::exp_f32(d) : __builtin_amdgcn_exp2f(d * myelin::kLog2e);
-    const float r = __builtin_amdgcn_rcpf(1.0f + e), s = e * r;
-    a = g >= 0.0f ? r : s;
-    b = g >= 0.0f ? s : r;
+    if constexpr (sizeof(typename E::T) == 2) {
+      const float e = __builtin_elementwise_minimum(__builtin_amdgcn_exp2f(g * -myelin::kLog2e), 0x1p125f);
+      a = __builtin_amdgcn_rcpf(1.0f + e);
+      b = e * a;
+    } else {
+      const float e = myelin::exp_f32(-__builtin_fabsf(g));
+      const float r = __builtin_amdgcn_rcpf(1.0f + e), s = e * r;
+      a = g >= 0.0f ? r : s;
+      b = g >= 0.0f ? s : r;
+    }
   }
 };
 
@@ -416,14 +423,16 @@ struct Plan {
   int waves;
 };
 
-// Time is split where the channels leave half of the CUs without a workgroup.
+// Time is split where the channels leave half of the CUs without a workgroup: 128
+// blocks in two segments, [8192, 4, 2048] bf16: forward 142 us either way, backward
+// 276 -> 210; 175 blocks are faster whole (70 and 140 us, against 101 and 172).
 Plan plan_of(int64_t T, int64_t B, int64_t N) {
   Plan p;
   p.blocks = (B * N + kWave - 1) / kWave;
   const int64_t needed = (T + kSteps - 1) / kSteps;
   p.waves = static_cast<int>(needed < kMaxWaves ? needed : kMaxWaves);
   const int64_t tile = p.waves * kSteps, tiles = (T + tile - 1) / tile;
-  int64_t n = p.blocks >= 128 ? 1 : 256 / p.blocks;
+  int64_t n = p.blocks > 128 ? 1 : 256 / p.blocks;
   if (n > tiles) n = tiles;
   const int64_t some = (tiles + n - 1) / n;
   p.seg_steps = some * tile;

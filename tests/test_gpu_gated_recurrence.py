@@ -5,10 +5,11 @@ Tolerances are majorants of fp32's errors, formed beside the reference.  With e 
 2^-24: a gate's two values carry at most 8 e (the exponential within 2 units in the
 last place, one sum, one quotient, one product), and each step adds its own
 roundings and, where steps are joined in another order, those of the products of
-decays: C e = 16 e of the sum of absolute terms, carried on as the state is.  An
-exponential below the least normal number is 0, so that a gate's smaller value is
-within TINY = 2^-126 besides, times what it multiplies.  A result in bfloat16 adds
-half a unit in its last place.
+decays: BASE = 16 e of the sum of absolute terms, carried on as the state is.  The
+kernels of bfloat16 leave the rounding of the exponential's argument, |gate| e more.
+An exponential below the least normal number is 0, or bounded at 2^-125, so that a
+gate's smaller value is within TINY = 2^-125 besides, times what it multiplies.  A
+result in bfloat16 adds half a unit in its last place.
 """
 
 from __future__ import annotations
@@ -23,8 +24,8 @@ import myelin_amd as myelin
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16}
-C = 16 * 2.0**-24
-TINY = 2.0**-126
+BASE = 16 * 2.0**-24
+TINY = 2.0**-125
 
 
 def _case(**kw):
@@ -38,8 +39,10 @@ def _half(dt):
 def _reference(x, gate, state, lengths, g_out=None, g_state=None):
     """Values and, beside each, the bound of its fp32 error."""
 
+    C = BASE if x.dtype == torch.float32 else BASE + gate.detach().double().cpu().abs().clamp(max=200.0) * 2.0**-24
     x, gate = x.detach().double().cpu(), gate.detach().double().cpu()
     T, B, N = x.shape
+    C = torch.as_tensor(C, dtype=torch.float64).expand(T, B, N)
     live = torch.full((B, 1), T) if lengths is None else lengths.cpu().long().clamp(0, T)[:, None]
     a, b = torch.sigmoid(gate), torch.sigmoid(-gate)
     on = torch.arange(T)[:, None, None] < live
@@ -54,7 +57,7 @@ def _reference(x, gate, state, lengths, g_out=None, g_state=None):
         h = a[t] * h + b[t] * x[t]
         tiny = TINY * (size + x[t].abs())
         size = a[t] * size + b[t] * x[t].abs()
-        err = a[t] * err + torch.where(on[t], C * size + tiny, 0.0)
+        err = a[t] * err + torch.where(on[t], C[t] * size + tiny, 0.0)
         hs.append(h)
         errs.append(err)
     out = torch.where(on, torch.stack(hs), 0.0)
@@ -68,14 +71,14 @@ def _reference(x, gate, state, lengths, g_out=None, g_state=None):
     gx, gg, ex, eg = ([None] * T for _ in range(4))
     for t in range(T - 1, -1, -1):
         g, size = g + go[t], size + go[t].abs()
-        err = err + torch.where(on[t], C * size + TINY * size, 0.0)
+        err = err + torch.where(on[t], C[t] * size + TINY * size, 0.0)
         d, dsize = before[t] - x[t], sizes[t] + x[t].abs()
-        gx[t], ex[t] = b[t] * g, b[t] * (err + C * size) + TINY * size
+        gx[t], ex[t] = b[t] * g, b[t] * (err + C[t] * size) + TINY * size
         gg[t] = b[t] * a[t] * g * d
-        eg[t] = b[t] * a[t] * (err * dsize + size * (errs_before[t] + C * dsize)) + TINY * size * dsize
+        eg[t] = b[t] * a[t] * (err * dsize + size * (errs_before[t] + C[t] * dsize)) + TINY * size * dsize
         g, size, err = a[t] * g, a[t] * size, a[t] * err
     r["x"], r["gate"] = (torch.stack(gx), torch.stack(ex)), (torch.stack(gg), torch.stack(eg))
-    r["initial"] = (g, err + C * size)
+    r["initial"] = (g, err + C[0] * size)
     return r
 
 
