@@ -40,25 +40,20 @@ struct Args {
   Affine *joins;                             // [segments, B, N]
 };
 
-// sigmoid and 1 - sigmoid, each to its own accuracy.  fp32 puts the rounding of the
-// exponential's argument back, |g| 2^-24 of the smaller of the two.  A bf16 gate is
-// itself only known to |g| 2^-9: it does without that, and bounds the exponential of
-// -g, keeping NaN (below -86.6 a stays at 2^-125), in place of a choice by its sign;
-// [2048, 8, 1500] bf16: backward 80 -> 75 us.
+// sigmoid and 1 - sigmoid, each to its own accuracy: the smaller of the two from the
+// exponential, the larger as what it leaves of 1 (a time constant of 1000 steps adds
+// up a thousand of its roundings; a reciprocal's would be twice as large).  fp32 puts
+// the rounding of the exponential's argument back, |g| 2^-24 of the smaller.  A bf16
+// gate is itself only known to |g| 2^-9.
 template <class E>
 struct Gate {
   float a, b;
   __device__ explicit Gate(float g) {
-    if constexpr (sizeof(typename E::T) == 2) {
-      const float e = __builtin_elementwise_minimum(__builtin_amdgcn_exp2f(g * -myelin::kLog2e), 0x1p125f);
-      a = __builtin_amdgcn_rcpf(1.0f + e);
-      b = e * a;
-    } else {
-      const float e = myelin::exp_f32(-__builtin_fabsf(g));
-      const float r = __builtin_amdgcn_rcpf(1.0f + e), s = e * r;
-      a = g >= 0.0f ? r : s;
-      b = g >= 0.0f ? s : r;
-    }
+    const float d = -__builtin_fabsf(g);
+    const float e = sizeof(typename E::T) == 4 ? myelin::exp_f32(d) : __builtin_amdgcn_exp2f(d * myelin::kLog2e);
+    const float s = e * __builtin_amdgcn_rcpf(1.0f + e), r = 1.0f - s;
+    a = g >= 0.0f ? r : s;
+    b = g >= 0.0f ? s : r;
   }
 };
 

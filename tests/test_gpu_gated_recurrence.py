@@ -3,13 +3,13 @@ one step after the other.
 
 Tolerances are majorants of fp32's errors, formed beside the reference.  With e =
 2^-24: a gate's two values carry at most 8 e (the exponential within 2 units in the
-last place, one sum, one quotient, one product), and each step adds its own
+last place, one sum, a reciprocal within 1, one product, one difference), and each step adds its own
 roundings and, where steps are joined in another order, those of the products of
 decays: BASE = 16 e of the sum of absolute terms, carried on as the state is.  The
 kernels of bfloat16 leave the rounding of the exponential's argument, |gate| e more.
-An exponential below the least normal number is 0, or bounded at 2^-125, so that a
-gate's smaller value is within TINY = 2^-125 besides, times what it multiplies.  A
-result in bfloat16 adds half a unit in its last place.
+An exponential below the least normal number is 0, so that a gate's smaller value is
+within TINY = 2^-126 besides, times what it multiplies.  A result in bfloat16 adds
+half a unit in its last place.
 """
 
 from __future__ import annotations
@@ -25,7 +25,7 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16}
 BASE = 16 * 2.0**-24
-TINY = 2.0**-125
+TINY = 2.0**-126
 
 
 def _case(**kw):
