@@ -140,8 +140,9 @@ __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int 
   float loss = 0.0f;
   for (int k = lane; k < a.K; k += kWave) {
     const int64_t token = a.tokens[first + k];
+    const bool there = !empty(token, a.values[first + k]);
     float p = 0.0f;
-    if (!empty(token, a.values[first + k])) {
+    if (there) {
       const float d = (a.values[first + k] - peak) * a.rate;
       p = myelin::exp_f32(d) / total;
       if (p != 0.0f && !bad) {
@@ -150,8 +151,8 @@ __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int 
         loss += p * ((d - log_total) - log_q);
       }
     }
-    if (a.probs && twice && p != 0.0f) {
-      // put together, in the places' order, at the first
+    if (a.probs && twice && there) {
+      // put together, in the places' order, at the first (whose own may be 0)
       float sum = 0.0f;
       bool mine = true;
       for (int o = 0; o < a.K; ++o)

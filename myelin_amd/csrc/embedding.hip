@@ -571,6 +571,17 @@ __global__ __launch_bounds__(kFewThreads) void sum_few(Args a, int per) {
     r.template store<false>(static_cast<T *>(a.to) + v * a.D + u * VEC, a.scale);
 }
 
+// no tokens at all
+template <class E, int VEC>
+__global__ __launch_bounds__(kThreads) void zeros(Args a) {
+  using T = typename E::T;
+  const int64_t i = (myelin::block_id() * kThreads + threadIdx.x) * VEC;
+  if (i >= a.V * a.D) return;
+  Vector<E, VEC> r;
+  r.zero();
+  r.template store<false>(static_cast<T *>(a.to) + i, 1.0f);
+}
+
 // ---- launches ---------------------------------------------------------------
 struct Layout {  // of the workspace, in bytes
   bool few, one;
@@ -632,6 +643,10 @@ void launch_lookup(Args &a, hipStream_t s) {
 template <class E, int VEC>
 void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
   a.units = a.D / VEC;
+  if (a.M == 0) {
+    zeros<E, VEC><<<myelin::grid_of((a.V * a.units + kThreads - 1) / kThreads), kThreads, 0, s>>>(a);
+    return;
+  }
   if (l.few) {
     const int per = threads_of(a.units, kWave);
     a.slices = (a.units + per - 1) / per;
@@ -730,7 +745,7 @@ extern "C" int myelin_token_embedding_bwd(const int64_t *tokens, const void *gra
   const char *what = "token_embedding_bwd";
   if (int rc = check(what, dtype, M, V, D, scale)) return rc;
   if (!grad_weight || (M > 0 && (!tokens || !grad_out))) return myelin::invalid("%s: null pointer", what);
-  Layout l = layout_of(M, V, D);
+  const Layout l = layout_of(M, V, D);
   if (l.size) {
     if (!workspace || workspace_bytes < l.size)
       return myelin::invalid("%s: workspace of %lld bytes needed", what, static_cast<long long>(l.size));
@@ -739,7 +754,6 @@ extern "C" int myelin_token_embedding_bwd(const int64_t *tokens, const void *gra
   Args a{};
   a.tokens = tokens, a.from = grad_out, a.to = grad_weight, a.ld = D, a.M = M, a.V = V, a.D = D;
   a.padding = padding, a.scale = scale;
-  if (M == 0) l.few = true;  // zeros
   const int64_t size = dtype == 0 ? 4 : 2;
   const bool vector = (D * size) % 16 == 0 && myelin::aligned(grad_out, 16) && myelin::aligned(grad_weight, 16);
   hipStream_t s = myelin::as_hip(stream);

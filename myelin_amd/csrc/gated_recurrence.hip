@@ -402,7 +402,7 @@ __global__ __launch_bounds__(256) void step(Args a) {
 
 // A workgroup's lanes reach over this many batch rows; their offsets have 32 bits.
 bool reachable(int64_t stride, int64_t B, int64_t N) {
-  return B == 1 || (stride < int64_t{1} << 29 && (64 / N + 1) * stride + N < int64_t{1} << 29);
+  return B == 1 || (stride >= 0 && stride < int64_t{1} << 29 && (64 / N + 1) * stride + N < int64_t{1} << 29);
 }
 
 int check(const char *what, int dtype, int64_t T, int64_t B, int64_t N) {
@@ -491,7 +491,7 @@ extern "C" int myelin_gated_recurrence_fwd(const void *x, const void *gate, int 
   if (B == 0 || N == 0) return MYELIN_OK;
   if (!x || !gate || !strides || !out || !state_out) return myelin::invalid("%s: null pointer", what);
   for (int o = 1; o < 4; o += 2)
-    if (!reachable(strides[o], B, N)) return myelin::invalid("%s: batch stride too large", what);
+    if (!reachable(strides[o], B, N)) return myelin::invalid("%s: batch stride negative or too large", what);
   Args a{};
   a.T = T, a.B = B, a.N = N;
   Plan p;
@@ -516,7 +516,7 @@ extern "C" int myelin_gated_recurrence_bwd(const void *x, const void *gate, cons
   if (B == 0 || N == 0) return MYELIN_OK;
   if (!x || !gate || !strides || !kept) return myelin::invalid("%s: null pointer", what);
   for (int o = 1; o < (grad_out ? 6 : 4); o += 2)
-    if (!reachable(strides[o], B, N)) return myelin::invalid("%s: batch stride too large", what);
+    if (!reachable(strides[o], B, N)) return myelin::invalid("%s: batch stride negative or too large", what);
   Args a{};
   a.T = T, a.B = B, a.N = N;
   Plan p;

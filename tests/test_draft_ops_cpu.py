@@ -3,6 +3,7 @@ that check their arguments without launching, and no lost derivative."""
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -32,6 +33,14 @@ def test_recurrence_entry_points_validate():
                         (dict(strides=None), "null pointer")):
         with pytest.raises(ValueError, match=message):
             fwd(**kw)
+    # batch rows that a workgroup's 32-bit offsets do not reach
+    for stride in (-1, 2**29, 2**62):
+        strides = (ctypes.c_int64 * 6)(6, stride, 6, 3, 6, 3)
+        with pytest.raises(ValueError, match="batch stride"):
+            fwd(strides=strides)
+        with pytest.raises(ValueError, match="batch stride"):
+            _lib.call("myelin_gated_recurrence_bwd", 16, 16, 16, 0, strides, None, 16, None, 16, 16, 16, 4, 2, 3, None, 0,
+                      None)
     fwd(x=None, B=0)  # nothing to do
     fwd(x=None, N=0)
     bwd = ("myelin_gated_recurrence_bwd", 16, 16, 16, 0, 16, None)

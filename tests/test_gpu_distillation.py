@@ -215,6 +215,13 @@ def test_a_token_named_twice():
         _close(loss, want[0], "loss")
         _close(gx, want[1], "gradient")
         assert not bool(gx[2].any())
+        # the first of the two places with a probability that is 0 in float32
+        values = torch.tensor([[-300.0, 0.0, 1.0, -400.0]] * 3, device=DEV)
+        tokens = torch.tensor([[4, 4, 7, 4], [7, 4, 4, 7], [5, 9, 9, 9]], device=DEV)
+        loss, gx = _run(x, values, tokens, 1.0, weights)
+        want = _reference(x, values, tokens, 1.0, weights)
+        _close(loss, want[0], "loss")
+        _close(gx, want[1], "gradient")
 
 
 @pytest.mark.parametrize("shift", [-1e4, 1e4, 3e38])

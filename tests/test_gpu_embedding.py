@@ -180,6 +180,11 @@ def test_no_tokens():
     assert y.shape == (3, 0, 4)
     (gw,) = torch.autograd.grad(y, w, torch.empty_like(y))
     assert torch.equal(gw, torch.zeros_like(w))
+    # and more rows than a launch of sum_few would have workgroups
+    many = torch.ones(2**23 + 100, 1, device=DEV, requires_grad=True)
+    y = myelin.token_embedding(tokens, many)
+    (gm,) = torch.autograd.grad(y, many, torch.empty_like(y))
+    assert not bool(gm.any())
     # nothing but padding
     tokens = torch.full((100,), 2, device=DEV)
     y = myelin.token_embedding(tokens, w, padding_index=2)
