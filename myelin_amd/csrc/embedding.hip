@@ -9,7 +9,7 @@
 // The gradient takes the positions in the order of their tokens (a stable sort), so
 // that each row of the table is written once, by the threads that sum it, and
 // nothing is atomic.  A token may have a tenth of all positions: a run of equal
-// tokens is cut at multiples of 64 sorted positions, whole pieces are summed by
+// tokens is cut at multiples of 32 sorted positions, whole pieces are summed by
 // workgroups of their own, and the row's threads add up what is left.
 
 #include "elements.h"
@@ -276,25 +276,44 @@ __global__ __launch_bounds__(kOneWaves * kWave) void sort_one(Args a, int rounds
 // the bins, the offsets of all counts, and each position to its place.
 constexpr int kSortWaves = 4, kSortRounds = 16, kTurn = kSortWaves * kSortRounds * kWave;
 
+// Up to this many workgroups add all counts up themselves; more have it done for
+// them.  131072 positions, [2000, 256] bf16: 103 -> 71 us, with two passes of 6 bits in
+// place of 9.
+constexpr int kDirect = 64;
+
 struct Sort {
   Args a;
   const int32_t *from_keys, *from_places;  // null: the tokens
-  int32_t *to_keys, *to_places, *counts;   // counts [kBins, blocks]
+  int32_t *to_keys, *to_places, *counts;   // counts [blocks, bins] if direct, else [bins, blocks]
   int blocks, shift;
+  bool direct;
   int64_t stretch;  // a multiple of kTurn
   __device__ int32_t key(int64_t i) const { return from_keys ? from_keys[i < a.M ? i : a.M - 1] : key_of(a, i); }
   __device__ int32_t place(int64_t i) const { return from_keys ? from_places[i] : static_cast<int32_t>(i); }
 };
 
+template <int BITS>
 __global__ __launch_bounds__(kThreads) void sort_count(Sort s) {
-  __shared__ int32_t count[kBins];
-  for (int b = threadIdx.x; b < kBins; b += kThreads) count[b] = 0;
-  __syncthreads();
+  constexpr int BINS = 1 << BITS;
+  __shared__ int32_t count[kSortWaves][BINS];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  for (int b = lane; b < BINS; b += kWave) count[wave][b] = 0;
   const int64_t begin = blockIdx.x * s.stretch, end = begin + s.stretch < s.a.M ? begin + s.stretch : s.a.M;
-  for (int64_t i = begin + threadIdx.x; i < end; i += kThreads)
-    atomicAdd(&count[s.key(i) >> s.shift & (kBins - 1)], 1);
+  for (int64_t turn = begin; turn < end; turn += kTurn) {
+    const int64_t first = turn + wave * kSortRounds * kWave + lane;
+    int32_t k[kSortRounds];
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) k[r] = s.key(first + r * kWave);
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r)
+      place_in_wave<BITS>(count[wave], k[r] >> s.shift & (BINS - 1), first + r * kWave < end);
+  }
   __syncthreads();
-  for (int b = threadIdx.x; b < kBins; b += kThreads) s.counts[static_cast<int64_t>(b) * s.blocks + blockIdx.x] = count[b];
+  for (int b = tid; b < BINS; b += kThreads) {
+    int32_t sum = 0;
+    for (int w = 0; w < kSortWaves; ++w) sum += count[w][b];
+    s.counts[s.direct ? blockIdx.x * BINS + b : static_cast<int64_t>(b) * s.blocks + blockIdx.x] = sum;
+  }
 }
 
 // one workgroup: the sums of all counts before each
@@ -332,26 +351,61 @@ __global__ __launch_bounds__(1024) void sort_offsets(int32_t *counts, int64_t n)
   }
 }
 
+template <int BITS>
 __global__ __launch_bounds__(kThreads) void sort_place(Sort s) {
-  __shared__ int32_t count[kSortWaves][kBins], next[kBins];
+  constexpr int BINS = 1 << BITS;
+  __shared__ int32_t count[kSortWaves][BINS], next[BINS];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  for (int b = tid; b < kBins; b += kThreads) next[b] = s.counts[static_cast<int64_t>(b) * s.blocks + blockIdx.x];
+  if (s.direct) {
+    // what comes before this workgroup's: all smaller digits, and equal ones of
+    // earlier workgroups
+    for (int b = tid; b < BINS; b += kThreads) {
+      int32_t all = 0, earlier = 0;
+#pragma unroll 8
+      for (int o = 0; o < s.blocks; ++o) {
+        const int32_t c = s.counts[o * BINS + b];
+        all += c;
+        earlier += o < static_cast<int>(blockIdx.x) ? c : 0;
+      }
+      next[b] = earlier;
+      count[0][b] = all;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      constexpr int EACH = (BINS + kWave - 1) / kWave;
+      int32_t v[EACH], sum = 0;
+      for (int o = 0; o < EACH; ++o) {
+        v[o] = count[0][lane * EACH + o];
+        sum += v[o];
+      }
+      int32_t run = sum;
+      for (int o = 1; o < kWave; o <<= 1) {
+        const int32_t up = __shfl_up(run, o);
+        if (lane >= o) run += up;
+      }
+      run -= sum;
+      for (int o = 0; o < EACH; ++o) {
+        next[lane * EACH + o] += run;
+        run += v[o];
+      }
+    }
+    __syncthreads();
+  } else {
+    for (int b = tid; b < BINS; b += kThreads) next[b] = s.counts[static_cast<int64_t>(b) * s.blocks + blockIdx.x];
+  }
   const int64_t begin = blockIdx.x * s.stretch, end = begin + s.stretch < s.a.M ? begin + s.stretch : s.a.M;
   for (int64_t turn = begin; turn < end; turn += kTurn) {
     const int64_t first = turn + wave * kSortRounds * kWave + lane;
     int32_t k[kSortRounds];
-    for (int b = lane; b < kBins; b += kWave) count[wave][b] = 0;
+    for (int b = lane; b < BINS; b += kWave) count[wave][b] = 0;
 #pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-      const int64_t i = first + r * kWave;
-      k[r] = s.key(i);
-    }
+    for (int r = 0; r < kSortRounds; ++r) k[r] = s.key(first + r * kWave);
     int32_t local[kSortRounds];
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r)
-      local[r] = place_in_wave<kDigit>(count[wave], k[r] >> s.shift & (kBins - 1), first + r * kWave < end);
+      local[r] = place_in_wave<BITS>(count[wave], k[r] >> s.shift & (BINS - 1), first + r * kWave < end);
     __syncthreads();
-    for (int b = tid; b < kBins; b += kThreads) {
+    for (int b = tid; b < BINS; b += kThreads) {
       int32_t run = next[b];
       for (int w = 0; w < kSortWaves; ++w) {
         const int32_t c = count[w][b];
@@ -365,7 +419,7 @@ __global__ __launch_bounds__(kThreads) void sort_place(Sort s) {
     for (int r = 0; r < kSortRounds; ++r) {
       const int64_t i = first + r * kWave;
       if (i < end) {
-        const int32_t to = count[wave][k[r] >> s.shift & (kBins - 1)] + local[r];
+        const int32_t to = count[wave][k[r] >> s.shift & (BINS - 1)] + local[r];
         s.to_keys[to] = k[r];
         s.to_places[to] = s.place(i);
       }
@@ -375,7 +429,7 @@ __global__ __launch_bounds__(kThreads) void sort_place(Sort s) {
 }
 
 // ---- gradient: sums ---------------------------------------------------------
-constexpr int kPiece = 64;  // sorted positions of a piece, pieces of a larger one
+constexpr int kPiece = 32;  // sorted positions of a piece, pieces of a larger one
 
 // Sums n rows (of the list places[0, n)) into r, in order, some loads at a time.
 template <class E, int VEC>
@@ -401,7 +455,7 @@ __device__ __forceinline__ void sum_rows(const Args &a, const int32_t *places, i
 // fp32 rows [n, D] in a row
 template <class E, int VEC>
 __device__ __forceinline__ void sum_pieces(const float *from, int64_t n, int64_t D, Vector<E, VEC> &r) {
-  constexpr int MANY = 4;
+  constexpr int MANY = 8;
   int64_t i = 0;
   for (; i + MANY <= n; i += MANY) {
     float v[MANY][VEC];
@@ -465,7 +519,7 @@ __global__ __launch_bounds__(kThreads) void sum_whole_pieces(Args a, int per, in
     for (int q = 0; q < VEC; ++q) a.pieces[piece * a.D + u * VEC + q] = r.v[q];
 }
 
-// and 64 of those that one token has
+// and 32 of those that one token has
 template <class E, int VEC>
 __global__ __launch_bounds__(kThreads) void sum_larger_pieces(Args a, int per) {
   __shared__ float red[kThreads * VEC];
@@ -487,21 +541,22 @@ __global__ __launch_bounds__(kThreads) void sum_larger_pieces(Args a, int per) {
 
 // Each row of the table: what of its run is before the first whole piece, the whole
 // pieces (the larger ones among them), what is behind them.  ZEROED: rows without
-// positions are there already.
-constexpr int kTableRows = 4;  // of a group of threads
+// positions are there already.  ROWS of a group of threads: 1 where the table is
+// small, so that its rows with many positions do not wait for each other.
+constexpr int kTableRows = 4;
 
-template <class E, int VEC, bool STREAM, bool ZEROED>
+template <class E, int VEC, int ROWS, bool STREAM, bool ZEROED>
 __global__ __launch_bounds__(kThreads) void sum_runs(Args a, int per) {
   using T = typename E::T;
   const int groups = kThreads / per, group = threadIdx.x / per;
   const int64_t block = myelin::block_id(), rows = block / a.slices, slice = block - rows * a.slices;
-  const int64_t first = (rows * groups + group) * kTableRows, u = slice * per + threadIdx.x % per;
+  const int64_t first = (rows * groups + group) * ROWS, u = slice * per + threadIdx.x % per;
   if (first >= a.V || u >= a.units) return;
-  int32_t start[kTableRows + 1];
+  int32_t start[ROWS + 1];
 #pragma unroll
-  for (int o = 0; o <= kTableRows; ++o) start[o] = a.starts[first + o < a.V ? first + o : a.V];
+  for (int o = 0; o <= ROWS; ++o) start[o] = a.starts[first + o < a.V ? first + o : a.V];
 #pragma unroll
-  for (int o = 0; o < kTableRows; ++o) {
+  for (int o = 0; o < ROWS; ++o) {
     const int64_t v = first + o, lo = start[o], hi = start[o + 1];
     if (v >= a.V) return;
     if (ZEROED && lo == hi) continue;
@@ -621,7 +676,7 @@ Layout layout_of(int64_t M, int64_t V, int64_t D) {
   }
   l.starts = take(4 * (V + 1));
   l.pieces = take(4 * (M / kPiece) * D);
-  // (a run of 16384 has 256 pieces: few enough to add up at once)
+  // (a run of 16384 has 512 pieces: few enough to add up at once)
   l.pieces2 = l.one ? -1 : take(4 * (M / (kPiece * kPiece)) * D);
   l.size = at;
   return l;
@@ -638,6 +693,13 @@ void launch_lookup(Args &a, hipStream_t s) {
     lookup<E, VEC, true><<<grid, kThreads, 0, s>>>(a, per);
   else
     lookup<E, VEC, false><<<grid, kThreads, 0, s>>>(a, per);
+}
+
+template <int BITS>
+void launch_sort(const Sort &t, hipStream_t s) {
+  sort_count<BITS><<<t.blocks, kThreads, 0, s>>>(t);
+  if (!t.direct) sort_offsets<<<1, 1024, 0, s>>>(t.counts, (int64_t{1} << BITS) * t.blocks);
+  sort_place<BITS><<<t.blocks, kThreads, 0, s>>>(t);
 }
 
 template <class E, int VEC>
@@ -671,12 +733,16 @@ void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
     a.keys = words(l.keys[0]);
     a.places = words(l.places[0]);
   } else {
+    const int digit = l.bits <= 6 ? 6 : l.bits <= 8 ? 8 : 9;
     for (int pass = 0; pass < l.passes; ++pass) {
       Sort t{a, pass ? a.keys : nullptr, pass ? a.places : nullptr, words(l.keys[pass & 1]), words(l.places[pass & 1]),
-             words(l.counts), l.blocks, pass * kDigit, l.stretch};
-      sort_count<<<l.blocks, kThreads, 0, s>>>(t);
-      sort_offsets<<<1, 1024, 0, s>>>(t.counts, static_cast<int64_t>(kBins) * l.blocks);
-      sort_place<<<l.blocks, kThreads, 0, s>>>(t);
+             words(l.counts), l.blocks, pass * digit, l.blocks <= kDirect, l.stretch};
+      if (digit == 6)
+        launch_sort<6>(t, s);
+      else if (digit == 8)
+        launch_sort<8>(t, s);
+      else
+        launch_sort<9>(t, s);
       a.keys = t.to_keys;
       a.places = t.to_places;
     }
@@ -690,15 +756,20 @@ void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
     sum_larger_pieces<E, VEC><<<myelin::grid_of(a.M / (kPiece * kPiece) * a.slices), kThreads, 0, s>>>(a, per);
   per = threads_of(a.units, kThreads);
   a.slices = (a.units + per - 1) / per;
-  const int64_t rows = kThreads / per * kTableRows;
-  const dim3 grid = myelin::grid_of((a.V + rows - 1) / rows * a.slices);
+  const int64_t groups = kThreads / per;
+  const auto grid = [&](int64_t rows) { return myelin::grid_of((a.V + rows - 1) / rows * a.slices); };
   const bool stream = bytes >= myelin::kStreamBytes;
-  if (zeroed)
-    stream ? sum_runs<E, VEC, true, true><<<grid, kThreads, 0, s>>>(a, per)
-           : sum_runs<E, VEC, false, true><<<grid, kThreads, 0, s>>>(a, per);
+  // 131072 positions, [2000, 256] bf16: 127 us with 4 rows a group, 110 with 2
+  if (!zeroed && !stream && a.V / groups * a.slices < 4096)
+    sum_runs<E, VEC, 1, false, false><<<grid(groups), kThreads, 0, s>>>(a, per);
+  else if (zeroed && stream)
+    sum_runs<E, VEC, kTableRows, true, true><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
+  else if (zeroed)
+    sum_runs<E, VEC, kTableRows, false, true><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
+  else if (stream)
+    sum_runs<E, VEC, kTableRows, true, false><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
   else
-    stream ? sum_runs<E, VEC, true, false><<<grid, kThreads, 0, s>>>(a, per)
-           : sum_runs<E, VEC, false, false><<<grid, kThreads, 0, s>>>(a, per);
+    sum_runs<E, VEC, kTableRows, false, false><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
 }
 
 int check(const char *what, int dtype, int64_t M, int64_t V, int64_t D, float scale) {

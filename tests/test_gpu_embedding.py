@@ -61,7 +61,8 @@ def _grad(tokens, weight, g, **kw):
 
 SIZES = [((1,), 1, 1), ((), 5, 3), ((3,), 7, 64), ((7, 5), 11, 130), ((64, 32), 50, 128), ((1000,), 3, 33),
          ((4097,), 1000, 17), ((300, 7), 2, 8), ((129,), 100003, 5), ((20000,), 700, 24), ((33, 1000), 40000, 9),
-         ((70000,), 5, 4), ((17000,), 300000, 3), ((2,), 3, 5000), ((140000,), 513, 2)]
+         ((70000,), 5, 4), ((17000,), 300000, 3), ((2,), 3, 5000), ((140000,), 513, 2), ((40000,), 30000, 2),
+         ((270000,), 200, 3), ((280000,), 90000, 2), ((265000,), 40, 5)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
