@@ -103,30 +103,40 @@ __device__ __forceinline__ void store_nothing(const Args &a, int64_t row, int la
   }
 }
 
-// Bits of the tokens seen, by their number modulo BITS: a wave's, cleared.  Only
-// where two meet is it looked at which are the same.
+// Bits of the tokens seen, by their number modulo BITS, and of those where two have
+// met: a wave's, cleared.  Only for the latter is it looked at which are the same.
 constexpr int kSeen = 1 << 15;
 
 template <int BITS>
-__device__ __forceinline__ void clear(uint32_t *seen, int lane) {
-  for (int o = lane; o < BITS / 32; o += kWave) seen[o] = 0;
-}
+struct Seen {
+  uint32_t once[BITS / 32], twice[BITS / 32];
+  __device__ void clear(int lane) {
+    for (int o = lane; o < BITS / 32; o += kWave) once[o] = twice[o] = 0;
+  }
+  __device__ void add(int64_t token) {
+    const uint32_t at = static_cast<uint32_t>(token) % BITS, bit = 1u << (at % 32);
+    if (atomicOr(&once[at / 32], bit) & bit) atomicOr(&twice[at / 32], bit);
+  }
+  __device__ bool met(int64_t token) const {
+    const uint32_t at = static_cast<uint32_t>(token) % BITS;
+    return twice[at / 32] >> (at % 32) & 1;
+  }
+};
 
 // The row's loss from its logits' statistics, by one wave.
 template <class E, int BITS>
-__device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int lane, uint32_t *seen) {
+__device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int lane, Seen<BITS> &seen) {
   const int64_t first = row * a.K;
   const typename E::T *x = static_cast<const typename E::T *>(a.x) + row * a.ld;
   float peak = kLowest;
-  bool bad = false, twice = false;
+  bool bad = false;
   for (int k = lane; k < a.K; k += kWave) {
     const int64_t token = a.tokens[first + k];
     const float v = a.values[first + k];
     if (empty(token, v)) continue;
     peak = fmaxf(peak, v);
     bad |= token < 0 || token >= a.V;
-    const uint32_t at = static_cast<uint32_t>(token) % BITS, bit = 1u << (at % 32);
-    if (a.probs) twice |= (atomicOr(&seen[at / 32], bit) & bit) != 0;
+    if (a.probs) seen.add(token);
   }
   for (int o = kWave >> 1; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
   float total = 0.0f;
@@ -135,15 +145,16 @@ __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int 
       total += myelin::exp_f32((a.values[first + k] - peak) * a.rate);
   total = wave_sum(total);
   bad = __any(bad);
-  twice = __any(twice);
   const float log_total = logf(total), log_s = t.s == 0.0f ? -kInf : logf(t.s);
   float loss = 0.0f;
-  for (int k = lane; k < a.K; k += kWave) {
-    const int64_t token = a.tokens[first + k];
-    const bool there = !empty(token, a.values[first + k]);
+  for (int at = 0; at < a.K; at += kWave) {
+    const int k = at + lane;
+    const int64_t token = k < a.K ? a.tokens[first + k] : -1;
+    const float value = k < a.K ? a.values[first + k] : 0.0f;
+    const bool there = !empty(token, value);
     float p = 0.0f;
     if (there) {
-      const float d = (a.values[first + k] - peak) * a.rate;
+      const float d = (value - peak) * a.rate;
       p = myelin::exp_f32(d) / total;
       if (p != 0.0f && !bad) {
         // nothing allowed: log q is -inf for every token
@@ -151,18 +162,25 @@ __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int 
         loss += p * ((d - log_total) - log_q);
       }
     }
-    if (a.probs && twice && there) {
-      // put together, in the places' order, at the first (whose own may be 0)
+    if (!a.probs) continue;
+    // what the places of a token have, in their order, goes to the first of them
+    for (uint64_t m = __ballot(there && seen.met(token)); m; m &= m - 1) {
+      const int one = __builtin_ctzll(m);
+      const int64_t name = __shfl(token, one);
+      int place = -1;
       float sum = 0.0f;
-      bool mine = true;
-      for (int o = 0; o < a.K; ++o)
-        if (a.tokens[first + o] == token && a.values[first + o] != -kInf) {
-          mine &= o >= k;
-          sum += myelin::exp_f32((a.values[first + o] - peak) * a.rate) / total;
+      for (int from = 0; from < a.K; from += kWave) {
+        const int o = from + lane;
+        const bool same = o < a.K && a.tokens[first + o] == name && a.values[first + o] != -kInf;
+        const float v = same ? myelin::exp_f32((a.values[first + o] - peak) * a.rate) / total : 0.0f;
+        for (uint64_t s = __ballot(same); s; s &= s - 1) {
+          if (place < 0) place = from + __builtin_ctzll(s);
+          sum += __shfl(v, __builtin_ctzll(s));
         }
-      p = mine ? sum : 0.0f;
+      }
+      if (lane == one) p = place == k ? sum : 0.0f;
     }
-    if (a.probs) a.probs[first + k] = p;
+    if (k < a.K) a.probs[first + k] = p;
   }
   loss = wave_sum(loss);
   if (lane == 0) {
@@ -176,13 +194,13 @@ __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int 
 // All of the row in registers: 2048 rows of 1000 fp32 6.5 us (8 MB), latency.
 template <class E>
 __global__ __launch_bounds__(kThreads) void narrow_rows(Args a) {
-  __shared__ uint32_t seen[kWaves][kNarrow / 32];
+  __shared__ Seen<kNarrow> seen[kWaves];
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x >> 6;
   const int64_t row = myelin::block_id() * kWaves + w;
   if (row >= a.R) return;  // whole waves
   const typename E::T *x = static_cast<const typename E::T *>(a.x) + row * a.ld;
   // (in LDS a wave's own writes and atomics are done in its order)
-  if (a.probs) clear<kNarrow>(seen[w], lane);
+  if (a.probs) seen[w].clear(lane);
   if (nothing(a, row, lane)) {
     store_nothing(a, row, lane);
     return;
@@ -198,7 +216,7 @@ __global__ __launch_bounds__(kThreads) void narrow_rows(Args a) {
 #pragma unroll
   for (int o = 0; o < kEach; ++o) t.s += r.exp(v[o] - t.m);
   t = across(t, a.rate);
-  finish<E, kNarrow>(a, row, t, lane, seen[w]);
+  finish<E>(a, row, t, lane, seen[w]);
 }
 
 // ---- wide rows: a workgroup to a row, or to one of its parts -------------
@@ -213,7 +231,7 @@ __global__ __launch_bounds__(kThreads) void wide_rows(Args a) {
   using T = typename E::T;
   constexpr int VEC = E::VEC, NV = kPerThread / VEC;
   __shared__ Stats red[kWaves];
-  __shared__ uint32_t seen[kSeen / 32];
+  __shared__ Seen<kSeen> seen;
   const int tid = threadIdx.x, lane = tid & (kWave - 1), w = tid >> 6;
   const int64_t row = blockIdx.x / a.parts + blockIdx.y * a.rows;
   if (row >= a.R) return;  // the whole workgroup
@@ -224,7 +242,7 @@ __global__ __launch_bounds__(kThreads) void wide_rows(Args a) {
     if (part == 0 && w == 0) store_nothing(a, row, lane);
     return;
   }
-  if (a.probs && w == 0) clear<kSeen>(seen, lane);
+  if (a.probs && w == 0 && a.parts == 1) seen.clear(lane);
   const Rate r(a.rate);
   const T *x = static_cast<const T *>(a.x) + row * a.ld;
   // whole vectors start where the address is a multiple of 16: `lead` elements
@@ -263,20 +281,20 @@ __global__ __launch_bounds__(kThreads) void wide_rows(Args a) {
     if (lane == 0) a.part_stats[row * a.parts + part] = t;
     return;
   }
-  finish<E, kSeen>(a, row, t, lane, seen);
+  finish<E>(a, row, t, lane, seen);
 }
 
 // joins a row's parts: a wave a row
 template <class E>
 __global__ __launch_bounds__(kWave) void join_parts(Args a) {
-  __shared__ uint32_t seen[kSeen / 32];
+  __shared__ Seen<kSeen> seen;
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
-  if (a.probs) clear<kSeen>(seen, lane);
+  if (a.probs) seen.clear(lane);
   if (nothing(a, row, lane)) return;
   Stats t = Stats::none();
   for (int p = lane; p < a.parts; p += kWave) t.merge(a.part_stats[row * a.parts + p], a.rate);
-  finish<E, kSeen>(a, row, across(t, a.rate), lane, seen);
+  finish<E>(a, row, across(t, a.rate), lane, seen);
 }
 
 // ---- gradient ------------------------------------------------------------
@@ -296,33 +314,47 @@ struct BwdArgs {
 // their p into LDS, at their element's place, and a bit that says that it is there:
 // an element looks at a bit, not at the tokens.  8192 x 32768 bf16 with 64 tokens: 176
 // us (1.02 GB, 5.8 TB/s), bound by memory.
-template <class E, int GROUP, bool VECTOR, bool STREAM>
+//
+// kSkewed: logits and gradients of a row start equally far from a multiple of 16
+// bytes.  Tiles start at the multiple before the row, and only what sticks out at its
+// ends goes element by element (2048 x 100003 bf16: 354 us element by element, 160
+// so).  kWhole: they start there and end there, which spares 2 % of the time.
+enum Rows { kSingly, kWhole, kSkewed };
+
+template <class E, int GROUP, Rows ROWS, bool STREAM>
 __global__ __launch_bounds__(kThreads) void gradient(BwdArgs a) {
   using T = typename E::T;
+  constexpr bool VECTOR = ROWS != kSingly;
   constexpr int VEC = VECTOR ? E::VEC : 1, NV = kPerThread / VEC, TILE = GROUP * kPerThread;
   typedef T vec __attribute__((ext_vector_type(VEC)));
   __shared__ float put[kThreads / GROUP][TILE];
   __shared__ uint32_t bits[kThreads / GROUP][TILE / 32];
   const int tid = threadIdx.x % GROUP, group = threadIdx.x / GROUP;
   const int64_t unit = myelin::block_id() * (kThreads / GROUP) + group, row = unit / a.per_row;
-  const int64_t at = (unit - row * a.per_row) * TILE;
   const bool in = row < a.R;
-  const float m = in ? a.stats[row] : 0.0f, log_s = in ? a.stats[a.R + row] : -kInf;
-  const bool zero = log_s == -kInf;
   const T *x = static_cast<const T *>(a.x) + (in ? row : 0) * a.ld;
   T *dx = static_cast<T *>(a.dx) + row * a.V;
+  const int lead = ROWS == kSkewed ? static_cast<int>(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)) : 0;
+  const int64_t at = (unit - row * a.per_row) * TILE - lead;
+  const float m = in ? a.stats[row] : 0.0f, log_s = in ? a.stats[a.R + row] : -kInf;
+  const bool zero = log_s == -kInf;
   float v[kPerThread];
   if (!zero) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int64_t i = at + (static_cast<int64_t>(j) * GROUP + tid) * VEC;
-      if (i >= a.V) continue;
-      if constexpr (VECTOR) {  // V is a multiple of VEC
-        const vec p = __builtin_nontemporal_load(reinterpret_cast<const vec *>(x + i));
+      if (ROWS == kWhole && i >= a.V) continue;
+      if (ROWS == kWhole || (i >= 0 && i + VEC <= a.V)) {
+        if constexpr (VECTOR) {
+          const vec p = __builtin_nontemporal_load(reinterpret_cast<const vec *>(x + i));
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) v[j * VEC + q] = E::get(p[q]);
+          for (int q = 0; q < VEC; ++q) v[j * VEC + q] = E::get(p[q]);
+        } else {
+          v[j] = E::get(x[i]);
+        }
       } else {
-        v[j] = E::get(x[i]);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) v[j * VEC + q] = i + q >= 0 && i + q < a.V ? E::get(x[i + q]) : 0.0f;
       }
     }
   }
@@ -344,7 +376,7 @@ __global__ __launch_bounds__(kThreads) void gradient(BwdArgs a) {
   for (int j = 0; j < NV; ++j) {
     const int o = (j * GROUP + tid) * VEC;
     const int64_t i = at + o;
-    if (i >= a.V) continue;
+    if (i >= a.V || i + VEC <= 0) continue;
     T out[VEC];
     if (zero) {
 #pragma unroll
@@ -362,13 +394,15 @@ __global__ __launch_bounds__(kThreads) void gradient(BwdArgs a) {
 #pragma unroll
       for (int q = 0; q < VEC; ++q) out[q] = E::put(g * d[q]);
     }
-    if constexpr (VECTOR) {
+    if (ROWS == kWhole || (VECTOR && i >= 0 && i + VEC <= a.V)) {
       vec w;
 #pragma unroll
       for (int q = 0; q < VEC; ++q) w[q] = out[q];
       myelin::store<STREAM>(w, reinterpret_cast<vec *>(dx + i));
     } else {
-      dx[i] = out[0];
+#pragma unroll
+      for (int q = 0; q < VEC; ++q)
+        if (i + q >= 0 && i + q < a.V) dx[i + q] = out[q];
     }
   }
 }
@@ -399,17 +433,22 @@ void launch_fwd(Args &a, hipStream_t s) {
 
 template <class E, int GROUP>
 void launch_gradient(BwdArgs &a, hipStream_t s) {
-  a.per_row = (a.V + GROUP * kPerThread - 1) / (GROUP * kPerThread);
+  const int64_t size = sizeof(typename E::T);
+  const bool vector = (reinterpret_cast<uintptr_t>(a.x) - reinterpret_cast<uintptr_t>(a.dx)) % 16 == 0 &&
+                      (a.R == 1 || (a.ld - a.V) * size % 16 == 0);
+  const bool whole = myelin::aligned(a.x, 16) && a.V * size % 16 == 0;
+  a.per_row = (a.V + (vector && !whole ? E::VEC - 1 : 0) + GROUP * kPerThread - 1) / (GROUP * kPerThread);
   const int64_t units = a.R * a.per_row, each = kThreads / GROUP;
   const dim3 grid = myelin::grid_of((units + each - 1) / each);
-  const bool vector = a.V % E::VEC == 0 && (a.ld * sizeof(typename E::T)) % 16 == 0 && myelin::aligned(a.x, 16) &&
-                      myelin::aligned(a.dx, 16);
+  const bool stream = a.R * a.V * size >= myelin::kStreamBytes;
   if (!vector)
-    gradient<E, GROUP, false, false><<<grid, kThreads, 0, s>>>(a);
-  else if (a.R * a.V * static_cast<int64_t>(sizeof(typename E::T)) >= myelin::kStreamBytes)
-    gradient<E, GROUP, true, true><<<grid, kThreads, 0, s>>>(a);
+    gradient<E, GROUP, kSingly, false><<<grid, kThreads, 0, s>>>(a);
+  else if (whole)
+    stream ? gradient<E, GROUP, kWhole, true><<<grid, kThreads, 0, s>>>(a)
+           : gradient<E, GROUP, kWhole, false><<<grid, kThreads, 0, s>>>(a);
   else
-    gradient<E, GROUP, true, false><<<grid, kThreads, 0, s>>>(a);
+    stream ? gradient<E, GROUP, kSkewed, true><<<grid, kThreads, 0, s>>>(a)
+           : gradient<E, GROUP, kSkewed, false><<<grid, kThreads, 0, s>>>(a);
 }
 
 template <class E>

@@ -136,18 +136,22 @@ __device__ __forceinline__ void mask(T *v, int n, T past) {
   for (int i = 0; i < STEPS; ++i) v[i] = i < n ? v[i] : past;
 }
 
-// The state before segment a.seg, from the one before the first.
-__device__ __forceinline__ float join_before(const Args &a, int64_t c, float s) {
-  for (int64_t o = 0; o < a.seg; ++o) {
-    const Affine m = a.joins[o * a.B * a.N + c];
-    s = __builtin_fmaf(m.A, s, m.H);
+// The state in front of a channel's segments joined in order, `step` apart from the
+// first of them: eight at a time, so that their loads do not wait for each other.
+__device__ __forceinline__ float join(const Args &a, int64_t c, float s, int64_t from, int64_t count, int64_t step) {
+  const int64_t BN = a.B * a.N;
+  const Affine *m = a.joins + from * BN + c;
+  int64_t o = 0;
+  for (; o + 8 <= count; o += 8) {
+    Affine q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = m[(o + i) * step * BN];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = __builtin_fmaf(q[i].A, s, q[i].H);
   }
-  return s;
-}
-__device__ __forceinline__ float join_after(const Args &a, int64_t c, float s) {
-  for (int64_t o = a.segments - 1; o > a.seg; --o) {
-    const Affine m = a.joins[o * a.B * a.N + c];
-    s = __builtin_fmaf(m.A, s, m.H);
+  for (; o < count; ++o) {
+    const Affine q = m[o * step * BN];
+    s = __builtin_fmaf(q.A, s, q.H);
   }
   return s;
 }
@@ -179,7 +183,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void forward(Args a) {
   const int64_t BN = a.B * a.N, first = a.seg * a.seg_steps;
   const int64_t end = first + a.seg_steps < a.T ? first + a.seg_steps : a.T;
   float s = p.in && a.state ? a.state[p.c()] : 0.0f;
-  if (p.in) s = join_before(a, p.c(), s);
+  if (p.in) s = join(a, p.c(), s, 0, a.seg, 1);
   T x[kSteps], gate[kSteps];
   int n = 0;
   const auto fetch = [&](int64_t tile) {
@@ -253,7 +257,7 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void backward(Args a) {
   const int64_t BN = a.B * a.N, first = a.seg * a.seg_steps;
   const int64_t end = first + a.seg_steps < a.T ? first + a.seg_steps : a.T;
   float s = p.in && a.state ? a.state[p.c()] : 0.0f;
-  if (p.in) s = join_after(a, p.c(), s);
+  if (p.in) s = join(a, p.c(), s, a.segments - 1, a.segments - 1 - a.seg, -1);
   T x[kBackSteps], gate[kBackSteps], go[kBackSteps];
   float start = 0.0f;
   int n = 0;
