@@ -381,17 +381,20 @@ struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
   }
 };
 
-// x and gate as recurrence_rows gives them, the others contiguous
-variable_list gated_recurrence(const Tensor &x, const Tensor &gate, const OptTensor &state, const OptTensor &lengths) {
-  const c10::DeviceGuard guard(x.device());
+// state and lengths contiguous
+variable_list gated_recurrence(const Tensor &given_x, const Tensor &given_gate, const OptTensor &state,
+                               const OptTensor &lengths) {
+  const c10::DeviceGuard guard(given_x.device());
+  const Tensor x = recurrence_rows(given_x), gate = recurrence_rows(given_gate);
   if (needs({x, gate, plain(state)})) return RecurrenceFunction::apply(x, gate, state, lengths);
   return recurrence_forward(x, gate, plain(state), plain(lengths), nullptr);
 }
 
 // {new state, out}; the new state goes to out_state, if given
-variable_list gated_recurrence_step(const Tensor &x, const Tensor &gate, const Tensor &state,
+variable_list gated_recurrence_step(const Tensor &given_x, const Tensor &given_gate, const Tensor &given_state,
                                     const OptTensor &out_state) {
-  const c10::DeviceGuard guard(x.device());
+  const c10::DeviceGuard guard(given_x.device());
+  const Tensor x = recurrence_rows(given_x), gate = recurrence_rows(given_gate), state = given_state.contiguous();
   const int64_t B = x.size(0), N = x.size(1);
   Tensor out = torch::empty({B, N}, x.options());
   Tensor to = out_state.has_value() ? *out_state : torch::empty({B, N}, state.options());

@@ -98,21 +98,19 @@ class HipGatedRecurrenceFunction(torch.autograd.Function):
 
 
 def _check(x, gate, ndim, dims):
-    for name, t in (("x", x), ("gate", gate)):
-        if t.ndim != ndim:
-            raise ValueError(f"{name} must be shaped {dims}; got {tuple(t.shape)}")
-        _lib.require_device(t, name)
-        if t.dtype not in _TYPES:
-            raise ValueError(f"{name} must be float32 or bfloat16; got {t.dtype}")
+    if x.ndim != ndim:
+        raise ValueError(f"x must be shaped {dims}; got {tuple(x.shape)}")
+    _lib.require_device(x, "x")
+    if x.dtype not in _TYPES:
+        raise ValueError(f"x must be float32 or bfloat16; got {x.dtype}")
     if gate.shape != x.shape or gate.dtype != x.dtype or gate.device != x.device:
         raise ValueError(f"gate must have the shape, dtype and device of x; got {gate.dtype}, {tuple(gate.shape)} on "
                          f"{gate.device}")
 
 
 def _check_state(state, x, name):
-    want = tuple(x.shape[-2:])
-    if tuple(state.shape) != want:
-        raise ValueError(f"{name} must be shaped [B, N] = {want}; got {tuple(state.shape)}")
+    if state.shape != x.shape[-2:]:
+        raise ValueError(f"{name} must be shaped [B, N] = {tuple(x.shape[-2:])}; got {tuple(state.shape)}")
     if state.dtype != torch.float32 or state.device != x.device:
         raise ValueError(f"{name} must be float32 on the device of x")
 
@@ -155,11 +153,10 @@ def gated_recurrence(
         if lengths.dtype == torch.int64:
             lengths = lengths.clamp(0, x.shape[0]).to(torch.int32)
         lengths = lengths.contiguous()
-    x, gate = _rows(x), _rows(gate)
     if autograd.plain(x, gate) and (initial_state is None or autograd.plain(initial_state)):
         state, out = autograd.native().gated_recurrence(x, gate, initial_state, lengths)
         return state, out
-    return HipGatedRecurrenceFunction.apply(x, gate, initial_state, lengths)
+    return HipGatedRecurrenceFunction.apply(_rows(x), _rows(gate), initial_state, lengths)
 
 
 def gated_recurrence_step(
@@ -173,7 +170,8 @@ def gated_recurrence_step(
     ``gate [B, N]``, ``state [B, N]``.
 
     Returns ``(state, out [B, N])``.  The new state goes to ``out_state``
-    (contiguous; ``state`` itself for an update in place) or to a new tensor.
+    (contiguous; ``state`` itself for an update in place; no part of ``x`` or
+    ``gate``) or to a new tensor.
     """
 
     _check(x, gate, 2, "[B, N]")
@@ -181,8 +179,8 @@ def gated_recurrence_step(
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, gate, state)):
         raise ValueError("gated_recurrence_step has no gradient; use gated_recurrence, or torch.no_grad()")
     autograd.refuse_tangents("gated_recurrence_step", x, gate, state)
-    state = state.contiguous()
     if out_state is not None:
+        state = state.contiguous()
         _check_state(out_state, x, "out_state")
         if not out_state.is_contiguous():
             raise ValueError("out_state must be contiguous")
@@ -191,7 +189,12 @@ def gated_recurrence_step(
         a, b, size = state.data_ptr(), out_state.data_ptr(), 4 * state.numel()
         if a != b and a < b + size and b < a + size:
             raise ValueError("out_state must be state itself or not overlap it")
-    new, out = autograd.native().gated_recurrence_step(_rows(x), _rows(gate), state, out_state)
+        for name, t in (("x", x), ("gate", gate)):
+            a = t.data_ptr()
+            end = a + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+            if size and a < b + size and b < end:
+                raise ValueError(f"out_state must not overlap {name}")
+    new, out = autograd.native().gated_recurrence_step(x, gate, state, out_state)
     return (new if out_state is None else out_state), out
 
 

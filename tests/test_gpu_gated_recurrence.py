@@ -421,3 +421,16 @@ def test_module():
             s, y = m.step(x[t], s, out_state=s)
     # (the projection of 3 rows and of 90 may differ in its sums' last bits)
     assert float((s - whole).abs().max()) <= 1e-5
+
+
+def test_a_state_that_overlaps_the_inputs_is_refused():
+    """Its elements would be written while others still read them as inputs."""
+
+    base = torch.zeros(16, device=DEV)
+    x, free, s = base[:6].view(2, 3), base[6:12].view(2, 3), torch.zeros(2, 3, device=DEV)
+    other = torch.zeros(2, 3, device=DEV)
+    for a, b, name in ((x, other, "x"), (other, x, "gate"), (base[:10].view(2, 5)[:, :3], other, "x")):
+        with pytest.raises(ValueError, match=f"must not overlap {name}"):
+            myelin.gated_recurrence_step(a, b, s, out_state=base[4:10].view(2, 3))
+    new, out = myelin.gated_recurrence_step(x, other, s + 1, out_state=free)  # beside them
+    assert torch.equal(free, out) and torch.equal(new, free) and torch.equal(free, torch.full_like(s, 0.5))
