@@ -432,6 +432,14 @@ struct Plan {
   int waves;
 };
 
+// A CU holds 16 waves of these registers: its workgroups share them, so that none waits
+// for others to end and each runs over several tiles, whose loads and sums overlap.
+// bf16, forward and backward, against 16 waves to each: [512, 32, 2048] 60 -> 50 us and
+// 97 -> 83, [67, 38, 6917] 45 -> 34 and 73 -> 56, [256, 66, 1000] 33 -> 26 and 59 -> 44.
+// (Powers of two: 5 waves fall on the SIMDs so that three workgroups do not fit a CU.
+// One wave to a workgroup of many: [200, 150, 2048] backward 151 -> 167.  LDS of the
+// waves' own size, so that two have 2 KB of it: 2 % slower everywhere.)
+//
 // Time is split where the channels leave half of the CUs without a workgroup: 128
 // blocks in two segments, [8192, 4, 2048] bf16: forward 142 us either way, backward
 // 276 -> 210; 175 blocks are faster whole (70 and 140 us, against 101 and 172).
@@ -439,7 +447,9 @@ Plan plan_of(int64_t T, int64_t B, int64_t N) {
   Plan p;
   p.blocks = (B * N + kWave - 1) / kWave;
   const int64_t needed = (T + kSteps - 1) / kSteps;
-  p.waves = static_cast<int>(needed < kMaxWaves ? needed : kMaxWaves);
+  int waves = kMaxWaves;
+  while (waves > 2 && p.blocks * waves > 256 * kMaxWaves) waves /= 2;
+  p.waves = static_cast<int>(needed < waves ? needed : waves);
   const int64_t tile = p.waves * kSteps, tiles = (T + tile - 1) / tile;
   int64_t n = p.blocks > 128 ? 1 : 256 / p.blocks;
   if (n > tiles) n = tiles;

@@ -434,3 +434,12 @@ def test_a_state_that_overlaps_the_inputs_is_refused():
             myelin.gated_recurrence_step(a, b, s, out_state=base[4:10].view(2, 3))
     new, out = myelin.gated_recurrence_step(x, other, s + 1, out_state=free)  # beside them
     assert torch.equal(free, out) and torch.equal(new, free) and torch.equal(free, torch.full_like(s, 0.5))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,B,N", [(150, 301, 64), (129, 5, 3301), (75, 150, 257), (50, 33, 2200), (41, 5, 27001)])
+def test_workgroups_that_share_a_cu(T, B, N, dtype):
+    """With more channels than the CUs have workgroups for at once, fewer waves to
+    each go over several tiles."""
+
+    test_sequences_and_gradients(T, B, N, dtype)
