@@ -156,137 +156,22 @@ __device__ __forceinline__ int32_t place_in_wave(int32_t *count, int digit, bool
   return had + rank;
 }
 
-// Takes each wave's counts of the bins to where its items of them go, with `base`
-// for each bin the count of all smaller ones.  WAVES * 64 threads; scratch of kBins.
-template <int WAVES>
-__device__ __forceinline__ void offsets(int32_t (*count)[kBins], int32_t *scratch) {
-  const int tid = threadIdx.x;
-  for (int b = tid; b < kBins; b += WAVES * kWave) {
-    int32_t c[WAVES], sum = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) c[w] = count[w][b];
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      count[w][b] = sum;
-      sum += c[w];
-    }
-    scratch[b] = sum;
-  }
-  __syncthreads();
-  if (tid < kWave) {  // a wave adds the bins up: 8 each, then the lanes
-    constexpr int EACH = kBins / kWave;
-    int32_t v[EACH], sum = 0;
-    for (int o = 0; o < EACH; ++o) {
-      v[o] = scratch[tid * EACH + o];
-      sum += v[o];
-    }
-    int32_t run = sum;
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int32_t up = __shfl_up(run, o);
-      if (tid >= o) run += up;
-    }
-    run -= sum;
-    for (int o = 0; o < EACH; ++o) {
-      scratch[tid * EACH + o] = run;
-      run += v[o];
-    }
-  }
-  __syncthreads();
-  for (int b = tid; b < kBins; b += WAVES * kWave) {
-    const int32_t base = scratch[b];
-    int32_t c[WAVES];
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) c[w] = count[w][b];
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) count[w][b] = c[w] + base;
-  }
-  __syncthreads();
-}
-
-// Up to 16384 positions: one workgroup, in LDS.  Each of 16 waves has a stretch of
-// the positions, 64 at a time.  (More are sorted by several workgroups, below.)
-constexpr int kOneWaves = 16, kOneRounds = 16, kOne = kOneWaves * kOneRounds * kWave;
-
-//
-// One CU sorts and the others have nothing to do: where most rows of the table stay
-// 0 (more rows than positions), the other workgroups write all of it as zeros
-// meanwhile, and only rows with tokens are written after that.  16384 positions take
-// 26 us, of which two passes' ballots are 15; 134 MB of zeros take as long.
-template <int BITS>
-__global__ __launch_bounds__(kOneWaves * kWave) void sort_one(Args a, int rounds, int passes, int32_t *keys,
-                                                              int32_t *places, int64_t zeros) {
-  __shared__ int32_t key[kOne];
-  __shared__ uint16_t place[kOne];
-  __shared__ int32_t count[kOneWaves][kBins], scratch[kBins];
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, M = static_cast<int>(a.M);
-  if (blockIdx.x > 0) {  // `zeros` whole vectors of 16 bytes of the table
-    typedef float vec __attribute__((ext_vector_type(4)));
-    const int64_t step = static_cast<int64_t>(gridDim.x - 1) * (kOneWaves * kWave);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x - 1) * (kOneWaves * kWave) + threadIdx.x; i < zeros; i += step)
-      __builtin_nontemporal_store(vec{0.0f, 0.0f, 0.0f, 0.0f}, static_cast<vec *>(a.to) + i);
-    return;
-  }
-  const int first = wave * rounds * kWave;
-  int32_t k[kOneRounds], p[kOneRounds];
-#pragma unroll
-  for (int r = 0; r < kOneRounds; ++r) {
-    const int i = first + r * kWave + lane;
-    p[r] = i;
-    k[r] = key_of(a, i);
-  }
-  for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * BITS;
-    for (int b = lane; b < kBins; b += kWave) count[wave][b] = 0;
-    // each item's place among the wave's of its digit
-    int32_t local[kOneRounds];
-#pragma unroll
-    for (int r = 0; r < kOneRounds; ++r) {
-      local[r] = 0;
-      if (r < rounds)
-        local[r] = place_in_wave<BITS>(count[wave], k[r] >> shift & ((1 << BITS) - 1), first + r * kWave + lane < M);
-    }
-    __syncthreads();
-    offsets<kOneWaves>(count, scratch);
-#pragma unroll
-    for (int r = 0; r < kOneRounds; ++r) {
-      if (r < rounds && first + r * kWave + lane < M) {
-        const int to = count[wave][k[r] >> shift & ((1 << BITS) - 1)] + local[r];
-        key[to] = k[r];
-        place[to] = static_cast<uint16_t>(p[r]);
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kOneRounds; ++r) {
-      const int i = first + r * kWave + lane;  // (what is not there is not looked at)
-      k[r] = key[i];
-      p[r] = place[i];
-    }
-  }
-  // (64 places of 64 lines would take a store 64 turns)
-#pragma unroll
-  for (int r = 0; r < kOneRounds; ++r) {
-    const int i = first + r * kWave + lane;
-    if (r < rounds && i < M) {
-      keys[i] = k[r];
-      places[i] = p[r];
-    }
-  }
-}
-
-// More positions: each workgroup has a stretch, in turns of kTurn.  Its counts of
-// the bins, the offsets of all counts, and each position to its place.
-constexpr int kSortWaves = 4, kSortRounds = 16, kTurn = kSortWaves * kSortRounds * kWave;
+// Each workgroup has a stretch of the positions, in turns of kTurn.  A pass over a
+// digit: its counts of the bins, the offsets of all counts, and each position to its
+// place.  (16 waves of a turn of 64 each: the ballots are what takes the time.  Waves of 4
+// turns: 131072 positions of [2000, 256] bf16 49 -> 59 us.  Up to 16384 positions in one
+// workgroup's LDS, in one launch: [10000, 256] 32 -> 40.)
+constexpr int kSortWaves = 16, kTurn = kSortWaves * kWave, kSortThreads = kTurn;
 
 // Up to this many workgroups add all counts up themselves; more have it done for
-// them.  131072 positions, [2000, 256] bf16: 103 -> 71 us, with two passes of 6 bits in
-// place of 9.
-constexpr int kDirect = 64;
+// them.  128 of them, [2000, 256] bf16: 49 us, 52 with the launch that does it.
+constexpr int kDirect = 128, kMostBlocks = 512;
 
 struct Sort {
   Args a;
   const int32_t *from_keys, *from_places;  // null: the tokens
-  int32_t *to_keys, *to_places, *counts;   // counts [blocks, bins] if direct, else [bins, blocks]
+  int32_t *to_keys, *to_places;
+  int32_t *counts;  // [blocks, bins] if direct, else [bins, blocks] and the bins' sums
   int blocks, shift;
   bool direct;
   int64_t stretch;  // a multiple of kTurn
@@ -295,40 +180,92 @@ struct Sort {
 };
 
 template <int BITS>
-__global__ __launch_bounds__(kThreads) void sort_count(Sort s) {
+__global__ __launch_bounds__(kSortThreads) void sort_count(Sort s) {
   constexpr int BINS = 1 << BITS;
   __shared__ int32_t count[kSortWaves][BINS];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   for (int b = lane; b < BINS; b += kWave) count[wave][b] = 0;
   const int64_t begin = blockIdx.x * s.stretch, end = begin + s.stretch < s.a.M ? begin + s.stretch : s.a.M;
-  for (int64_t turn = begin; turn < end; turn += kTurn) {
-    const int64_t first = turn + wave * kSortRounds * kWave + lane;
-    int32_t k[kSortRounds];
-#pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) k[r] = s.key(first + r * kWave);
-#pragma unroll
-    for (int r = 0; r < kSortRounds; ++r)
-      place_in_wave<BITS>(count[wave], k[r] >> s.shift & (BINS - 1), first + r * kWave < end);
-  }
+  for (int64_t i = begin + tid; i - tid < end; i += kTurn)
+    place_in_wave<BITS>(count[wave], s.key(i) >> s.shift & (BINS - 1), i < end);
   __syncthreads();
-  for (int b = tid; b < BINS; b += kThreads) {
+  for (int b = tid; b < BINS; b += kSortThreads) {
     int32_t sum = 0;
     for (int w = 0; w < kSortWaves; ++w) sum += count[w][b];
     s.counts[s.direct ? blockIdx.x * BINS + b : static_cast<int64_t>(b) * s.blocks + blockIdx.x] = sum;
   }
 }
 
-// one workgroup: the sums of all counts before each
-__global__ __launch_bounds__(1024) void sort_offsets(int32_t *counts, int64_t n) {
-  __shared__ int32_t sums[16];
+// A wave to a bin: what each workgroup's positions of it come after, and behind all
+// of these the bins' sums.
+template <int BITS>
+__global__ __launch_bounds__(kThreads) void sort_offsets(int32_t *counts, int blocks) {
+  constexpr int BINS = 1 << BITS, EACH = kMostBlocks / kWave;
+  const int lane = threadIdx.x & (kWave - 1), bin = blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave;
+  const int each = (blocks + kWave - 1) / kWave, first = lane * each;
+  int32_t *const of = counts + static_cast<int64_t>(bin) * blocks;
+  int32_t v[EACH], sum = 0;
+#pragma unroll
+  for (int o = 0; o < EACH; ++o) v[o] = of[first + o < blocks ? first + o : blocks - 1];
+#pragma unroll
+  for (int o = 0; o < EACH; ++o) sum += o < each && first + o < blocks ? v[o] : 0;
+  int32_t run = sum;
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int32_t up = __shfl_up(run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == kWave - 1) counts[static_cast<int64_t>(BINS) * blocks + bin] = run;
+  run -= sum;
+#pragma unroll
+  for (int o = 0; o < EACH; ++o) {
+    if (o < each && first + o < blocks) of[first + o] = run;
+    run += v[o];
+  }
+}
+
+template <int BITS>
+__global__ __launch_bounds__(kSortThreads) void sort_place(Sort s) {
+  constexpr int BINS = 1 << BITS;
+  __shared__ int32_t count[kSortWaves][BINS], next[BINS];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  constexpr int EACH = 8;
-  int32_t base = 0;
-  for (int64_t at = 0; at < n; at += 1024 * EACH) {
+  // what comes before this workgroup's: all smaller digits, and equal ones of earlier
+  // workgroups
+  if (s.direct) {
+    constexpr int GROUPS = kSortThreads / BINS < kSortWaves / 2 ? kSortThreads / BINS : kSortWaves / 2;
+    const int b = tid % BINS, group = tid / BINS, each = (s.blocks + GROUPS - 1) / GROUPS;
+    const int last = (group + 1) * each < s.blocks ? (group + 1) * each : s.blocks;
+    if (group < GROUPS) {
+      int32_t all = 0, earlier = 0;
+#pragma unroll 8
+      for (int o = group * each; o < last; ++o) {
+        const int32_t c = s.counts[o * BINS + b];
+        all += c;
+        earlier += o < static_cast<int>(blockIdx.x) ? c : 0;
+      }
+      count[2 * group][b] = all;
+      count[2 * group + 1][b] = earlier;
+    }
+    __syncthreads();
+    if (tid < BINS) {
+      int32_t total = 0, before = 0;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        total += count[2 * g][tid];
+        before += count[2 * g + 1][tid];
+      }
+      count[0][tid] = total;
+      next[tid] = before;
+    }
+  } else if (tid < BINS) {
+    next[tid] = s.counts[static_cast<int64_t>(tid) * s.blocks + blockIdx.x];
+    count[0][tid] = s.counts[static_cast<int64_t>(BINS) * s.blocks + tid];
+  }
+  __syncthreads();
+  if (wave == 0) {
+    constexpr int EACH = BINS / kWave;
     int32_t v[EACH], sum = 0;
-    const int64_t mine = at + tid * EACH;
     for (int o = 0; o < EACH; ++o) {
-      v[o] = mine + o < n ? counts[mine + o] : 0;
+      v[o] = count[0][lane * EACH + o];
       sum += v[o];
     }
     int32_t run = sum;
@@ -336,79 +273,24 @@ __global__ __launch_bounds__(1024) void sort_offsets(int32_t *counts, int64_t n)
       const int32_t up = __shfl_up(run, o);
       if (lane >= o) run += up;
     }
-    __syncthreads();
-    if (lane == kWave - 1) sums[wave] = run;
-    __syncthreads();
-    int32_t total = 0;
-    run += base - sum;
-    for (int w = 0; w < 16; ++w) {
-      if (w < wave) run += sums[w];
-      total += sums[w];
-    }
+    run -= sum;
     for (int o = 0; o < EACH; ++o) {
-      if (mine + o < n) counts[mine + o] = run;
+      next[lane * EACH + o] += run;
       run += v[o];
     }
-    base += total;
   }
-}
-
-template <int BITS>
-__global__ __launch_bounds__(kThreads) void sort_place(Sort s) {
-  constexpr int BINS = 1 << BITS;
-  __shared__ int32_t count[kSortWaves][BINS], next[BINS];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  if (s.direct) {
-    // what comes before this workgroup's: all smaller digits, and equal ones of
-    // earlier workgroups
-    for (int b = tid; b < BINS; b += kThreads) {
-      int32_t all = 0, earlier = 0;
-#pragma unroll 8
-      for (int o = 0; o < s.blocks; ++o) {
-        const int32_t c = s.counts[o * BINS + b];
-        all += c;
-        earlier += o < static_cast<int>(blockIdx.x) ? c : 0;
-      }
-      next[b] = earlier;
-      count[0][b] = all;
-    }
-    __syncthreads();
-    if (wave == 0) {
-      constexpr int EACH = (BINS + kWave - 1) / kWave;
-      int32_t v[EACH], sum = 0;
-      for (int o = 0; o < EACH; ++o) {
-        v[o] = count[0][lane * EACH + o];
-        sum += v[o];
-      }
-      int32_t run = sum;
-      for (int o = 1; o < kWave; o <<= 1) {
-        const int32_t up = __shfl_up(run, o);
-        if (lane >= o) run += up;
-      }
-      run -= sum;
-      for (int o = 0; o < EACH; ++o) {
-        next[lane * EACH + o] += run;
-        run += v[o];
-      }
-    }
-    __syncthreads();
-  } else {
-    for (int b = tid; b < BINS; b += kThreads) next[b] = s.counts[static_cast<int64_t>(b) * s.blocks + blockIdx.x];
-  }
+  __syncthreads();
   const int64_t begin = blockIdx.x * s.stretch, end = begin + s.stretch < s.a.M ? begin + s.stretch : s.a.M;
   for (int64_t turn = begin; turn < end; turn += kTurn) {
-    const int64_t first = turn + wave * kSortRounds * kWave + lane;
-    int32_t k[kSortRounds];
+    const int64_t i = turn + tid;
+    const int32_t k = s.key(i);
+    const int digit = k >> s.shift & (BINS - 1);
     for (int b = lane; b < BINS; b += kWave) count[wave][b] = 0;
-#pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) k[r] = s.key(first + r * kWave);
-    int32_t local[kSortRounds];
-#pragma unroll
-    for (int r = 0; r < kSortRounds; ++r)
-      local[r] = place_in_wave<BITS>(count[wave], k[r] >> s.shift & (BINS - 1), first + r * kWave < end);
+    const int32_t local = place_in_wave<BITS>(count[wave], digit, i < end);
     __syncthreads();
-    for (int b = tid; b < BINS; b += kThreads) {
+    for (int b = tid; b < BINS; b += kSortThreads) {
       int32_t run = next[b];
+#pragma unroll
       for (int w = 0; w < kSortWaves; ++w) {
         const int32_t c = count[w][b];
         count[w][b] = run;
@@ -417,14 +299,10 @@ __global__ __launch_bounds__(kThreads) void sort_place(Sort s) {
       next[b] = run;
     }
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSortRounds; ++r) {
-      const int64_t i = first + r * kWave;
-      if (i < end) {
-        const int32_t to = count[wave][k[r] >> s.shift & (BINS - 1)] + local[r];
-        s.to_keys[to] = k[r];
-        s.to_places[to] = s.place(i);
-      }
+    if (i < end) {
+      const int32_t to = count[wave][digit] + local;
+      s.to_keys[to] = k;
+      s.to_places[to] = s.place(i);
     }
     __syncthreads();
   }
@@ -488,8 +366,8 @@ __device__ __forceinline__ void join(float *red, int groups, int group, int per,
 }
 
 // The pieces of the sorted positions that one token has, a workgroup each (and
-// slice); the workgroups after them find where each token's positions start.  5 us:
-// of latency, one after the other.
+// slice); the workgroups after them find where each token's positions start.  7 us:
+// of latency.  (A search among keys in LDS first changes nothing.)
 template <class E, int VEC>
 __global__ __launch_bounds__(kThreads) void sum_whole_pieces(Args a, int per, int64_t blocks, int32_t *starts) {
   __shared__ float red[kThreads * VEC];
@@ -543,14 +421,14 @@ __global__ __launch_bounds__(kThreads) void sum_larger_pieces(Args a, int per) {
 }
 
 // Each row of the table: what of its run is before the first whole piece, the whole
-// pieces (the larger ones among them), what is behind them.  ZEROED: rows without
-// positions are there already (16384 positions of [32768, 2048] bf16: 24 us, where
-// writing the zeros as well took 46; the rows of frequent tokens are the last to end).
-// ROWS of a group of threads: 1 where the table is
-// small, so that its rows with many positions do not wait for each other.
+// pieces (the larger ones among them), what is behind them.  ROWS of a group of threads:
+// 1 where the table is small, so that its rows with many positions do not wait for each
+// other.  16384 positions of [32768, 2048] bf16: 35 us (201 MB, 5.7 TB/s).  (Zeros that the
+// sort's launches write on CUs that it leaves free, and only rows with positions here: 5
+// us more in all.)
 constexpr int kTableRows = 4;
 
-template <class E, int VEC, int ROWS, bool STREAM, bool ZEROED>
+template <class E, int VEC, int ROWS, bool STREAM>
 __global__ __launch_bounds__(kThreads) void sum_runs(Args a, int per) {
   using T = typename E::T;
   const int groups = kThreads / per, group = threadIdx.x / per;
@@ -564,7 +442,6 @@ __global__ __launch_bounds__(kThreads) void sum_runs(Args a, int per) {
   for (int o = 0; o < ROWS; ++o) {
     const int64_t v = first + o, lo = start[o], hi = start[o + 1];
     if (v >= a.V) return;
-    if (ZEROED && lo == hi) continue;
     Vector<E, VEC> r;
     r.zero();
     const int64_t p0 = (lo + kPiece - 1) / kPiece, p1 = hi / kPiece;
@@ -645,7 +522,7 @@ __global__ __launch_bounds__(kThreads) void zeros(Args a) {
 
 // ---- launches ---------------------------------------------------------------
 struct Layout {  // of the workspace, in bytes
-  bool few, one;
+  bool few;
   int passes, bits, blocks;
   int64_t stretch, keys[2], places[2], counts, starts, pieces, pieces2, size;
 };
@@ -658,7 +535,6 @@ Layout layout_of(int64_t M, int64_t V, int64_t D) {
   Layout l{};
   l.few = M <= kFew && V * ((D + 63) / 64) <= kFewRows;
   if (l.few || M == 0) return l;
-  l.one = M <= kOne;
   int bits = 1;
   while (V >> bits) ++bits;
   l.passes = (bits + kDigit - 1) / kDigit;
@@ -669,21 +545,19 @@ Layout layout_of(int64_t M, int64_t V, int64_t D) {
     at += (bytes + 15) / 16 * 16;
     return here;
   };
-  for (int o = 0; o < (l.one ? 1 : 2); ++o) {
+  for (int o = 0; o < 2; ++o) {
     l.keys[o] = take(4 * M);
     l.places[o] = take(4 * M);
   }
-  if (!l.one) {
-    // up to 1024 workgroups, of whole turns
-    const int64_t turns = (M + kTurn - 1) / kTurn, each = (turns + 1023) / 1024;
-    l.stretch = each * kTurn;
-    l.blocks = static_cast<int>((M + l.stretch - 1) / l.stretch);
-    l.counts = take(4 * static_cast<int64_t>(kBins) * l.blocks);
-  }
+  // workgroups of whole turns
+  const int64_t turns = (M + kTurn - 1) / kTurn, each = (turns + kMostBlocks - 1) / kMostBlocks;
+  l.stretch = each * kTurn;
+  l.blocks = static_cast<int>((M + l.stretch - 1) / l.stretch);
+  l.counts = take(4 * static_cast<int64_t>(kBins) * (l.blocks + 1));
   l.starts = take(4 * (V + 1));
   l.pieces = take(4 * (M / kPiece) * D);
   // (a run of 16384 has 512 pieces: few enough to add up at once)
-  l.pieces2 = l.one ? -1 : take(4 * (M / (kPiece * kPiece)) * D);
+  l.pieces2 = M <= 16384 ? -1 : take(4 * (M / (kPiece * kPiece)) * D);
   l.size = at;
   return l;
 }
@@ -703,9 +577,9 @@ void launch_lookup(Args &a, hipStream_t s) {
 
 template <int BITS>
 void launch_sort(const Sort &t, hipStream_t s) {
-  sort_count<BITS><<<t.blocks, kThreads, 0, s>>>(t);
-  if (!t.direct) sort_offsets<<<1, 1024, 0, s>>>(t.counts, (int64_t{1} << BITS) * t.blocks);
-  sort_place<BITS><<<t.blocks, kThreads, 0, s>>>(t);
+  sort_count<BITS><<<t.blocks, kSortThreads, 0, s>>>(t);
+  if (!t.direct) sort_offsets<BITS><<<(1 << BITS) / (kThreads / kWave), kThreads, 0, s>>>(t.counts, t.blocks);
+  sort_place<BITS><<<t.blocks, kSortThreads, 0, s>>>(t);
 }
 
 template <class E, int VEC>
@@ -726,32 +600,18 @@ void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
   a.pieces2 = l.pieces2 < 0 ? nullptr : reinterpret_cast<float *>(ws + l.pieces2);
   const auto words = [&](int64_t at) { return reinterpret_cast<int32_t *>(ws + at); };
   const int64_t bytes = a.V * a.D * static_cast<int64_t>(sizeof(typename E::T));
-  const bool zeroed = l.one && a.V > a.M && bytes % 16 == 0 && myelin::aligned(a.to, 16);
-  if (l.one) {
-    // (workgroups of 256 KB: a CU has one at a time)
-    const int64_t zeros = zeroed ? bytes / 16 : 0, fill = (zeros + 16383) / 16384;
-    const unsigned grid = static_cast<unsigned>(1 + (fill < 4096 ? fill : 4096));
-    const int rounds = static_cast<int>((a.M + kOneWaves * kWave - 1) / (kOneWaves * kWave));
-    if (l.bits <= 8)
-      sort_one<8><<<grid, kOneWaves * kWave, 0, s>>>(a, rounds, l.passes, words(l.keys[0]), words(l.places[0]), zeros);
+  const int digit = l.bits <= 6 ? 6 : l.bits <= 8 ? 8 : 9;
+  for (int pass = 0; pass < l.passes; ++pass) {
+    const Sort t{a, pass ? a.keys : nullptr, pass ? a.places : nullptr, words(l.keys[pass & 1]), words(l.places[pass & 1]),
+           words(l.counts), l.blocks, pass * digit, l.blocks <= kDirect, l.stretch};
+    if (digit == 6)
+      launch_sort<6>(t, s);
+    else if (digit == 8)
+      launch_sort<8>(t, s);
     else
-      sort_one<9><<<grid, kOneWaves * kWave, 0, s>>>(a, rounds, l.passes, words(l.keys[0]), words(l.places[0]), zeros);
-    a.keys = words(l.keys[0]);
-    a.places = words(l.places[0]);
-  } else {
-    const int digit = l.bits <= 6 ? 6 : l.bits <= 8 ? 8 : 9;
-    for (int pass = 0; pass < l.passes; ++pass) {
-      Sort t{a, pass ? a.keys : nullptr, pass ? a.places : nullptr, words(l.keys[pass & 1]), words(l.places[pass & 1]),
-             words(l.counts), l.blocks, pass * digit, l.blocks <= kDirect, l.stretch};
-      if (digit == 6)
-        launch_sort<6>(t, s);
-      else if (digit == 8)
-        launch_sort<8>(t, s);
-      else
-        launch_sort<9>(t, s);
-      a.keys = t.to_keys;
-      a.places = t.to_places;
-    }
+      launch_sort<9>(t, s);
+    a.keys = t.to_keys;
+    a.places = t.to_places;
   }
   int per = threads_of(a.units, kWave);
   a.slices = (a.units + per - 1) / per;
@@ -765,17 +625,14 @@ void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
   const int64_t groups = kThreads / per;
   const auto grid = [&](int64_t rows) { return myelin::grid_of((a.V + rows - 1) / rows * a.slices); };
   const bool stream = bytes >= myelin::kStreamBytes;
-  // 131072 positions, [2000, 256] bf16: 127 us with 4 rows a group, 110 with 2
-  if (!zeroed && !stream && a.V / groups * a.slices < 4096)
-    sum_runs<E, VEC, 1, false, false><<<grid(groups), kThreads, 0, s>>>(a, per);
-  else if (zeroed && stream)
-    sum_runs<E, VEC, kTableRows, true, true><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
-  else if (zeroed)
-    sum_runs<E, VEC, kTableRows, false, true><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
+  // with 4 rows a group: 131072 positions of [2000, 256] bf16 49 -> 72 us, 2^20 of
+  // [32000, 32] 111 -> 150; with 1: 57049 rows of 73 66 -> 98, of [32768, 2048] 54 -> 64
+  if (!stream && a.V / groups * a.slices < 4096)
+    sum_runs<E, VEC, 1, false><<<grid(groups), kThreads, 0, s>>>(a, per);
   else if (stream)
-    sum_runs<E, VEC, kTableRows, true, false><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
+    sum_runs<E, VEC, kTableRows, true><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
   else
-    sum_runs<E, VEC, kTableRows, false, false><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
+    sum_runs<E, VEC, kTableRows, false><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
 }
 
 int check(const char *what, int dtype, int64_t M, int64_t V, int64_t D, float scale) {

@@ -17,3 +17,11 @@ def test_nothing_is_spilled(kernels):  # noqa: F811
     assert not spilled, spilled
     tight = [k for n, k in found.items() if any(name in n for name in NAMES[:4])]
     assert len(tight) >= 8 and all(k[".vgpr_count"] <= 128 for k in tight)
+
+
+def test_sorts_fit_two_workgroups(kernels):  # noqa: F811
+    found = {n: k for n, k in kernels.items() if "10sort_countI" in n or "10sort_placeI" in n}
+    assert len(found) == 6
+    for n, k in found.items():
+        assert k[".vgpr_count"] <= 64 and not k[".vgpr_spill_count"], (n, k[".vgpr_count"])
+        assert k[".group_segment_fixed_size"] <= 80 * 1024, n

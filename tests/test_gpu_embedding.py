@@ -250,3 +250,24 @@ def test_module():
     assert torch.equal(y.detach(), _want(t, m.weight, 2.0, 0))
     y.sum().backward()
     assert torch.equal(m.weight.grad[5], torch.full((8,), 4.0, device=DEV)) and not bool(m.weight.grad[0].any())
+
+
+@pytest.mark.parametrize("V", [40, 300, 40000, 70000])
+@pytest.mark.parametrize("M", [4097, 131072, 131073, 524289, 1500000])
+def test_positions_of_many_workgroups(M, V):
+    """Sorts by digits of 6, 8 and 9 bits, by up to 128 workgroups, by more and in
+    several turns of each.  Whole numbers: their sums are exact, in any order."""
+
+    _case(test="embedding_many", M=M, V=V)
+    g = torch.Generator().manual_seed(M + V)
+    spread = torch.rand(M, generator=g)
+    tokens = (V * spread**3).long().clamp(max=V - 1)  # small ones more often
+    tokens[torch.randint(0, M, (M // 50,), generator=g)] = 2  # padding
+    tokens[torch.randint(0, M, (9,), generator=g)] = V  # outside
+    gy = torch.randint(-3, 4, (M, 2), generator=g).float()
+    want = torch.zeros(V, 2, dtype=torch.float64)
+    counted = (tokens < V) & (tokens != 2)
+    want.index_add_(0, tokens[counted], gy[counted].double())
+    assert float(torch.bincount(tokens).max()) * 3 < 2**24
+    gw = _grad(tokens.to(DEV), torch.zeros(V, 2, device=DEV), gy.to(DEV), padding_index=2)
+    assert torch.equal(gw.cpu().double(), want)
