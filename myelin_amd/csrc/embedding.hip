@@ -163,17 +163,20 @@ __device__ __forceinline__ int32_t place_in_wave(int32_t *count, int digit, bool
 // workgroup's LDS, in one launch: [10000, 256] 32 -> 40.)
 constexpr int kSortWaves = 16, kTurn = kSortWaves * kWave, kSortThreads = kTurn;
 
-// Up to this many workgroups add all counts up themselves; more have it done for
-// them.  128 of them, [2000, 256] bf16: 49 us, 52 with the launch that does it.
-constexpr int kDirect = 128, kMostBlocks = 512;
+// Up to kAlone workgroups count all positions themselves: no launch before that (8192
+// positions 28 us either way, 16384 6 us more).  Up to kDirect add up all workgroups'
+// counts; more have it done for them (128 of them, [2000, 256] bf16: 49 us, 52 with the
+// launch that does it).
+constexpr int kAlone = 8, kDirect = 128, kMostBlocks = 512;
+enum Counts { kOwn, kOthers, kSums };
 
 struct Sort {
   Args a;
   const int32_t *from_keys, *from_places;  // null: the tokens
   int32_t *to_keys, *to_places;
-  int32_t *counts;  // [blocks, bins] if direct, else [bins, blocks] and the bins' sums
+  int32_t *counts;  // kOthers: [blocks, bins]; kSums: [bins, blocks] and the bins' sums
   int blocks, shift;
-  bool direct;
+  Counts which;
   int64_t stretch;  // a multiple of kTurn
   __device__ int32_t key(int64_t i) const { return from_keys ? from_keys[i < a.M ? i : a.M - 1] : key_of(a, i); }
   __device__ int32_t place(int64_t i) const { return from_keys ? from_places[i] : static_cast<int32_t>(i); }
@@ -192,7 +195,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_count(Sort s) {
   for (int b = tid; b < BINS; b += kSortThreads) {
     int32_t sum = 0;
     for (int w = 0; w < kSortWaves; ++w) sum += count[w][b];
-    s.counts[s.direct ? blockIdx.x * BINS + b : static_cast<int64_t>(b) * s.blocks + blockIdx.x] = sum;
+    s.counts[s.which == kOthers ? blockIdx.x * BINS + b : static_cast<int64_t>(b) * s.blocks + blockIdx.x] = sum;
   }
 }
 
@@ -230,7 +233,34 @@ __global__ __launch_bounds__(kSortThreads) void sort_place(Sort s) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
   // what comes before this workgroup's: all smaller digits, and equal ones of earlier
   // workgroups
-  if (s.direct) {
+  if (s.which == kOwn) {  // (whole numbers: the order of the atomics does not show)
+    for (int b = tid; b < 2 * BINS; b += kSortThreads) count[b / BINS][b % BINS] = 0;
+    __syncthreads();
+    constexpr int MANY = 8;
+    for (int turn = 0; turn < s.blocks; turn += MANY) {
+      int digit[MANY];
+#pragma unroll
+      for (int o = 0; o < MANY; ++o)
+        digit[o] = s.key(static_cast<int64_t>(turn + o) * kTurn + tid) >> s.shift & (BINS - 1);
+#pragma unroll
+      for (int o = 0; o < MANY; ++o) {
+        int32_t *const to = count[turn + o < static_cast<int>(blockIdx.x)];
+        const bool in = static_cast<int64_t>(turn + o) * kTurn + tid < s.a.M;
+        // (one token in all lanes: they would wait for each other)
+        const int first = __builtin_amdgcn_readfirstlane(digit[o]);
+        if (__all(in && digit[o] == first)) {
+          if (lane == 0) atomicAdd(to + first, kWave);
+        } else if (in) {
+          atomicAdd(to + digit[o], 1);
+        }
+      }
+    }
+    __syncthreads();
+    if (tid < BINS) {
+      next[tid] = count[1][tid];
+      count[0][tid] += count[1][tid];
+    }
+  } else if (s.which == kOthers) {
     constexpr int GROUPS = kSortThreads / BINS < kSortWaves / 2 ? kSortThreads / BINS : kSortWaves / 2;
     const int b = tid % BINS, group = tid / BINS, each = (s.blocks + GROUPS - 1) / GROUPS;
     const int last = (group + 1) * each < s.blocks ? (group + 1) * each : s.blocks;
@@ -467,17 +497,20 @@ __global__ __launch_bounds__(kThreads) void sum_runs(Args a, int per) {
 // ---- gradient: few tokens, small tables -------------------------------------
 // A workgroup to a row (and slice): it goes through all tokens itself, keeps the
 // positions of its own in order, and sums their rows.  No sort, one launch: 2048
-// tokens of [50, 128] fp32 6.6 us, latency.
-constexpr int kFewThreads = 512, kFew = 4096;
+// tokens of [50, 128] fp32 6.6 us, latency.  Tables of more rows are zeros first, and a
+// workgroup has a position, and its token's row if no earlier position has.
+constexpr int kFewThreads = 512, kFew = 4096;  // (kFewPositions is less)
 
-template <class E, int VEC>
+template <class E, int VEC, bool POSITIONS>
 __global__ __launch_bounds__(kFewThreads) void sum_few(Args a, int per) {
   using T = typename E::T;
   __shared__ int32_t list[kFew];
   __shared__ int found[kFew / kFewThreads][kFewThreads / kWave];
   __shared__ float red[kFewThreads * VEC];
   const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-  const int64_t block = myelin::block_id(), v = block / a.slices, slice = block - v * a.slices;
+  const int64_t block = myelin::block_id(), unit = block / a.slices, slice = block - unit * a.slices;
+  const int64_t v = POSITIONS ? key_of(a, unit) : unit;
+  if (POSITIONS && (unit >= a.M || v == a.V)) return;  // the whole workgroup
   constexpr int ROUNDS = kFew / kFewThreads, WAVES = kFewThreads / kWave;
   uint64_t hit[ROUNDS];
 #pragma unroll
@@ -497,6 +530,7 @@ __global__ __launch_bounds__(kFewThreads) void sum_few(Args a, int per) {
     if (hit[o] >> lane & 1) list[before + lower(hit[o])] = o * kFewThreads + tid;
   }
   __syncthreads();
+  if (POSITIONS && list[0] != unit) return;
   const int groups = kFewThreads / per, group = tid / per, at = tid % per;
   const int64_t u = slice * per + at;
   const int each = (n + groups - 1) / groups, from = group * each < n ? group * each : n,
@@ -530,6 +564,11 @@ struct Layout {  // of the workspace, in bytes
 // Rows of the table times slices that sum_few is taken for: each goes through all
 // tokens.
 constexpr int64_t kFewRows = 2048;
+
+// Positions times slices of 128 threads (so that a group of threads has at most 512 rows,
+// if all are one token's) that it is taken for elsewhere, against the sort: 60 of [5407, 26]
+// bf16 16 -> 6 us, 1024 of [32000, 512] 27 -> 16, 2048 30 -> 23, 4096 32 -> 42.
+constexpr int64_t kFewPositions = 2048;
 
 Layout layout_of(int64_t M, int64_t V, int64_t D) {
   Layout l{};
@@ -577,22 +616,27 @@ void launch_lookup(Args &a, hipStream_t s) {
 
 template <int BITS>
 void launch_sort(const Sort &t, hipStream_t s) {
-  sort_count<BITS><<<t.blocks, kSortThreads, 0, s>>>(t);
-  if (!t.direct) sort_offsets<BITS><<<(1 << BITS) / (kThreads / kWave), kThreads, 0, s>>>(t.counts, t.blocks);
+  if (t.which != kOwn) sort_count<BITS><<<t.blocks, kSortThreads, 0, s>>>(t);
+  if (t.which == kSums) sort_offsets<BITS><<<(1 << BITS) / (kThreads / kWave), kThreads, 0, s>>>(t.counts, t.blocks);
   sort_place<BITS><<<t.blocks, kSortThreads, 0, s>>>(t);
 }
 
 template <class E, int VEC>
 void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
   a.units = a.D / VEC;
-  if (a.M == 0) {
+  const auto zero = [&] {
     zeros<E, VEC><<<myelin::grid_of((a.V * a.units + kThreads - 1) / kThreads), kThreads, 0, s>>>(a);
+  };
+  if (a.M == 0) return zero();
+  const int some = threads_of(a.units, l.few ? kWave : 2 * kWave);
+  a.slices = (a.units + some - 1) / some;
+  if (l.few) {
+    sum_few<E, VEC, false><<<myelin::grid_of(a.V * a.slices), kFewThreads, 0, s>>>(a, some);
     return;
   }
-  if (l.few) {
-    const int per = threads_of(a.units, kWave);
-    a.slices = (a.units + per - 1) / per;
-    sum_few<E, VEC><<<myelin::grid_of(a.V * a.slices), kFewThreads, 0, s>>>(a, per);
+  if (a.M * a.slices <= kFewPositions) {
+    zero();
+    sum_few<E, VEC, true><<<myelin::grid_of(a.M * a.slices), kFewThreads, 0, s>>>(a, some);
     return;
   }
   a.starts = reinterpret_cast<int32_t *>(ws + l.starts);
@@ -601,9 +645,18 @@ void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
   const auto words = [&](int64_t at) { return reinterpret_cast<int32_t *>(ws + at); };
   const int64_t bytes = a.V * a.D * static_cast<int64_t>(sizeof(typename E::T));
   const int digit = l.bits <= 6 ? 6 : l.bits <= 8 ? 8 : 9;
+  const Counts which = l.blocks <= kAlone ? kOwn : l.blocks <= kDirect ? kOthers : kSums;
   for (int pass = 0; pass < l.passes; ++pass) {
-    const Sort t{a, pass ? a.keys : nullptr, pass ? a.places : nullptr, words(l.keys[pass & 1]), words(l.places[pass & 1]),
-           words(l.counts), l.blocks, pass * digit, l.blocks <= kDirect, l.stretch};
+    const Sort t{a,
+                 pass ? a.keys : nullptr,
+                 pass ? a.places : nullptr,
+                 words(l.keys[pass & 1]),
+                 words(l.places[pass & 1]),
+                 words(l.counts),
+                 l.blocks,
+                 pass * digit,
+                 which,
+                 l.stretch};
     if (digit == 6)
       launch_sort<6>(t, s);
     else if (digit == 8)

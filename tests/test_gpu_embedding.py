@@ -271,3 +271,39 @@ def test_positions_of_many_workgroups(M, V):
     assert float(torch.bincount(tokens).max()) * 3 < 2**24
     gw = _grad(tokens.to(DEV), torch.zeros(V, 2, device=DEV), gy.to(DEV), padding_index=2)
     assert torch.equal(gw.cpu().double(), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,V,D", [(1, 5000, 3), (33, 2049, 64), (60, 5407, 26), (511, 4102, 73), (700, 9000, 640),
+                                   (1023, 2200, 1001), (2048, 40000, 16), (2049, 40000, 16), (3000, 2500, 130)])
+def test_few_positions_of_a_large_table(M, V, D, dtype):
+    """A workgroup to a position, beside the sort of a few more: whole numbers, whose
+    sums are exact and round once."""
+
+    _case(test="embedding_positions", M=M, V=V, D=D, dtype=dtype)
+    g = torch.Generator().manual_seed(M + V + D)
+    for tokens in (torch.randint(0, V, (M,), generator=g), torch.randint(0, 9, (M,), generator=g) * (V // 9),
+                   torch.full((M,), V - 1), torch.arange(M).flip(0) % V):
+        tokens = tokens.clone()
+        tokens[M // 2] = 3  # padding
+        tokens[M // 3] = -1
+        gy = torch.randint(-2, 3, (M, D), generator=g).to(DTYPES[dtype])
+        want = torch.zeros(V, D, dtype=torch.float64)
+        counted = (tokens >= 0) & (tokens != 3)
+        want.index_add_(0, tokens[counted], gy[counted].double())
+        gw = _grad(tokens.to(DEV), torch.zeros(V, D, dtype=DTYPES[dtype], device=DEV), gy.to(DEV), padding_index=3)
+        assert torch.equal(gw.cpu(), want.to(DTYPES[dtype]))
+
+
+@pytest.mark.parametrize("V,width", [(5000, 1), (5000, 8), (300, 300)])
+def test_the_order_is_kept_in_larger_tables(V, width):
+    big = 2.0**24
+    values = torch.tensor([big, 1.0, -big, 1.0])
+    for gap in (0, 3, 200, 500, 3000, 40000):
+        M = 4 + 4 * gap
+        tokens = torch.arange(M) % (V - 10) + 6
+        gy = torch.zeros(M, width)
+        for i in range(4):
+            tokens[i * (gap + 1)], gy[i * (gap + 1)] = 5, values[i]
+        gw = _grad(tokens.to(DEV), torch.zeros(V, width, device=DEV), gy.to(DEV))
+        assert bool((gw[5] == 1.0).all()), gap
