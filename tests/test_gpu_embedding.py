@@ -13,6 +13,7 @@ import pytest
 import torch
 
 import myelin_amd as myelin
+from myelin_amd import _lib
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -307,3 +308,41 @@ def test_the_order_is_kept_in_larger_tables(V, width):
             tokens[i * (gap + 1)], gy[i * (gap + 1)] = 5, values[i]
         gw = _grad(tokens.to(DEV), torch.zeros(V, width, device=DEV), gy.to(DEV))
         assert bool((gw[5] == 1.0).all()), gap
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,V,D", [(70, 30, 9), (300, 50, 17), (2500, 3001, 33), (5000, 1000, 301), (9, 7, 8)])
+def test_rows_that_start_anywhere(M, V, D, dtype):
+    """Tables and gradients that start one element behind 16 bytes, rows of odd widths
+    and strides: what is beside them is neither read into results nor written."""
+
+    _case(test="embedding_anywhere", M=M, V=V, D=D, dtype=dtype)
+    g = torch.Generator().manual_seed(M + V + D)
+    dt = DTYPES[dtype]
+    base = torch.full((V * (D + 2) + 1,), math.nan, dtype=dt, device=DEV)
+    weight = base[1:].view(V, D + 2)[:, :D]
+    weight.copy_(torch.randn(V, D, generator=g))
+    tokens = torch.randint(0, V, (M,), generator=g)
+    y = myelin.token_embedding(tokens.to(DEV), weight, scale=0.5)
+    assert torch.equal(y, _want(tokens.to(DEV), weight, 0.5, None))
+    behind = torch.full((M * D + 1,), math.nan, dtype=dt, device=DEV)
+    gy = behind[1:].view(M, D)
+    gy.copy_(torch.randint(-2, 3, (M, D), generator=g))
+    want = torch.zeros(V, D, dtype=torch.float64)
+    want.index_add_(0, tokens, gy.cpu().double())
+    gw = _grad(tokens.to(DEV), weight, gy, scale=1.0)
+    assert torch.equal(gw.cpu(), want.to(dt))
+    # the entry points write no more than their rows
+    lib_out = torch.full((M * D + 2,), 7.0, dtype=dt, device=DEV)
+    grad_out = torch.full((V * D + 2,), 7.0, dtype=dt, device=DEV)
+    on = tokens.to(DEV)
+    need = _lib.load().myelin_token_embedding_bwd_workspace_bytes(M, V, D)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    size, s = lib_out.element_size(), torch.cuda.current_stream().cuda_stream
+    _lib.call("myelin_token_embedding", on.data_ptr(), weight.data_ptr(), _lib.DT[dt], D + 2, lib_out.data_ptr() + size,
+              M, V, D, 0.5, -(2**63), s)
+    _lib.call("myelin_token_embedding_bwd", on.data_ptr(), gy.data_ptr(), _lib.DT[dt], grad_out.data_ptr() + size, M, V,
+              D, 1.0, -(2**63), ws.data_ptr(), need, s)
+    assert torch.equal(lib_out[1:-1].view(M, D), y) and torch.equal(grad_out[1:-1].view(V, D), gw)
+    for t in (lib_out, grad_out):
+        assert float(t[0]) == 7.0 and float(t[-1]) == 7.0
