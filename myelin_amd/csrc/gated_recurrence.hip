@@ -23,6 +23,7 @@ using myelin::F32;
 constexpr int kSteps = 16;     // steps of a wave at a time
 constexpr int kBackSteps = 8;  // and in the backward pass; and steps between two kept states
 constexpr int kMaxWaves = 16;
+constexpr int kApart = 4;      // waves of a workgroup whose waves have channels of their own
 constexpr int kWave = myelin::kWave;
 
 struct Affine;
@@ -77,6 +78,7 @@ template <int STEPS>
 struct Place {
   int64_t first;  // the workgroup's first channel, of B * N
   int lane, wave, waves;
+  int base = 0;                    // the first wave's
   int64_t live;                    // the channel's steps
   bool in;
   const char *x, *gate, *out;      // of the first channel's batch row
@@ -90,13 +92,21 @@ struct Place {
     return n < 0 ? 0 : n < STEPS ? static_cast<int>(n) : STEPS;
   }
 
-  template <class T>
+  template <class T, bool APART>
   __device__ void set(const Args &a, int64_t block) {
     lane = threadIdx.x % kWave;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    waves = blockDim.x / kWave;
-    first = block * kWave;
-    in = c() < a.B * a.N;
+    // (one where they are apart; known to the compiler, it takes more addresses into
+    // scalar registers than there are)
+    waves = blockDim.x / (APART ? kApart * kWave : kWave);
+    if (APART) {
+      block = block * kApart + wave;
+      base = wave;
+      wave = 0;
+    }
+    // (behind the last block: the last one, with nothing to do)
+    first = (!APART || block < a.blocks ? block : a.blocks - 1) * kWave;
+    in = (!APART || block < a.blocks) && c() < a.B * a.N;
     const int64_t mine = in ? c() : first;
     const int64_t b0 = first / a.N, b = mine / a.N, n = mine - b * a.N;
     x = reinterpret_cast<const char *>(static_cast<const T *>(a.x) + b0 * a.xb);
@@ -159,27 +169,29 @@ __device__ __forceinline__ float join(const Args &a, int64_t c, float s, int64_t
 // A workgroup's segment and block of channels, or -1.  Consecutive workgroups run on
 // XCDs in turn; each XCD takes a stretch of the (segment, channels), so that blocks
 // that share lines of 128 bytes share an L2.
+template <bool APART>
 __device__ __forceinline__ int64_t locate(Args &a, int64_t segments) {
   constexpr int kXcds = 8;
-  const int64_t id = myelin::block_id(), units = a.blocks * segments, each = (units + kXcds - 1) / kXcds;
+  const int64_t blocks = APART ? (a.blocks + kApart - 1) / kApart : a.blocks, units = blocks * segments;
+  const int64_t id = myelin::block_id(), each = (units + kXcds - 1) / kXcds;
   const int64_t unit = id % kXcds * each + id / kXcds;
   if (id >= each * kXcds || unit >= units) return -1;
-  a.seg = unit / a.blocks;
-  return unit - a.seg * a.blocks;
+  a.seg = unit / blocks;
+  return unit - a.seg * blocks;
 }
 
 // Bound by memory, with the gates' instructions half of the time beside it: [2048, 8,
 // 2048] bf16 48 us with the kept states (218 MB, 4.5 TB/s), 256 workgroups of 16
 // waves, one to a CU.  The next tile's rows are on their way while the waves join.
-template <class E>
+template <class E, bool APART>
 __global__ __launch_bounds__(kMaxWaves * kWave) void forward(Args a) {
   using T = typename E::T;
   using P = Place<kSteps>;
   __shared__ Affine maps[2][kMaxWaves][kWave];
-  const int64_t block = locate(a, a.segments);
+  const int64_t block = locate<APART>(a, a.segments);
   if (block < 0) return;  // the whole workgroup
   P p;
-  p.template set<T>(a, block);
+  p.template set<T, APART>(a, block);
   const int64_t BN = a.B * a.N, first = a.seg * a.seg_steps;
   const int64_t end = first + a.seg_steps < a.T ? first + a.seg_steps : a.T;
   float s = p.in && a.state ? a.state[p.c()] : 0.0f;
@@ -208,15 +220,16 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void forward(Args a) {
       ru[i] = g.b * E::get(x[i]);
       m = {m.A * g.a, __builtin_fmaf(g.a, m.H, ru[i])};
     }
-    maps[turn & 1][p.wave][p.lane] = m;
+    Affine(*const map)[kWave] = &maps[turn & 1][p.base];
+    map[p.wave][p.lane] = m;
     const int mine = n;
     if (tile + p.tile_steps() < end) fetch(tile + p.tile_steps());
-    __syncthreads();
+    if (!APART) __syncthreads();
     float h = s;
 #pragma unroll 4
     for (int o = 0; o < p.waves; ++o) {
       if (o == p.wave) h = s;
-      const Affine q = maps[turn & 1][o][p.lane];
+      const Affine q = map[o][p.lane];
       s = __builtin_fmaf(q.A, s, q.H);
     }
     const int64_t here = p.step(tile);
@@ -245,15 +258,15 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void forward(Args a) {
 // As forward, from the last tile, with three rows in and two out: 84 us (352 MB, 4.2
 // TB/s) for the same.  8 steps of a wave: 16 do not fit 128 registers, and 16 waves of
 // them are a CU's.
-template <class E>
+template <class E, bool APART>
 __global__ __launch_bounds__(kMaxWaves * kWave) void backward(Args a) {
   using T = typename E::T;
   using P = Place<kBackSteps>;
   __shared__ Affine maps[2][kMaxWaves][kWave];
-  const int64_t block = locate(a, a.segments);
+  const int64_t block = locate<APART>(a, a.segments);
   if (block < 0) return;  // the whole workgroup
   P p;
-  p.template set<T>(a, block);
+  p.template set<T, APART>(a, block);
   const int64_t BN = a.B * a.N, first = a.seg * a.seg_steps;
   const int64_t end = first + a.seg_steps < a.T ? first + a.seg_steps : a.T;
   float s = p.in && a.state ? a.state[p.c()] : 0.0f;
@@ -294,15 +307,16 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void backward(Args a) {
     }
 #pragma unroll
     for (int i = kBackSteps - 1; i >= 0; --i) m = {m.A * ra[i], ra[i] * (rg[i] + m.H)};
-    maps[turn & 1][p.wave][p.lane] = m;
+    Affine(*const map)[kWave] = &maps[turn & 1][p.base];
+    map[p.wave][p.lane] = m;
     const int mine = n;
     if (tile > first) fetch(tile - p.tile_steps());
-    __syncthreads();
+    if (!APART) __syncthreads();
     float c = s;
 #pragma unroll 4
     for (int o = p.waves - 1; o >= 0; --o) {
       if (o == p.wave) c = s;
-      const Affine q = maps[turn & 1][o][p.lane];
+      const Affine q = map[o][p.lane];
       s = __builtin_fmaf(q.A, s, q.H);
     }
     const int64_t here = p.step(tile);
@@ -338,11 +352,11 @@ __global__ __launch_bounds__(kMaxWaves * kWave) void summarise(Args a) {
   using P = Place<STEPS>;
   __shared__ Affine maps[kTiles][kMaxWaves][kWave];
   __shared__ Affine whole[kTiles][kWave];
-  const int64_t block = locate(a, a.segments - 1);
+  const int64_t block = locate<false>(a, a.segments - 1);
   if (block < 0) return;  // the whole workgroup
   if (BACK) ++a.seg;      // the first needs none, as the last forward
   P p;
-  p.template set<T>(a, block);
+  p.template set<T, false>(a, block);
   const int64_t first = a.seg * a.seg_steps;
   const int64_t end = first + a.seg_steps < a.T ? first + a.seg_steps : a.T;
   const int tiles = static_cast<int>((end - first + p.tile_steps() - 1) / p.tile_steps());
@@ -430,6 +444,7 @@ int check(const char *what, int dtype, int64_t T, int64_t B, int64_t N) {
 struct Plan {
   int64_t blocks, segments, seg_steps;
   int waves;
+  bool apart;
 };
 
 // A CU holds 16 waves of these registers: its workgroups share them, so that none waits
@@ -440,6 +455,12 @@ struct Plan {
 // One wave to a workgroup of many: [200, 150, 2048] backward 151 -> 167.  LDS of the
 // waves' own size, so that two have 2 KB of it: 2 % slower everywhere.)
 //
+// Up to 64 steps of many channels, a wave goes over all of a block's time, beside three of
+// other blocks in its workgroup (APART): nothing is exchanged, and a CU does not run out of
+// LDS for workgroups of one.  [24, 700, 2048] bf16, forward and backward: 63 -> 56 us and
+// 92 -> 80, [8, 1024, 4096] 135 -> 92 and 122 -> 82; of 67 steps the backward pass is slower
+// so, 55 -> 61.
+//
 // Time is split where the channels leave half of the CUs without a workgroup: 128
 // blocks in two segments, [8192, 4, 2048] bf16: forward 142 us either way, backward
 // 276 -> 210; 175 blocks are faster whole (70 and 140 us, against 101 and 172).
@@ -448,8 +469,10 @@ Plan plan_of(int64_t T, int64_t B, int64_t N) {
   p.blocks = (B * N + kWave - 1) / kWave;
   const int64_t needed = (T + kSteps - 1) / kSteps;
   int waves = kMaxWaves;
-  while (waves > 2 && p.blocks * waves > 256 * kMaxWaves) waves /= 2;
+  const int least = needed > kApart ? 2 : 1;
+  while (waves > least && p.blocks * waves > 256 * kMaxWaves) waves /= 2;
   p.waves = static_cast<int>(needed < waves ? needed : waves);
+  p.apart = p.waves == 1 && p.blocks > 2048;
   const int64_t tile = p.waves * kSteps, tiles = (T + tile - 1) / tile;
   int64_t n = p.blocks > 128 ? 1 : 256 / p.blocks;
   if (n > tiles) n = tiles;
@@ -487,10 +510,13 @@ template <class E, bool BACK>
 void launch(const Args &a, const Plan &p, hipStream_t s) {
   const int threads = p.waves * kWave;
   if (p.segments > 1) summarise<E, BACK><<<grid_for(p.blocks * (p.segments - 1)), threads, 0, s>>>(a);
-  if (BACK)
-    backward<E><<<grid_for(p.blocks * p.segments), threads, 0, s>>>(a);
-  else
-    forward<E><<<grid_for(p.blocks * p.segments), threads, 0, s>>>(a);
+  if (p.apart) {
+    const dim3 grid = grid_for((p.blocks + kApart - 1) / kApart);
+    BACK ? backward<E, true><<<grid, kApart * kWave, 0, s>>>(a) : forward<E, true><<<grid, kApart * kWave, 0, s>>>(a);
+  } else {
+    const dim3 grid = grid_for(p.blocks * p.segments);
+    BACK ? backward<E, false><<<grid, threads, 0, s>>>(a) : forward<E, false><<<grid, threads, 0, s>>>(a);
+  }
 }
 
 }  // namespace

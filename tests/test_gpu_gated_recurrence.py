@@ -443,3 +443,11 @@ def test_workgroups_that_share_a_cu(T, B, N, dtype):
     each go over several tiles."""
 
     test_sequences_and_gradients(T, B, N, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,B,N", [(1, 3, 50001), (16, 70, 1999), (33, 131100, 1), (64, 33, 4003), (65, 33, 4003)])
+def test_few_steps_of_many_channels(T, B, N, dtype):
+    """A wave to 64 channels, up to 64 steps; the last workgroup has waves without any."""
+
+    test_sequences_and_gradients(T, B, N, dtype)
