@@ -459,11 +459,12 @@ struct Distilled {
   Tensor loss, probs, stats;
 };
 
-Distilled distillation_forward(const Tensor &x, const Tensor &values, const Tensor &tokens, double temperature,
-                               bool keep) {
+// rows x [R, V]; the loss in the shape `lead` of R rows
+Distilled distillation_forward(const Tensor &x, at::IntArrayRef lead, const Tensor &values, const Tensor &tokens,
+                               double temperature, bool keep) {
   const int64_t R = x.size(0), V = x.size(1), K = tokens.size(1);
   const auto f32s = x.options().dtype(torch::kFloat32);
-  Distilled d{torch::empty({R}, f32s), Tensor(), torch::empty({2, R}, f32s)};
+  Distilled d{torch::empty(lead, f32s), Tensor(), torch::empty({2, R}, f32s)};
   if (keep) d.probs = torch::empty({R, K}, f32s);
   const int64_t need = lib.distillation_workspace(R, V);
   Tensor ws;
@@ -475,10 +476,20 @@ Distilled distillation_forward(const Tensor &x, const Tensor &values, const Tens
   return d;
 }
 
+// [..., V] as rows [R, V] of unit stride
+Tensor distillation_rows(const Tensor &logits) {
+  const int64_t V = logits.size(-1);
+  const Tensor x = logits.dim() == 2 ? logits : logits.reshape({-1, V});
+  return (x.size(0) > 1 && x.stride(0) < V) || x.stride(1) != 1 ? x.contiguous() : x;
+}
+
+at::IntArrayRef lead_of(const Tensor &logits) { return logits.sizes().slice(0, logits.dim() - 1); }
+
 struct DistillationFunction : torch::autograd::Function<DistillationFunction> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &values, const Tensor &tokens,
+  static Tensor forward(AutogradContext *ctx, const Tensor &logits, const Tensor &values, const Tensor &tokens,
                         double temperature) {
-    const Distilled d = distillation_forward(x, values, tokens, temperature, true);
+    const Tensor x = distillation_rows(logits);
+    const Distilled d = distillation_forward(x, lead_of(logits), values, tokens, temperature, true);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({x, tokens, d.probs, d.stats});
     ctx->saved_data["temperature"] = temperature;
@@ -492,7 +503,9 @@ struct DistillationFunction : torch::autograd::Function<DistillationFunction> {
     const Tensor &x = saved[0], g = grads[0].contiguous();
     const int64_t R = x.size(0), V = x.size(1);
     const c10::DeviceGuard guard(x.device());
-    out[0] = torch::empty({R, V}, x.options());
+    std::vector<int64_t> shape = g.sizes().vec();
+    shape.push_back(V);
+    out[0] = torch::empty(shape, x.options());
     check(lib.distillation_bwd(at(x), code_of(x), x.stride(0), i64(saved[1]), f32(saved[2]), f32(saved[3]), f32(g),
                                static_cast<float>(ctx->saved_data["temperature"].toDouble()), at(out[0]), R, V,
                                static_cast<int>(saved[1].size(1)), stream_of(x)),
@@ -501,23 +514,28 @@ struct DistillationFunction : torch::autograd::Function<DistillationFunction> {
   }
 };
 
-// x with rows of unit stride, values [R, K] fp32 and tokens [R, K] int64 contiguous
-Tensor distillation_loss(const Tensor &x, const Tensor &values, const Tensor &tokens, double temperature) {
-  const c10::DeviceGuard guard(x.device());
-  if (needs({x})) return DistillationFunction::apply(x, values, tokens, temperature);
-  return distillation_forward(x, values, tokens, temperature, false).loss;
+Tensor distillation_loss(const Tensor &logits, const Tensor &teacher_logits, const Tensor &teacher_tokens,
+                         double temperature) {
+  const c10::DeviceGuard guard(logits.device());
+  const int64_t K = teacher_logits.size(-1);
+  const Tensor values = teacher_logits.reshape({-1, K}).to(torch::kFloat32).contiguous();
+  const Tensor tokens = teacher_tokens.reshape({-1, K}).to(torch::kInt64).contiguous();
+  if (needs({logits})) return DistillationFunction::apply(logits, values, tokens, temperature);
+  return distillation_forward(distillation_rows(logits), lead_of(logits), values, tokens, temperature, false).loss;
 }
 
 // ---- verification --------------------------------------------------------
-// {accepted, tokens}; probabilities with unit stride in their last dimension, the
-// others contiguous
-variable_list verify_draft(const Tensor &target, const OptTensor &draft, const Tensor &tokens, const Tensor &uniforms,
-                           const OptTensor &lengths) {
-  const c10::DeviceGuard guard(target.device());
+// {accepted, tokens}; lengths contiguous
+variable_list verify_draft(const Tensor &given_target, const OptTensor &given_draft, const Tensor &given_tokens,
+                           const Tensor &given_uniforms, const OptTensor &lengths) {
+  const c10::DeviceGuard guard(given_target.device());
+  const torch::NoGradGuard no_grad;
+  const Tensor target = unit_stride(given_target), uniforms = given_uniforms.contiguous();
+  const Tensor q = given_draft.has_value() ? unit_stride(*given_draft) : Tensor();
+  const Tensor tokens = given_tokens.to(torch::kInt64).contiguous();
   const int64_t n = target.size(0) - 1, B = target.size(1), V = target.size(2);
   const auto whole = target.options().dtype(torch::kInt64);
   Tensor accepted = torch::empty({B}, whole), out = torch::empty({n + 1, B}, whole);
-  const Tensor q = plain(draft);
   const int64_t need = lib.verify_workspace(B, V);
   Tensor ws;
   if (need) ws = torch::empty({need}, target.options().dtype(torch::kUInt8));

@@ -114,13 +114,12 @@ def distillation_loss(
     temperature = float(temperature)
     if not (2.0**-64 <= temperature <= 2.0**64):
         raise ValueError(f"temperature must be positive and finite, within 2**-64 and 2**64; got {temperature}")
+    if autograd.plain(logits):
+        return autograd.native().distillation_loss(logits, teacher_logits, teacher_tokens, temperature)
     values = teacher_logits.reshape(-1, K).float().contiguous()
     tokens = teacher_tokens.reshape(-1, K).to(torch.int64).contiguous()
     x = logits if logits.ndim == 2 else logits.reshape(-1, V)
     if (x.shape[0] > 1 and x.stride(0) < V) or x.stride(1) != 1:
         x = x.contiguous()
-    if autograd.plain(x):
-        loss = autograd.native().distillation_loss(x, values, tokens, temperature)
-    else:
-        loss = HipDistillationLossFunction.apply(x, values, tokens, temperature)
+    loss = HipDistillationLossFunction.apply(x, values, tokens, temperature)
     return loss if len(lead) == 1 else loss.view(lead)

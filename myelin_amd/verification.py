@@ -107,9 +107,9 @@ def verify_draft(
         if lengths.dtype == torch.int64:
             lengths = lengths.clamp(0, rows - 1).to(torch.int32)
         lengths = lengths.contiguous()
-    target = _rows(target_probs.detach())
-    draft = None if draft_probs is None else _rows(draft_probs.detach())
-    tokens, uniforms = draft_tokens.to(torch.int64).contiguous(), uniforms.detach().contiguous()
-    if autograd.plain(target, tokens, uniforms) and (draft is None or autograd.plain(draft)):
-        return VerifiedTokens(*autograd.native().verify_draft(target, draft, tokens, uniforms, lengths))
-    return VerifiedTokens(*_verify(target, draft, tokens, uniforms, lengths))
+    if autograd.plain(target_probs, draft_tokens, uniforms) and (draft_probs is None or autograd.plain(draft_probs)):
+        return VerifiedTokens(*autograd.native().verify_draft(target_probs, draft_probs, draft_tokens, uniforms,
+                                                              lengths))
+    return VerifiedTokens(*_verify(
+        _rows(target_probs.detach()), None if draft_probs is None else _rows(draft_probs.detach()),
+        draft_tokens.to(torch.int64).contiguous(), uniforms.detach().contiguous(), lengths))

@@ -203,3 +203,31 @@ def test_the_same_bits_on_every_run():
     want = _everything(xs)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(_everything(xs), want))
+
+
+def test_losses_in_the_rows_shape_may_be_changed_in_place():
+    g = torch.Generator().manual_seed(3)
+    logits, teacher = torch.randn(4, 3, 50, generator=g), torch.randn(4, 3, 5, generator=g)
+    tokens = torch.randint(0, 50, (4, 3, 5), generator=g).to(DEV)
+    mask = (torch.arange(12) % 3 > 0).float().view(4, 3).to(DEV)
+    for lead in ((4, 3), (12,), (2, 2, 3), (4, 3, 1)):
+        x = logits.to(DEV).view(*lead, 50).clone().requires_grad_()
+        loss = myelin.distillation_loss(x, teacher.to(DEV).view(*lead, 5), tokens.view(*lead, 5))
+        assert loss.shape == lead
+        loss.mul_(mask.view(lead))
+        loss.sum().backward()
+        y = logits.to(DEV).view(12, 50).clone().requires_grad_()
+        rows = myelin.distillation_loss(y, teacher.to(DEV).view(12, 5), tokens.view(12, 5))
+        rows.backward(mask.view(12))
+        assert torch.equal(x.grad.view(12, 50), y.grad)
+    one = logits[0, 0].to(DEV).requires_grad_()
+    loss = myelin.distillation_loss(one, teacher[0, 0].to(DEV), tokens[0, 0])
+    assert loss.shape == ()
+    loss.backward()
+    assert one.grad.shape == (50,)
+    # rows that are not one after the other in memory
+    wide = logits.to(DEV).transpose(0, 1).clone().transpose(0, 1).requires_grad_()
+    myelin.distillation_loss(wide, teacher.to(DEV), tokens).sum().backward()
+    flat = logits.to(DEV).requires_grad_()
+    myelin.distillation_loss(flat, teacher.to(DEV), tokens).sum().backward()
+    assert torch.equal(wide.grad, flat.grad)
