@@ -123,6 +123,43 @@ struct Seen {
   }
 };
 
+// What the places of this lane's token have, added up in their order, where place k is
+// the first of them, and 0 elsewhere; a lane without such a token has -1.  The places of
+// tokens that have met (among the 64 of each bit of `met`) come past all lanes one at a
+// time, at most K^2 / 64 of them for a row, until each lane knows of a place before its
+// own.  Each place looked for and added up by itself took K^2: 4 rows of 1024 places of
+// one token 50 ms -> 0.10, of two places to a token 2.9 ms -> 0.60; 2048 rows of 64 places
+// of one token 302 us -> 57, as of different ones.
+template <int BITS>
+__device__ __forceinline__ float together(const Args &a, int64_t first, uint32_t met, int token, int k, float peak,
+                                          float total, const Seen<BITS> &seen) {
+  constexpr int kSome = 28;  // of 64: 60 ns each; past that all of them, 1.8 us
+  const int lane = threadIdx.x & (kWave - 1);
+  bool later = token < 0;
+  float sum = 0.0f;
+  for (uint32_t m = met; m && __any(!later); m &= m - 1) {
+    const int from = __builtin_ctz(m) * kWave, o = from + lane, before = k - from;
+    const int64_t other = o < a.K ? a.tokens[first + o] : -1;
+    const float value = o < a.K ? a.values[first + o] : 0.0f;
+    const bool there = !empty(other, value) && seen.met(other);
+    const int name = there ? static_cast<int>(other) : -2;
+    const int v = __builtin_bit_cast(int, there ? myelin::exp_f32((value - peak) * a.rate) / total : 0.0f);
+    const auto pass = [&](int i) {
+      const bool same = __builtin_amdgcn_readlane(name, i) == token;
+      later |= same && i < before;
+      sum += same ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(v, i)) : 0.0f;
+    };
+    uint64_t s = __ballot(there);
+    if (__builtin_popcountll(s) > kSome) {
+#pragma unroll
+      for (int i = 0; i < kWave; ++i) pass(i);
+    } else {
+      for (; s; s &= s - 1) pass(__builtin_ctzll(s));
+    }
+  }
+  return later ? 0.0f : sum;
+}
+
 // The row's loss from its logits' statistics, by one wave.
 template <class E, int BITS>
 __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int lane, Seen<BITS> &seen) {
@@ -139,12 +176,18 @@ __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int 
     if (a.probs) seen.add(token);
   }
   for (int o = kWave >> 1; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o));
-  float total = 0.0f;
-  for (int k = lane; k < a.K; k += kWave)
-    if (!empty(a.tokens[first + k], a.values[first + k]))
-      total += myelin::exp_f32((a.values[first + k] - peak) * a.rate);
-  total = wave_sum(total);
   bad = __any(bad);
+  float total = 0.0f;
+  uint32_t met = 0;  // the 64 places with tokens that have met
+  for (int at = 0; at < a.K; at += kWave) {
+    const int k = at + lane;
+    const int64_t token = k < a.K ? a.tokens[first + k] : -1;
+    const float value = k < a.K ? a.values[first + k] : 0.0f;
+    const bool there = !empty(token, value);
+    if (there) total += myelin::exp_f32((value - peak) * a.rate);
+    if (a.probs && !bad && __any(there && seen.met(token))) met |= 1u << (at / kWave);
+  }
+  total = wave_sum(total);
   const float log_total = logf(total), log_s = t.s == 0.0f ? -kInf : logf(t.s);
   float loss = 0.0f;
   for (int at = 0; at < a.K; at += kWave) {
@@ -163,22 +206,10 @@ __device__ __forceinline__ void finish(const Args &a, int64_t row, Stats t, int 
       }
     }
     if (!a.probs) continue;
-    // what the places of a token have, in their order, goes to the first of them
-    for (uint64_t m = __ballot(there && seen.met(token)); m; m &= m - 1) {
-      const int one = __builtin_ctzll(m);
-      const int64_t name = __shfl(token, one);
-      int place = -1;
-      float sum = 0.0f;
-      for (int from = 0; from < a.K; from += kWave) {
-        const int o = from + lane;
-        const bool same = o < a.K && a.tokens[first + o] == name && a.values[first + o] != -kInf;
-        const float v = same ? myelin::exp_f32((a.values[first + o] - peak) * a.rate) / total : 0.0f;
-        for (uint64_t s = __ballot(same); s; s &= s - 1) {
-          if (place < 0) place = from + __builtin_ctzll(s);
-          sum += __shfl(v, __builtin_ctzll(s));
-        }
-      }
-      if (lane == one) p = place == k ? sum : 0.0f;
+    if (met >> (at / kWave) & 1) {
+      const bool mine = there && seen.met(token);
+      const float sum = together(a, first, met, mine ? static_cast<int>(token) : -1, k, peak, total, seen);
+      if (mine) p = sum;
     }
     if (k < a.K) a.probs[first + k] = p;
   }
