@@ -21,6 +21,7 @@ using myelin::F32;
 using myelin::kWave;
 
 constexpr int kThreads = 256;
+constexpr int64_t kNoPadding = INT64_MIN;  // no token is padding, this one neither
 
 struct Args {
   const int64_t *tokens;
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(kThreads) void lookup(Args a, int per) {
 #pragma unroll
   for (int o = 0; o < kRows; ++o) {
     if (i[o] >= a.M) continue;
-    const bool hole = token[o] == a.padding, outside = token[o] < 0 || token[o] >= a.V;
+    const bool hole = a.padding != kNoPadding && token[o] == a.padding, outside = token[o] < 0 || token[o] >= a.V;
 #pragma unroll
     for (int q = 0; q < VEC; ++q) r[o].v[q] = hole ? 0.0f : outside ? __builtin_nanf("") : r[o].v[q];
     r[o].template store<STREAM>(static_cast<T *>(a.to) + i[o] * a.D + column<VEC>(a, u), a.scale);

@@ -13,7 +13,7 @@ from myelin_amd import _lib, autograd
 from myelin_amd.packing import _device_of
 
 _TYPES = (torch.float32, torch.bfloat16)
-NO_PADDING = -(2**63)  # no token has this number
+NO_PADDING = -(2**63)  # for the kernels: no token is padding, this one neither
 
 
 def _forward(tokens, weight, scale, padding):
@@ -64,9 +64,9 @@ def token_embedding(
     """``scale * weight[tokens]``, a float32 product rounded to the weight's type: ``[..., D]``.
 
     ``tokens [...]`` int64 or int32, ``weight [V, D]`` float32 or bfloat16.  Tokens
-    equal to ``padding_index`` (any number, also one outside the table) give zeros
-    and no gradient; any other token outside ``[0, V)`` gives a row of NaN and no
-    gradient (nothing is read out of range).
+    equal to ``padding_index`` (any number above -2^63, also one outside the table)
+    give zeros and no gradient; any other token outside ``[0, V)`` gives a row of NaN
+    and no gradient (nothing is read out of range).
 
     Differentiable in the weight.  A row's gradient is the float32 sum over its tokens,
     in an order that their positions alone decide (the same bits on every run),
