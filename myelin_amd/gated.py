@@ -134,9 +134,10 @@ def gated_recurrence(
     Returns ``(final state [B, N] float32, out [T, B, N])``, differentiable in x,
     the gate and the initial state.  States and sums are float32.
 
-    An infinity or a NaN of a step makes the results that it is part of (of its own
-    step and later ones; of gradients, its own step and earlier ones) infinite or
-    NaN, and no others.
+    An infinity or a NaN makes the results that it is part of infinite or NaN, and no
+    others: of ``x``, a gate or the initial state, the states from its step on and the
+    gates' gradients from there on; of a gate (NaN) or an incoming gradient, the
+    gradients of its own step and earlier ones.
     """
 
     _check(x, gate, 3, "[T, B, N]")
