@@ -703,8 +703,10 @@ int myelin_decay_attention_step(const void *q, const void *k, const void *v,
  * last dimension and element strides of t and b in `strides` (host memory: x's
  * two, gate's, and for the backward pass grad_out's); states [B, N] contiguous
  * fp32, state NULL for zeros; lengths [B] int32 or NULL: steps of each batch row
- * (taken into [0, T]); later steps keep the state and give 0, and their inputs
- * are not read.  out, grad_x and grad_gate are contiguous in x's type.
+ * (taken into [0, T]); later steps keep the state and give 0, and no result
+ * depends on their inputs, which have to be there all the same: all T rows of x,
+ * gate and grad_out may be read.  out, grad_x and grad_gate are contiguous in x's
+ * type.
  * kept (or NULL): myelin_gated_recurrence_kept_elems floats (host only) that the
  * forward pass writes for the backward pass.  That takes grad_out and
  * grad_state_out (either may be NULL) and writes grad_x, grad_gate and

@@ -129,7 +129,8 @@ def gated_recurrence(
     ``initial_state [B, N]`` float32 (zeros by default).
 
     ``lengths [B]`` (int32 or int64 on the device, taken into [0, T]) gives each
-    sample's steps: later ones are not read, leave the state and give zeros.
+    sample's steps: later ones are part of no result, leave the state and give zeros
+    (their memory may be read; what it holds, NaN too, does not count).
 
     Returns ``(final state [B, N] float32, out [T, B, N])``, differentiable in x,
     the gate and the initial state.  States and sums are float32.
