@@ -128,12 +128,12 @@ struct Seen {
 // tokens that have met (among the 64 of each bit of `met`) come past all lanes one at a
 // time, at most K^2 / 64 of them for a row, until each lane knows of a place before its
 // own.  Each place looked for and added up by itself took K^2: 4 rows of 1024 places of
-// one token 50 ms -> 0.10, of two places to a token 2.9 ms -> 0.60; 2048 rows of 64 places
-// of one token 302 us -> 57, as of different ones.
+// one token 50 ms -> 0.12, of two places to a token 2.9 ms -> 0.66; 2048 rows of 40000 and 64
+// places of one token 302 us -> 60, 56 of different ones.
 template <int BITS>
 __device__ __forceinline__ float together(const Args &a, int64_t first, uint32_t met, int token, int k, float peak,
                                           float total, const Seen<BITS> &seen) {
-  constexpr int kSome = 28;  // of 64: 60 ns each; past that all of them, 1.8 us
+  constexpr int kSome = 28;  // of 64: 60 ns each; past that all of them, 2 us
   const int lane = threadIdx.x & (kWave - 1);
   bool later = token < 0;
   float sum = 0.0f;
@@ -151,7 +151,7 @@ __device__ __forceinline__ float together(const Args &a, int64_t first, uint32_t
     };
     uint64_t s = __ballot(there);
     if (__builtin_popcountll(s) > kSome) {
-#pragma unroll
+#pragma unroll 16  // (whole, it takes 100 registers, and 8 waves a SIMD have 64)
       for (int i = 0; i < kWave; ++i) pass(i);
     } else {
       for (; s; s &= s - 1) pass(__builtin_ctzll(s));
