@@ -62,7 +62,6 @@ struct Weights {
   using T = typename E::T;
   const T *p, *q;  // q null: p alone, less `without`
   int64_t without;
-  __device__ double of_p(int64_t i) const { return positive(E::get(p[i])); }
   __device__ double operator()(int64_t i) const {
     const double w = E::get(p[i]);
     if (q) return positive(w - static_cast<double>(E::get(q[i])));
