@@ -745,8 +745,9 @@ int myelin_gated_recurrence_step(const void *x, const void *gate, int dtype,
  * (fp32) or 2 (bf16), out [M, D] contiguous in its type.  A token equal to
  * padding (INT64_MIN: none is) gives zeros; any other outside [0, V) gives NaN.
  * The backward pass writes the whole of grad_weight [V, D], contiguous, from
- * grad_out [M, D], contiguous: fp32 sums over each token's positions in order,
- * scaled and rounded once; padding and tokens outside the table give nothing.
+ * grad_out [M, D], contiguous: fp32 sums over each token's positions, grouped in a
+ * way that the positions alone decide, scaled and rounded once; padding and tokens
+ * outside the table give nothing.
  * workspace: myelin_token_embedding_bwd_workspace_bytes (host only), 16-byte
  * aligned.
  * No counterpart in myelin.

@@ -4,11 +4,13 @@
 //
 // A padding token's row is 0 and has no gradient; a token outside [0, V) gives a
 // row of NaN and has none either: nothing is read out of range.  The sums are
-// fp32, in an order that the positions alone decide: the same bits on every run.
+// fp32, of groups of a token's positions that the positions alone decide, and of those
+// groups in their order: the same bits on every run.
 //
 // The gradient takes the positions in the order of their tokens (a stable sort), so
-// that each row of the table is written once, by the threads that sum it, and
-// nothing is atomic.  A token may have a tenth of all positions: a run of equal
+// that each row of the table is written once, by the threads that sum it, and nothing
+// in memory is atomic (the sort's whole numbers are counted with atomics in LDS, whose
+// order does not show).  A token may have a tenth of all positions: a run of equal
 // tokens is cut at multiples of 32 sorted positions, whole pieces are summed by
 // workgroups of their own, and the row's threads add up what is left.
 
@@ -574,8 +576,8 @@ struct Layout {  // of the workspace, in bytes
   int64_t stretch, keys[2], places[2], counts, starts, pieces, pieces2, size;
 };
 
-// Rows of the table times slices that sum_few is taken for: each goes through all
-// tokens.
+// Rows of the table, times D / 64 where they are wider, that sum_few is taken for: each
+// goes through all tokens.
 constexpr int64_t kFewRows = 2048;
 
 // Positions times slices of 128 threads (so that a group of threads has at most 512 rows,
