@@ -571,7 +571,7 @@ __global__ __launch_bounds__(kThreads) void zeros(Args a) {
 
 // ---- launches ---------------------------------------------------------------
 struct Layout {  // of the workspace, in bytes
-  bool few;
+  bool few, positions;  // a workgroup to a row, to a position: none
   int passes, bits, blocks;
   int64_t stretch, keys[2], places[2], counts, starts, pieces, pieces2, size;
 };
@@ -585,10 +585,13 @@ constexpr int64_t kFewRows = 2048;
 // bf16 16 -> 6 us, 1024 of [32000, 512] 27 -> 16, 2048 30 -> 23, 4096 32 -> 42.
 constexpr int64_t kFewPositions = 2048;
 
-Layout layout_of(int64_t M, int64_t V, int64_t D) {
+// vec: elements of a thread's vector
+Layout layout_of(int64_t M, int64_t V, int64_t D, int vec) {
   Layout l{};
   l.few = M <= kFew && V * ((D + 63) / 64) <= kFewRows;
-  if (l.few || M == 0) return l;
+  const int64_t units = (D + vec - 1) / vec, some = threads_of(units, 2 * kWave);
+  l.positions = !l.few && M * ((units + some - 1) / some) <= kFewPositions;
+  if (l.few || l.positions || M == 0) return l;
   int bits = 1;
   while (V >> bits) ++bits;
   l.passes = (bits + kDigit - 1) / kDigit;
@@ -650,7 +653,7 @@ void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
     sum_few<E, VEC, false><<<myelin::grid_of(a.V * a.slices), kFewThreads, 0, s>>>(a, some);
     return;
   }
-  if (a.M * a.slices <= kFewPositions) {
+  if (l.positions) {
     zero();
     sum_few<E, VEC, true><<<myelin::grid_of(a.M * a.slices), kFewThreads, 0, s>>>(a, some);
     return;
@@ -704,6 +707,11 @@ void launch_gradient(Args &a, const Layout &l, char *ws, hipStream_t s) {
     sum_runs<E, VEC, kTableRows, false><<<grid(groups * kTableRows), kThreads, 0, s>>>(a, per);
 }
 
+int vector_of(int dtype, int64_t D) {
+  const int vec = dtype == 0 ? F32::VEC : BF16::VEC;
+  return D >= vec ? vec : 1;
+}
+
 int check(const char *what, int dtype, int64_t M, int64_t V, int64_t D, float scale) {
   if (dtype != 0 && dtype != 2) return myelin::invalid("%s: unsupported dtype %d", what, dtype);
   if (M < 0 || V < 1 || D < 1) return myelin::invalid("%s: V and D must be positive, M not negative", what);
@@ -728,15 +736,18 @@ extern "C" int myelin_token_embedding(const int64_t *tokens, const void *weight,
   a.tokens = tokens, a.from = weight, a.to = out, a.ld = ld, a.M = M, a.V = V, a.D = D;
   a.padding = padding, a.scale = scale;
   hipStream_t s = myelin::as_hip(stream);
+  const bool vector = vector_of(dtype, D) > 1;
   if (dtype == 0)
-    D >= F32::VEC ? launch_lookup<F32, F32::VEC>(a, s) : launch_lookup<F32, 1>(a, s);
+    vector ? launch_lookup<F32, F32::VEC>(a, s) : launch_lookup<F32, 1>(a, s);
   else
-    D >= BF16::VEC ? launch_lookup<BF16, BF16::VEC>(a, s) : launch_lookup<BF16, 1>(a, s);
+    vector ? launch_lookup<BF16, BF16::VEC>(a, s) : launch_lookup<BF16, 1>(a, s);
   return myelin::launched(what);
 }
 
 extern "C" int64_t myelin_token_embedding_bwd_workspace_bytes(int64_t M, int64_t V, int64_t D) {
-  return M < 1 || V < 1 || D < 1 ? 0 : layout_of(M, V, D).size;
+  if (M < 1 || V < 1 || D < 1) return 0;
+  const int64_t f32 = layout_of(M, V, D, vector_of(0, D)).size, bf16 = layout_of(M, V, D, vector_of(2, D)).size;
+  return f32 > bf16 ? f32 : bf16;
 }
 
 extern "C" int myelin_token_embedding_bwd(const int64_t *tokens, const void *grad_out, int dtype, void *grad_weight,
@@ -745,7 +756,7 @@ extern "C" int myelin_token_embedding_bwd(const int64_t *tokens, const void *gra
   const char *what = "token_embedding_bwd";
   if (int rc = check(what, dtype, M, V, D, scale)) return rc;
   if (!grad_weight || (M > 0 && (!tokens || !grad_out))) return myelin::invalid("%s: null pointer", what);
-  const Layout l = layout_of(M, V, D);
+  const Layout l = layout_of(M, V, D, vector_of(dtype, D));
   if (l.size) {
     if (!workspace || workspace_bytes < l.size)
       return myelin::invalid("%s: workspace of %lld bytes needed", what, static_cast<long long>(l.size));
@@ -755,10 +766,11 @@ extern "C" int myelin_token_embedding_bwd(const int64_t *tokens, const void *gra
   a.tokens = tokens, a.from = grad_out, a.to = grad_weight, a.ld = D, a.M = M, a.V = V, a.D = D;
   a.padding = padding, a.scale = scale;
   hipStream_t s = myelin::as_hip(stream);
+  const bool vector = vector_of(dtype, D) > 1;
   char *ws = static_cast<char *>(workspace);
   if (dtype == 0)
-    D >= F32::VEC ? launch_gradient<F32, F32::VEC>(a, l, ws, s) : launch_gradient<F32, 1>(a, l, ws, s);
+    vector ? launch_gradient<F32, F32::VEC>(a, l, ws, s) : launch_gradient<F32, 1>(a, l, ws, s);
   else
-    D >= BF16::VEC ? launch_gradient<BF16, BF16::VEC>(a, l, ws, s) : launch_gradient<BF16, 1>(a, l, ws, s);
+    vector ? launch_gradient<BF16, BF16::VEC>(a, l, ws, s) : launch_gradient<BF16, 1>(a, l, ws, s);
   return myelin::launched(what);
 }

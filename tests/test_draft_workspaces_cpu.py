@@ -67,3 +67,15 @@ def test_verification():
         assert n == B * -(-V // 1024) * 16
         _refused("myelin_verify_draft", [16, None, 0, 16, 16, 16, None, 16, 16, 3, B, V], n)
     assert need(0, 10) == 0 and need(3, 0) == 0
+
+
+def test_embedding_of_few_positions():
+    """A workgroup to a position needs nothing either; a wide row's slices count."""
+
+    need = _lib.load().myelin_token_embedding_bwd_workspace_bytes
+    for M, V, D in ((60, 5407, 26), (1024, 32000, 512), (2048, 100000, 1), (512, 150000, 2048)):
+        assert need(M, V, D) == 0
+    for M, V, D in ((2049, 100000, 1), (1025, 32000, 1024), (4096, 32000, 512)):
+        n = need(M, V, D)
+        assert n >= 16 * M
+        _refused("myelin_token_embedding_bwd", [16, 16, 0, 16, M, V, D, 1.0, 0], n)
